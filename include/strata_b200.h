@@ -44,7 +44,8 @@ int strata_abi_version(void);
 const char* strata_error_string(int code);
 
 /* Reads (and, if reset != 0, clears) the device status word of the current device.
- * Synchronises the device. *h_status: 0 = ok, 101..105 = a bounded wait timed out. */
+ * Synchronises the device. *h_status: 0 = ok, 101..105 = a bounded wait timed out, 107 = a position given to
+ * strata_qk_norm_rope lies behind its table. */
 int strata_device_status(int* h_status, int reset);
 
 /* Non-affine LayerNorm over channels: y[m,:] = (x[m,:] - mean) * rsqrt(var + eps).
@@ -60,6 +61,42 @@ int strata_layernorm_bf16(const void* x, int64_t ldx, void* y, int64_t ldy, int 
 int strata_linear_bf16(const void* x, int64_t ldx, const void* w, int64_t ldw, const float* bias,
                        void* y, int64_t ldy, int M, int N, int K, int epilogue, const void* aux,
                        int64_t ldaux, void* stream);
+
+/* Element types of the dense layer and of strata_qk_norm_rope. */
+#define STRATA_BF16 0
+#define STRATA_F16 1
+
+/* Activations of strata_linear_act. */
+#define STRATA_ACT_NONE 0
+#define STRATA_ACT_GELU 1      /* z Phi(z) */
+#define STRATA_ACT_GELU_TANH 2 /* its tanh form, with the hardware's tanh as STRATA_EPI_GELU */
+#define STRATA_ACT_SILU 3
+#define STRATA_ACT_RELU 4
+
+/* Dense layer: y[M,N] = residual + act(z), z = x[M,K] W[N,K]^T + bias, any M, N, K and row strides; x, W, residual, y
+ * and preact are of one 16-bit type (dtype), bias fp32; sums and the epilogue are fp32, y is rounded once. residual,
+ * bias and preact may be NULL; preact receives z, which the backward pass needs for any activation. y may be residual
+ * (same stride), nothing else may overlap.
+ * workspace: 256-byte aligned, of strata_linear_act_workspace_bytes(M, N, K, x_aligned, w_aligned) bytes (negative: an
+ * error code), where an operand counts as aligned when its address and its row stride are multiples of 16 bytes (others
+ * are copied there first). Up to 8 rows are one launch without workspace; M = 0 does nothing. Replaces the nn.Linear
+ * calls of a block together with the operators around them (attn.proj, mlp.layers.*) in fine-tuning. */
+int64_t strata_linear_act_workspace_bytes(int M, int N, int K, int x_aligned, int w_aligned);
+int strata_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const float* bias, const void* residual,
+                      int64_t ldr, void* y, int64_t ldy, void* preact, int64_t ldz, int M, int N, int K, int activation,
+                      int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Its gradients, from dy[M,N] and the stored z (preact; unused for STRATA_ACT_NONE):
+ *   dz = dy act'(z), dx[M,K] = dz W, dW[N,K] = dz^T x, db[N] = sum over the rows of dz (fp32).
+ * Outputs that are NULL are not computed, and x (w) may be NULL without dw (dx). dz is rounded to the 16-bit type in
+ * front of the two products (not for db, and not without an activation). No atomics: the same bits every time. M = 0
+ * sets dW and db to zero. Workspace as above. */
+int64_t strata_linear_act_backward_workspace_bytes(int M, int N, int K, int activation, int dy_aligned, int z_aligned,
+                                                   int x_aligned, int w_aligned, int need_dx, int need_dw, int need_db);
+int strata_linear_act_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, int64_t ldw,
+                               const void* preact, int64_t ldz, void* dx, int64_t lddx, void* dw, int64_t lddw,
+                               float* db, int M, int N, int K, int activation, int dtype, void* workspace,
+                               int64_t workspace_bytes, void* stream);
 
 /* y[M,C] = aux + [gate *] (W2 gelu(W1 x + b1) + b2): the MLP of a narrow block in one kernel, same bits as
  * strata_linear_bf16 with STRATA_EPI_GELU and then with STRATA_EPI_RESIDUAL (aux, no gate), STRATA_EPI_BIAS (neither)
@@ -262,6 +299,38 @@ int strata_adaln_rows_bf16(const void* x, int64_t ldx, const void* y, int64_t ld
 /* In-place RMS norm of the q and k heads (64 channels each) of packed rows [M, 3C]
  * (qk_norm_pixel of screamcast/strata_wrappers.py:437, non-affine). */
 int strata_qk_norm_rows_bf16(void* qkv, int64_t ld, int64_t M, int C, float eps, void* stream);
+
+/* q and k heads of M tokens, one entry for each: element (m, head, c) at base + m*stride_token + head*stride_head + c,
+ * strides in elements, multiples of 8; bases 16-byte aligned. */
+typedef struct strata_heads {
+  void* data;
+  int64_t stride_token, stride_head;
+} strata_heads;
+
+/* Per-head RMS norm and rotation of q and k in one pass: y = R (x (mean x^2 + eps)^-1/2 w), for `heads_q` and `heads_k`
+ * heads of head_dim channels (a multiple of 8, at most 256) in one 16-bit type. w_q, w_k: [head_dim] fp32 or NULL.
+ * R turns the first `rot` channels of a head by the (cos, sin) pairs of the token's row of table [table_rows, rot/2]
+ * (IEEE half, or float with table_f32; 16-byte aligned; NULL: no rotation): pairs (2i, 2i+1) with `adjacent`, rot a
+ * multiple of 8, else (i, i + rot/2), rot a multiple of 16. The row is positions[m] (int32, or int64 with
+ * positions_64); without positions m / tokens_per_tile * hw + m % hw, which has to stay below table_rows. A negative
+ * position is padding: its outputs are zero. One behind the table gives NaN and device status 107. y may be x.
+ * The q/k norm and rotation of strata_qkv_rope_bf16 and strata_qk_norm_rows_bf16 for projections made elsewhere, with
+ * affine weights, shared key heads and other widths. */
+int strata_qk_norm_rope(const strata_heads* h_q, const strata_heads* h_k, const strata_heads* h_q_out,
+                        const strata_heads* h_k_out, const float* w_q, const float* w_k, int heads_q, int heads_k,
+                        int head_dim, int rot, int adjacent, const void* table, int table_f32, int table_rows,
+                        const void* positions, int positions_64, int tokens_per_tile, int hw, int64_t M, float eps,
+                        int dtype, void* stream);
+/* Its gradients from dq, dk: dx of q and k, and dw_q, dw_k [head_dim] fp32 (NULL where there are no weights). dw is
+ * summed without atomics: the same bits every time. workspace: strata_qk_norm_rope_backward_workspace_bytes bytes,
+ * 16-byte aligned (NULL without dw). */
+int64_t strata_qk_norm_rope_backward_workspace_bytes(int64_t M, int heads, int head_dim);
+int strata_qk_norm_rope_backward(const strata_heads* h_dq, const strata_heads* h_dk, const strata_heads* h_q,
+                                 const strata_heads* h_k, const strata_heads* h_dq_in, const strata_heads* h_dk_in,
+                                 const float* w_q, const float* w_k, float* dw_q, float* dw_k, int heads_q, int heads_k,
+                                 int head_dim, int rot, int adjacent, const void* table, int table_f32, int table_rows,
+                                 const void* positions, int positions_64, int tokens_per_tile, int hw, int64_t M,
+                                 float eps, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Conditioning rows of the "bilinear_dw" AdaLN mode (screamcast/strata_wrappers.py:491-495;
  * parameters adaln_bilinear_dw_conv.{weight,bias} of the parameter manifest

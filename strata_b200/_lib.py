@@ -24,6 +24,11 @@ class BlockWeights(Structure):
                                         "w_fc1", "b_fc1", "w_fc2", "b_fc2")]
 
 
+class Heads(Structure):
+    """struct strata_heads (a device pointer and two element strides)."""
+    _fields_ = [("data", c_void_p), ("stride_token", c_int64), ("stride_head", c_int64)]
+
+
 class BackboneDesc(Structure):
     """struct strata_backbone_desc."""
     _fields_ = ([(n, c_int32) for n in ("in_channels", "out_channels", "patch_v", "patch_h", "patch_w",
@@ -60,6 +65,14 @@ _SIGNATURES = {
     "strata_linear_bf16": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
                                    c_int64, c_int, c_int, c_int, c_int, c_void_p, c_int64,
                                    c_void_p]),
+    "strata_linear_act_workspace_bytes": (c_int64, [c_int] * 5),
+    "strata_linear_act": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64,
+                                  c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int64,
+                                  c_void_p]),
+    "strata_linear_act_backward_workspace_bytes": (c_int64, [c_int] * 11),
+    "strata_linear_act_backward": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64,
+                                           c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_int,
+                                           c_int, c_void_p, c_int64, c_void_p]),
     "strata_mlp_fused": (c_int, [c_int, c_int, c_int]),
     "strata_mlp_bf16": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
                                 c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int, c_void_p]),
@@ -104,6 +117,13 @@ _SIGNATURES = {
                                        c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p,
                                        c_int64, c_int, c_int, c_float, c_void_p]),
     "strata_qk_norm_rows_bf16": (c_int, [c_void_p, c_int64, c_int64, c_int, c_float, c_void_p]),
+    "strata_qk_norm_rope": (c_int, [POINTER(Heads)] * 4 + [c_void_p] * 2 + [c_int] * 5
+                            + [c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_int, c_int64, c_float, c_int,
+                               c_void_p]),
+    "strata_qk_norm_rope_backward_workspace_bytes": (c_int64, [c_int64, c_int, c_int]),
+    "strata_qk_norm_rope_backward": (c_int, [POINTER(Heads)] * 6 + [c_void_p] * 4 + [c_int] * 5
+                                     + [c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_int, c_int64, c_float, c_int,
+                                        c_void_p, c_int64, c_void_p]),
     "strata_adaln_cond_bf16": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,
                                        c_void_p, c_void_p, c_int, c_int64, c_int64, c_void_p,
                                        c_void_p, c_void_p]),

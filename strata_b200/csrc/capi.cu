@@ -17,6 +17,8 @@
 #include "prepost.cuh"
 #include "adaln.cuh"
 #include "geometry.cuh"
+#include "dense.cuh"
+#include "qk_norm_rope.cuh"
 
 using namespace strata;
 
@@ -132,6 +134,94 @@ int strata_linear_bf16(const void* x, int64_t ldx, const void* w, int64_t ldw, c
     case STRATA_EPI_GATE: return launch_gemm<EPI_GATE>(A, ldx, W, ldw, p, sms, st);
     default: return STRATA_ERR_UNSUPPORTED;
   }
+}
+
+// Sizes that the dense layer's kernels index with 32 bits.
+static bool dense_sizes(int M, int N, int K, int act, int dtype) {
+  constexpr int kMost = 0x7FFF0000;
+  return M >= 0 && N > 0 && K > 0 && M <= kMost && N <= kMost && K <= kMost && act >= 0 && act < ACT_COUNT &&
+         (dtype == STRATA_BF16 || dtype == STRATA_F16);
+}
+static bool dense_rows_ok(const void* p, int64_t ld, int cols) {
+  return p != nullptr && ld >= cols && (reinterpret_cast<uintptr_t>(p) & 1u) == 0;
+}
+
+int64_t strata_linear_act_workspace_bytes(int M, int N, int K, int x_aligned, int w_aligned) {
+  const int sms = current_sm_count();
+  if (sms <= 0) return STRATA_ERR_NO_DEVICE;
+  if (!dense_sizes(M, N, K, 0, 0)) return STRATA_ERR_ARG;
+  return dense_forward_bytes(M, N, K, x_aligned != 0, w_aligned != 0, sms);
+}
+
+int strata_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const float* bias, const void* residual,
+                      int64_t ldr, void* y, int64_t ldy, void* preact, int64_t ldz, int M, int N, int K, int activation,
+                      int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  const int sms = current_sm_count();
+  if (sms <= 0) return STRATA_ERR_NO_DEVICE;
+  if (!dense_sizes(M, N, K, activation, dtype)) return STRATA_ERR_ARG;
+  if (M == 0) return STRATA_OK;
+  if (!dense_rows_ok(x, ldx, K) || !dense_rows_ok(w, ldw, K) || !dense_rows_ok(y, ldy, N) ||
+      (residual && !dense_rows_ok(residual, ldr, N)) || (preact && !dense_rows_ok(preact, ldz, N)) ||
+      (reinterpret_cast<uintptr_t>(bias) & 3u) != 0)
+    return STRATA_ERR_ARG;
+  const int64_t need = dense_forward_bytes(M, N, K, dense_aligned(x, ldx), dense_aligned(w, ldw), sms);
+  if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0))
+    return STRATA_ERR_ARG;
+  DenseParams p{};
+  p.M = M; p.N = N; p.K = K;
+  p.out = y; p.ldo = ldy;
+  p.keep = preact; p.ldk = ldz;
+  p.aux = residual; p.ldaux = ldr;
+  p.bias = bias;
+  p.act = activation;
+  p.fp16 = dtype == STRATA_F16;
+  p.direct = !dense_whole(y, ldy, N) || (preact && !dense_whole(preact, ldz, N)) ||
+             (residual && !dense_aligned(residual, ldr));
+  return launch_dense_forward({x, ldx}, {w, ldw}, p, workspace, sms, as_stream(stream));
+}
+
+int64_t strata_linear_act_backward_workspace_bytes(int M, int N, int K, int activation, int dy_aligned, int z_aligned,
+                                                   int x_aligned, int w_aligned, int need_dx, int need_dw,
+                                                   int need_db) {
+  const int sms = current_sm_count();
+  if (sms <= 0) return STRATA_ERR_NO_DEVICE;
+  if (!dense_sizes(M, N, K, activation, 0)) return STRATA_ERR_ARG;
+  if (M == 0) return 0;
+  return dense_grad_plan(M, N, K, activation != ACT_NONE, dy_aligned != 0, z_aligned != 0, x_aligned != 0,
+                         w_aligned != 0, need_dx != 0, need_dw != 0, need_db != 0, nullptr, sms).bytes;
+}
+
+int strata_linear_act_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, int64_t ldw,
+                               const void* preact, int64_t ldz, void* dx, int64_t lddx, void* dw, int64_t lddw,
+                               float* db, int M, int N, int K, int activation, int dtype, void* workspace,
+                               int64_t workspace_bytes, void* stream) {
+  const int sms = current_sm_count();
+  if (sms <= 0) return STRATA_ERR_NO_DEVICE;
+  if (!dense_sizes(M, N, K, activation, dtype)) return STRATA_ERR_ARG;
+  const cudaStream_t st = as_stream(stream);
+  if (M == 0) {      // sums over no rows
+    cudaError_t e = cudaSuccess;
+    if (dw && lddw < K) return STRATA_ERR_ARG;
+    if (dw) e = cudaMemset2DAsync(dw, static_cast<size_t>(lddw) * 2, 0, static_cast<size_t>(K) * 2, N, st);
+    if (e == cudaSuccess && db) e = cudaMemsetAsync(db, 0, static_cast<size_t>(N) * 4, st);
+    return e == cudaSuccess ? STRATA_OK : -static_cast<int>(e) - 1000;
+  }
+  if (!dense_rows_ok(dy, lddy, N) || (dw && !dense_rows_ok(x, ldx, K)) || (dx && !dense_rows_ok(w, ldw, K)) ||
+      (activation != ACT_NONE && !dense_rows_ok(preact, ldz, N)) || (dx && !dense_rows_ok(dx, lddx, K)) ||
+      (dw && !dense_rows_ok(dw, lddw, K)) || (reinterpret_cast<uintptr_t>(db) & 3u) != 0)
+    return STRATA_ERR_ARG;
+  if (activation == ACT_NONE) preact = nullptr;
+  const DenseGradPlan g =
+      dense_grad_plan(M, N, K, activation != ACT_NONE, dense_aligned(dy, lddy), dense_aligned(preact, ldz),
+                      dense_aligned(x, ldx), dense_aligned(w, ldw), dx != nullptr, dw != nullptr, db != nullptr, workspace,
+                      sms);
+  if (g.bytes > 0 && (!workspace || workspace_bytes < g.bytes || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0))
+    return STRATA_ERR_ARG;
+  DenseGradParams q{};
+  q.M = M; q.N = N; q.K = K; q.act = activation; q.fp16 = dtype == STRATA_F16;
+  q.dy = {dy, lddy}; q.x = {x, ldx}; q.w = {w, ldw}; q.z = {preact, ldz};
+  q.dx = dx; q.lddx = lddx; q.dw = dw; q.lddw = lddw; q.db = db;
+  return launch_dense_backward(q, g, sms, st);
 }
 
 int strata_mlp_fused(int M, int C, int hidden) {
@@ -894,6 +984,104 @@ static int strata_adaln_cond_ready_bf16(const void* tokens, int B, int D, int h,
   p.D = D; p.h = h; p.w = w; p.Cb = Cb; p.factor = factor; p.ks = ks;
   int r = launch_adaln_cond(p, table, sms, as_stream(stream));
   return r == -2 ? STRATA_ERR_ARG : r;
+}
+
+static bool qk_heads_ok(const strata_heads* t, int head_dim) {
+  return t && t->data && aligned16(t->data) && t->stride_token % 8 == 0 && t->stride_head % 8 == 0 &&
+         t->stride_token >= 0 && t->stride_head >= 0 && head_dim > 0;
+}
+
+// Checks what both directions share and fills p; out: the tensors that are written.
+static int qk_params(QkParams& p, const strata_heads* q, const strata_heads* k, const strata_heads* yq,
+                     const strata_heads* yk, const float* w_q, const float* w_k, int heads_q, int heads_k, int head_dim,
+                     int rot, int adjacent, const void* table, int table_f32, int table_rows, const void* positions,
+                     int positions_64, int tokens_per_tile, int hw, int64_t M, float eps, int dtype) {
+  if (M < 0 || M > 0x7FFF0000 || heads_q <= 0 || heads_k <= 0 || heads_q > 65536 || heads_k > 65536 || head_dim <= 0 ||
+      (dtype != STRATA_BF16 && dtype != STRATA_F16))
+    return STRATA_ERR_ARG;
+  if (head_dim % 8 != 0 || head_dim > 256) return STRATA_ERR_UNSUPPORTED;
+  if (table) {
+    if (rot <= 0 || rot > head_dim || table_rows <= 0 || !aligned16(table)) return STRATA_ERR_ARG;
+    if (rot % (adjacent ? 8 : 16) != 0) return STRATA_ERR_UNSUPPORTED;
+    if (!positions && M > 0) {
+      if (tokens_per_tile <= 0 || hw <= 0) return STRATA_ERR_ARG;
+      // the largest row of the rule
+      const int64_t tile = (M - 1) / tokens_per_tile;
+      if (tile * hw + (M < hw ? M : hw) - 1 >= table_rows) return STRATA_ERR_ARG;
+    }
+    if (positions && (reinterpret_cast<uintptr_t>(positions) & (positions_64 ? 7u : 3u)) != 0) return STRATA_ERR_ARG;
+  }
+  if (!qk_heads_ok(q, head_dim) || !qk_heads_ok(k, head_dim) || !qk_heads_ok(yq, head_dim) ||
+      !qk_heads_ok(yk, head_dim) || ((reinterpret_cast<uintptr_t>(w_q) | reinterpret_cast<uintptr_t>(w_k)) & 3u) != 0)
+    return STRATA_ERR_ARG;
+  auto of = [](const strata_heads* t) { return QkTensor{t->data, t->stride_token, t->stride_head}; };
+  p.x[0] = of(q); p.x[1] = of(k);
+  p.y[0] = of(yq); p.y[1] = of(yk);
+  p.w[0] = w_q; p.w[1] = w_k;
+  p.heads[0] = heads_q; p.heads[1] = heads_k;
+  p.head_dim = head_dim; p.rot = table ? rot : 0;
+  p.table = table; p.table_f32 = table_f32; p.table_rows = table_rows;
+  p.positions = positions; p.positions_64 = positions_64;
+  p.tokens_per_tile = tokens_per_tile; p.hw = hw;
+  p.M = M; p.eps = eps;
+  return STRATA_OK;
+}
+
+int strata_qk_norm_rope(const strata_heads* h_q, const strata_heads* h_k, const strata_heads* h_q_out,
+                        const strata_heads* h_k_out, const float* w_q, const float* w_k, int heads_q, int heads_k,
+                        int head_dim, int rot, int adjacent, const void* table, int table_f32, int table_rows,
+                        const void* positions, int positions_64, int tokens_per_tile, int hw, int64_t M, float eps,
+                        int dtype, void* stream) {
+  const int sms = current_sm_count();
+  if (sms <= 0) return STRATA_ERR_NO_DEVICE;
+  if (M == 0) return STRATA_OK;
+  QkParams p{};
+  const int r = qk_params(p, h_q, h_k, h_q_out, h_k_out, w_q, w_k, heads_q, heads_k, head_dim, rot, adjacent, table,
+                          table_f32, table_rows, positions, positions_64, tokens_per_tile, hw, M, eps, dtype);
+  if (r != STRATA_OK) return r;
+  return launch_qk<false>(p, adjacent != 0, dtype == STRATA_F16, qk_blocks(M, heads_q + heads_k, head_dim, false, sms),
+                          as_stream(stream));
+}
+
+int64_t strata_qk_norm_rope_backward_workspace_bytes(int64_t M, int heads, int head_dim) {
+  const int sms = current_sm_count();
+  if (sms <= 0) return STRATA_ERR_NO_DEVICE;
+  if (M < 0 || M > 0x7FFF0000 || heads <= 0 || head_dim <= 0 || head_dim > 256) return STRATA_ERR_ARG;
+  return qk_blocks(M, heads, head_dim, true, sms) * 2 * head_dim * 4;
+}
+
+int strata_qk_norm_rope_backward(const strata_heads* h_dq, const strata_heads* h_dk, const strata_heads* h_q,
+                                 const strata_heads* h_k, const strata_heads* h_dq_in, const strata_heads* h_dk_in,
+                                 const float* w_q, const float* w_k, float* dw_q, float* dw_k, int heads_q, int heads_k,
+                                 int head_dim, int rot, int adjacent, const void* table, int table_f32, int table_rows,
+                                 const void* positions, int positions_64, int tokens_per_tile, int hw, int64_t M,
+                                 float eps, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  const int sms = current_sm_count();
+  if (sms <= 0) return STRATA_ERR_NO_DEVICE;
+  const cudaStream_t st = as_stream(stream);
+  if (M == 0) {
+    if (head_dim <= 0 || head_dim > 256) return STRATA_ERR_ARG;
+    cudaError_t e = cudaSuccess;
+    if (dw_q) e = cudaMemsetAsync(dw_q, 0, static_cast<size_t>(head_dim) * 4, st);
+    if (e == cudaSuccess && dw_k) e = cudaMemsetAsync(dw_k, 0, static_cast<size_t>(head_dim) * 4, st);
+    return e == cudaSuccess ? STRATA_OK : -static_cast<int>(e) - 1000;
+  }
+  QkParams p{};
+  int r = qk_params(p, h_q, h_k, h_dq_in, h_dk_in, w_q, w_k, heads_q, heads_k, head_dim, rot, adjacent, table, table_f32,
+                    table_rows, positions, positions_64, tokens_per_tile, hw, M, eps, dtype);
+  if (r != STRATA_OK) return r;
+  if (!qk_heads_ok(h_dq, head_dim) || !qk_heads_ok(h_dk, head_dim)) return STRATA_ERR_ARG;
+  p.dy[0] = {h_dq->data, h_dq->stride_token, h_dq->stride_head};
+  p.dy[1] = {h_dk->data, h_dk->stride_token, h_dk->stride_head};
+  const long long blocks = qk_blocks(M, heads_q + heads_k, head_dim, true, sms);
+  if (dw_q || dw_k) {
+    if (!workspace || !aligned16(workspace) || workspace_bytes < blocks * 2 * head_dim * 4) return STRATA_ERR_ARG;
+    p.partial = static_cast<float*>(workspace);
+  }
+  r = launch_qk<true>(p, adjacent != 0, dtype == STRATA_F16, blocks, st);
+  if (r != 0 || !p.partial) return r;
+  return launch_chained(qk_weight_grad_kernel, dim3((2 * head_dim + 31) / 32), 256, 0, st, 1,
+                        static_cast<const float*>(p.partial), static_cast<int>(blocks), head_dim, dw_q, dw_k);
 }
 
 int strata_adaln_cond_bf16(const void* tokens, int B, int D, int h, int w, int Cb, int factor,

@@ -27,6 +27,7 @@ enum StatusCode : int {
   ST_TIMEOUT_SOFTMAX = 104,    // attention softmax warps waited too long
   ST_TIMEOUT_PEER_FLAG = 105,  // halo consumer waited too long for a peer's ready flag
   ST_BAD_TMEM = 106,
+  ST_BAD_POSITION = 107,       // a token's position lies behind the rotary table
 };
 
 constexpr long long WAIT_LIMIT_CYCLES = 4000000000LL;  // ~2 s at 2 GHz

@@ -1,0 +1,369 @@
+// Host side of the dense layer: which kernel, tile and split a product takes, its workspace, and the launches of a
+// forward and a backward pass.
+#pragma once
+#include "dense_rows.cuh"
+
+namespace strata {
+
+// ---------------------------------------------------------------- tile and split of a product
+struct DenseChoice {
+  int bn;          // 64, 128: one CTA, 128 rows; 256: a pair of CTAs, 256 rows
+  bool split;
+  DensePlan plan;
+  int tile_m() const { return bn == 256 ? 2 * GEMM_BM : GEMM_BM; }
+  int64_t slab_bytes() const { return split ? static_cast<int64_t>(plan.slots()) * tile_m() * bn * 4 : 0; }
+};
+
+inline int dense_tiles(int M, int N, int bn) {
+  const int tm = bn == 256 ? 2 * GEMM_BM : GEMM_BM;
+  return ((M + tm - 1) / tm) * ((N + bn - 1) / bn);
+}
+
+// CTA pairs that are resident at once (not every SM has a partner), asked once per device.
+inline int dense_pairs(int sms) {
+  static std::atomic<int> cached[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return sms / 2;
+  int fit = cached[dev].load(std::memory_order_relaxed);
+  if (fit != 0) return fit;
+  using S = DenseSmem<256, true, DENSE_Y>;
+  auto kern = dense_tcgen05_kernel<256, true, DENSE_NT, DENSE_Y, __nv_bfloat16>;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(sms & ~1));
+  cfg.blockDim = dim3(GEMM_THREADS);
+  cfg.dynamicSmemBytes = S::TOTAL;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TOTAL) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&fit, kern, &cfg) != cudaSuccess || fit <= 0) {
+    cudaGetLastError();
+    return sms / 2;
+  }
+  if (fit > sms / 2) fit = sms / 2;
+  cached[dev].store(fit, std::memory_order_relaxed);
+  return fit;
+}
+
+// The cheapest form by a model of each one's time, in microseconds: a k-block of 64 on one unit, the part of a tile's
+// epilogue that nothing hides, a launch, and a slab's way to memory and back.
+inline DenseChoice dense_choice(int M, int N, int K, int sms) {
+  const int num_kb = (K + GEMM_BK - 1) / GEMM_BK;
+  DenseChoice best{};
+  double best_us = 0.0;
+  for (int bn = 64; bn <= 256; bn *= 2) {
+    const int units = bn == 256 ? dense_pairs(sms) : sms, tiles = dense_tiles(M, N, bn);
+    const double kb_us = bn == 256 ? 0.27 : bn == 128 ? 0.19 : 0.15;
+    const double tile_us = bn == 256 ? 1.6 : bn == 128 ? 1.0 : 0.8;     // epilogue that nothing hides
+    const int turns = (tiles + units - 1) / units;
+    const double us = turns * (num_kb * kb_us > tile_us ? num_kb * kb_us : tile_us) + tile_us + 2.0;
+    if (best.bn == 0 || us < best_us) {
+      best = DenseChoice{bn, false, {}};
+      best.plan.tiles = tiles;
+      best.plan.units = units;
+      best.plan.num_kb = num_kb;
+      best_us = us;
+    }
+    const DensePlan s = dense_plan(tiles, units, num_kb, 4);
+    if (s.rest == 0 || (s.chunks == 1 && s.tail == 0)) continue;
+    const int tm = bn == 256 ? 2 * GEMM_BM : GEMM_BM;
+    const double rows = static_cast<double>(M < tm ? M : tm) / tm;       // of a slab that exist
+    const double slab_mb = s.slots() * rows * tm * bn * 4e-6;
+    const int kbs = s.whole / units * num_kb + s.head;
+    const double split_us = kbs * kb_us + 2 * tile_us + 2.0 + 3.0 + slab_mb * 2 / 5.0;
+    if (split_us < 0.95 * best_us) {
+      best = DenseChoice{bn, true, s};
+      best_us = split_us;
+    }
+  }
+  return best;
+}
+
+// ---------------------------------------------------------------- launches
+struct DenseOperand { const void* p; long long ld; };
+
+template <int BN, bool PAIR, int LAY, int EPI, typename T>
+inline int launch_dense_t(const DenseOperand& A, const DenseOperand& B, const DenseParams& p, int units, cudaStream_t st) {
+  const bool a_mn = LAY == DENSE_TN, b_mn = LAY != DENSE_NT;
+  constexpr int TILE_M = PAIR ? 2 * GEMM_BM : GEMM_BM;
+  CUtensorMap tmA, tmB, tmOut, tmKeep, tmAux;
+  auto map = [](CUtensorMap* tm, const DenseOperand& o, int rows, int cols, uint32_t bx, uint32_t by, TmapSwizzle sw) {
+    const uint64_t dims[2] = {static_cast<uint64_t>(cols), static_cast<uint64_t>(rows)};
+    const uint64_t str[1] = {static_cast<uint64_t>(o.ld) * 2};
+    const uint32_t box[2] = {bx, by};
+    return make_tmap_bf16(tm, o.p, 2, dims, str, box, sw);      // (either 16-bit type: nothing is converted)
+  };
+  if (map(&tmA, A, a_mn ? p.K : p.M, a_mn ? p.M : p.K, 64, a_mn ? 64 : GEMM_BM, TMAP_SWIZZLE_128B) != 0) return -20;
+  if (map(&tmB, B, b_mn ? p.K : p.N, b_mn ? p.N : p.K, 64, b_mn ? 64 : (PAIR ? BN / 2 : BN), TMAP_SWIZZLE_128B) != 0)
+    return -21;
+  tmOut = tmKeep = tmAux = tmA;
+  if (EPI != DENSE_PART && !p.direct) {
+    if (map(&tmOut, {p.out, p.ldo}, p.M, p.N, 32, 32, TMAP_SWIZZLE_64B) != 0) return -22;
+    if (p.aux && map(&tmAux, {p.aux, p.ldaux}, p.M, p.N, 32, 32, TMAP_SWIZZLE_64B) != 0) return -23;
+    if (p.keep && map(&tmKeep, {p.keep, p.ldk}, p.M, p.N, 32, 32, TMAP_SWIZZLE_64B) != 0) return -25;
+  }
+  using S = DenseSmem<BN, PAIR, EPI>;
+  auto kern = dense_tcgen05_kernel<BN, PAIR, LAY, EPI, T>;
+  static std::atomic<uint64_t> smem_set;
+  if (const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), S::TOTAL, smem_set); e != cudaSuccess)
+    return -static_cast<int>(e) - 1000;
+  const int tiles = ((p.M + TILE_M - 1) / TILE_M) * ((p.N + BN - 1) / BN);
+  // a split's units are its plan's: blocks that are not resident at once run one after the other, none waits
+  // for another
+  int grid = EPI == DENSE_PART || tiles >= units ? units : tiles;
+  return launch_chained(kern, dim3(static_cast<unsigned>(PAIR ? 2 * grid : grid)), GEMM_THREADS, S::TOTAL, st,
+                        PAIR ? 2 : 1, tmA, tmB, tmOut, tmKeep, tmAux, p);
+}
+
+template <int LAY, int EPI, typename T>
+inline int launch_dense_bn(int bn, const DenseOperand& A, const DenseOperand& B, const DenseParams& p, int units,
+                           cudaStream_t st) {
+  if (bn == 256) return launch_dense_t<256, true, LAY, EPI, T>(A, B, p, units, st);
+  if (bn == 128) return launch_dense_t<128, false, LAY, EPI, T>(A, B, p, units, st);
+  return launch_dense_t<64, false, LAY, EPI, T>(A, B, p, units, st);
+}
+
+inline int launch_dense_finish(const DenseFinish& f, cudaStream_t st) {
+  const DensePlan& s = f.p.plan;
+  const int blocks = (f.p.part ? s.tiles * f.blocks_per_tile : 0) + (f.db ? (f.sum_cols + 31) / 32 : 0);
+  if (blocks == 0) return 0;
+  if (f.p.fp16)
+    return launch_chained(dense_finish_kernel<__half>, dim3(blocks), FINISH_THREADS, 0, st, 1, f);
+  return launch_chained(dense_finish_kernel<__nv_bfloat16>, dim3(blocks), FINISH_THREADS, 0, st, 1, f);
+}
+
+// One product of a choice, with the second kernel where it is split. `fin`: the column sums that kernel adds up besides
+// (their fields only), or nullptr.
+template <int LAY>
+inline int launch_dense(const DenseOperand& A, const DenseOperand& B, DenseParams p, const DenseChoice& c, void* slabs,
+                        const DenseFinish* sums, cudaStream_t st) {
+  DenseFinish f{};
+  if (sums) f = *sums;
+  int r;
+  if (c.split) {
+    p.part = static_cast<float*>(slabs);
+    p.plan = c.plan;
+    // (the slabs are fp32 and the type is a bit of the instruction descriptor: one kernel for both)
+    r = launch_dense_bn<LAY, DENSE_PART, __nv_bfloat16>(c.bn, A, B, p, c.plan.units, st);
+    f.p = p;
+    f.tile_m = c.tile_m();
+    f.bn = c.bn;
+    f.tiles_n = (p.N + c.bn - 1) / c.bn;
+    const int rows = p.M < f.tile_m ? p.M : f.tile_m;        // of a slab that exist
+    f.blocks_per_tile = (rows * c.bn + 4 * FINISH_THREADS - 1) / (4 * FINISH_THREADS);
+  } else {
+    p.part = nullptr;
+    if (LAY == DENSE_NT && p.keep != nullptr) {
+      r = p.fp16 ? launch_dense_bn<DENSE_NT, DENSE_Y_KEEP, __half>(c.bn, A, B, p, c.plan.units, st)
+                 : launch_dense_bn<DENSE_NT, DENSE_Y_KEEP, __nv_bfloat16>(c.bn, A, B, p, c.plan.units, st);
+    } else {
+      r = p.fp16 ? launch_dense_bn<LAY, DENSE_Y, __half>(c.bn, A, B, p, c.plan.units, st)
+                 : launch_dense_bn<LAY, DENSE_Y, __nv_bfloat16>(c.bn, A, B, p, c.plan.units, st);
+    }
+    f.p = p;
+  }
+  if (r != 0 || (!c.split && !sums)) return r;
+  return launch_dense_finish(f, st);
+}
+
+template <typename T>
+inline int launch_few_rows_t(const DenseOperand& x, const DenseOperand& w, const DenseParams& p, bool vec, int sms,
+                             cudaStream_t st) {
+  // warps: a column group of four each; split along the contraction until every SM has eight
+  const int groups = (p.N + FEW_COLS - 1) / FEW_COLS;
+  int kw = 1;
+  while (kw < 8 && groups * kw < 8 * sms && p.K >= 2 * kw * 32 * (vec ? 8 : 1)) kw *= 2;
+  const dim3 grid(static_cast<unsigned>((groups + 8 / kw - 1) / (8 / kw)));
+  const T* xp = static_cast<const T*>(x.p);
+  const T* wp = static_cast<const T*>(w.p);
+#define STRATA_FEW(R)                                                                                              \
+  (vec ? launch_chained(dense_few_rows_kernel<T, R, 8>, grid, 256, 0, st, 1, xp, x.ld, wp, w.ld, kw, p)            \
+       : launch_chained(dense_few_rows_kernel<T, R, 1>, grid, 256, 0, st, 1, xp, x.ld, wp, w.ld, kw, p))
+  if (p.M == 1) return STRATA_FEW(1);
+  if (p.M == 2) return STRATA_FEW(2);
+  if (p.M <= 4) return STRATA_FEW(4);
+  return STRATA_FEW(8);
+#undef STRATA_FEW
+}
+
+inline long long dense_round8(long long n) { return (n + 7) / 8 * 8; }
+inline bool dense_aligned(const void* p, long long ld) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % 8 == 0; }
+// Rows that TMA may store: it writes whole 16-byte pieces, with zeros behind the last column.
+inline bool dense_whole(const void* p, long long ld, int cols) { return dense_aligned(p, ld) && cols % 8 == 0; }
+
+// Pieces of a workspace, 256-byte aligned.
+struct DenseArena {
+  uint8_t* base;
+  int64_t used;
+  void* take(int64_t bytes) {
+    void* p = base ? base + used : nullptr;
+    used += (bytes + 255) / 256 * 256;
+    return p;
+  }
+};
+
+inline int launch_align_rows(const AlignRows& a, int n, int sms, cudaStream_t st) {
+  long long most = 0;
+  for (int j = 0; j < n; ++j) {
+    const long long v = a.rows[j] * (a.ldd[j] / 8);
+    most = v > most ? v : most;
+  }
+  long long blocks = (most + 255) / 256;
+  if (blocks > 8LL * sms) blocks = 8LL * sms;
+  return launch_chained(dense_align_rows_kernel, dim3(static_cast<unsigned>(blocks), n), 256, 0, st, 1, a);
+}
+
+// ---------------------------------------------------------------- forward
+// Workspace: aligned copies of x and w where they are not aligned themselves, then the slabs of a split. With base
+// nullptr nothing is launched and `used` says how much is needed.
+inline int64_t dense_forward_bytes(int M, int N, int K, bool x_ok, bool w_ok, int sms) {
+  if (M <= FEW_ROWS) return 0;
+  DenseArena ws{nullptr, 0};
+  if (!x_ok) ws.take(2 * dense_round8(K) * M);
+  if (!w_ok) ws.take(2 * dense_round8(K) * N);
+  ws.take(dense_choice(M, N, K, sms).slab_bytes());
+  return ws.used;
+}
+
+inline int launch_dense_forward(DenseOperand x, DenseOperand w, const DenseParams& p, void* workspace, int sms,
+                                cudaStream_t st) {
+  const bool x_ok = dense_aligned(x.p, x.ld), w_ok = dense_aligned(w.p, w.ld);
+  if (p.M <= FEW_ROWS) {
+    const bool vec = x_ok && w_ok && p.K % 8 == 0;
+    return p.fp16 ? launch_few_rows_t<__half>(x, w, p, vec, sms, st)
+                  : launch_few_rows_t<__nv_bfloat16>(x, w, p, vec, sms, st);
+  }
+  DenseArena ws{static_cast<uint8_t*>(workspace), 0};
+  AlignRows a{};
+  int n = 0;
+  auto align = [&](DenseOperand& o, long long rows, int cols) {
+    const long long ld = dense_round8(cols);
+    void* to = ws.take(2 * ld * rows);
+    a.src[n] = static_cast<const uint16_t*>(o.p); a.lds[n] = o.ld;
+    a.dst[n] = static_cast<uint16_t*>(to); a.ldd[n] = ld;
+    a.rows[n] = rows; a.cols[n++] = cols;
+    o = {to, ld};
+  };
+  if (!x_ok) align(x, p.M, p.K);
+  if (!w_ok) align(w, p.N, p.K);
+  if (n > 0)
+    if (const int r = launch_align_rows(a, n, sms, st); r != 0) return r;
+  const DenseChoice c = dense_choice(p.M, p.N, p.K, sms);
+  return launch_dense<DENSE_NT>(x, w, p, c, ws.take(c.slab_bytes()), nullptr, st);
+}
+
+// ---------------------------------------------------------------- backward
+struct DenseGradParams {
+  int M, N, K, act, fp16;
+  DenseOperand dy, x, w, z;        // z.p nullptr: act is none
+  void* dx; long long lddx;        // any of the three outputs may be absent
+  void* dw; long long lddw;
+  float* db;
+};
+
+struct DenseGradSums { int lanes, cols, rows_per_block, blocks; };     // geometry of dense_slope_kernel
+
+inline DenseGradSums dense_grad_sums(int M, int N, int vec, int sms) {
+  DenseGradSums g{};
+  const int units = (N + vec - 1) / vec;
+  g.lanes = 1;
+  while (g.lanes < 32 && g.lanes < units) g.lanes *= 2;
+  g.cols = (units + g.lanes - 1) / g.lanes;
+  const int step = 256 / g.lanes;
+  // eight blocks of 256 threads on every SM, but no fewer than four rows a thread
+  long long blocks = (8LL * sms + g.cols - 1) / g.cols;
+  const long long most = (M + 4LL * step - 1) / (4LL * step);
+  if (blocks > most) blocks = most;
+  g.rows_per_block = static_cast<int>((M + blocks - 1) / blocks);
+  g.blocks = (M + g.rows_per_block - 1) / g.rows_per_block;
+  return g;
+}
+
+// dz goes through memory when there is an activation, or when dy is not aligned; then it is [M, round8(N)].
+struct DenseGradPlan {
+  bool copy_x, copy_w, make_dz, vec;
+  DenseChoice cx, cw;
+  DenseGradSums sums;
+  int64_t bytes;
+  void *dz, *xs, *ws, *slabs;
+  float* col_sums;
+};
+
+inline DenseGradPlan dense_grad_plan(int M, int N, int K, bool act, bool dy_ok, bool z_ok, bool x_ok, bool w_ok, bool dx,
+                                     bool dw, bool db, void* workspace, int sms) {
+  DenseGradPlan g{};
+  g.make_dz = (dx || dw) && (act || !dy_ok);
+  g.copy_x = dw && !x_ok;
+  g.copy_w = dx && !w_ok;
+  g.vec = dy_ok && (!act || z_ok) && N % 8 == 0;
+  g.sums = dense_grad_sums(M, N, g.vec ? 8 : 1, sms);
+  if (dx) g.cx = dense_choice(M, K, N, sms);
+  if (dw) g.cw = dense_choice(N, K, M, sms);
+  DenseArena ws{static_cast<uint8_t*>(workspace), 0};
+  if (g.make_dz) g.dz = ws.take(2 * dense_round8(N) * M);
+  if (g.copy_x) g.xs = ws.take(2 * dense_round8(K) * M);
+  if (g.copy_w) g.ws = ws.take(2 * dense_round8(K) * N);
+  if (db) g.col_sums = static_cast<float*>(ws.take(4LL * g.sums.blocks * N));
+  const int64_t sx = g.cx.slab_bytes(), sw = g.cw.slab_bytes();
+  g.slabs = ws.take(sx > sw ? sx : sw);        // one after the other on the stream
+  g.bytes = ws.used;
+  return g;
+}
+
+inline int launch_dense_backward(const DenseGradParams& q, const DenseGradPlan& g, int sms, cudaStream_t st) {
+  DenseOperand x = q.x, w = q.w, dz = q.dy;
+  int r;
+  if (g.copy_x || g.copy_w) {
+    AlignRows a{};
+    int n = 0;
+    auto align = [&](DenseOperand& o, void* to, long long rows) {
+      const long long ld = dense_round8(q.K);
+      a.src[n] = static_cast<const uint16_t*>(o.p); a.lds[n] = o.ld;
+      a.dst[n] = static_cast<uint16_t*>(to); a.ldd[n] = ld;
+      a.rows[n] = rows; a.cols[n++] = q.K;
+      o = {to, ld};
+    };
+    if (g.copy_x) align(x, g.xs, q.M);
+    if (g.copy_w) align(w, g.ws, q.N);
+    if ((r = launch_align_rows(a, n, sms, st)) != 0) return r;
+  }
+  if (g.make_dz || q.db) {
+    SlopeParams s{};
+    s.dy = q.dy.p; s.ldy = q.dy.ld;
+    s.z = q.z.p; s.ldz = q.z.ld;
+    s.dz = g.make_dz ? g.dz : nullptr; s.lddz = dense_round8(q.N);
+    s.sums = g.col_sums;
+    s.M = q.M; s.N = q.N; s.act = q.act; s.lanes = g.sums.lanes; s.rows_per_block = g.sums.rows_per_block;
+    const dim3 grid(static_cast<unsigned>(g.sums.cols), static_cast<unsigned>(g.sums.blocks));
+#define STRATA_SLOPE(T) \
+  (g.vec ? launch_chained(dense_slope_kernel<T, 8>, grid, 256, 0, st, 1, s) \
+         : launch_chained(dense_slope_kernel<T, 1>, grid, 256, 0, st, 1, s))
+    r = q.fp16 ? STRATA_SLOPE(__half) : STRATA_SLOPE(__nv_bfloat16);
+#undef STRATA_SLOPE
+    if (r != 0) return r;
+    if (g.make_dz) dz = {g.dz, dense_round8(q.N)};
+  }
+  if (q.dx) {
+    DenseParams p{};
+    p.M = q.M; p.N = q.K; p.K = q.N;
+    p.out = q.dx; p.ldo = q.lddx; p.fp16 = q.fp16;
+    p.direct = !dense_whole(q.dx, q.lddx, q.K);
+    if ((r = launch_dense<DENSE_NN>(dz, w, p, g.cx, g.slabs, nullptr, st)) != 0) return r;
+  }
+  DenseFinish f{};
+  f.sums = g.col_sums;
+  f.sum_rows = g.sums.blocks; f.sum_cols = q.N; f.db = q.db;
+  if (q.dw) {
+    DenseParams p{};
+    p.M = q.N; p.N = q.K; p.K = q.M;
+    p.out = q.dw; p.ldo = q.lddw; p.fp16 = q.fp16;
+    p.direct = !dense_whole(q.dw, q.lddw, q.K);
+    return launch_dense<DENSE_TN>(dz, x, p, g.cw, g.slabs, q.db ? &f : nullptr, st);
+  }
+  return q.db ? launch_dense_finish(f, st) : 0;
+}
+
+}  // namespace strata

@@ -113,6 +113,162 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     return out if x.dim() == 2 else out.reshape(*x.shape[:-1], N)
 
 
+# ------------------------------------------------------------------ dense layer, bf16 or fp16, with gradients
+ACTIVATIONS = {"none": 0, "gelu": 1, "gelu_tanh": 2, "silu": 3, "relu": 4}
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+
+
+def _activation(name: str) -> int:
+    try:
+        return ACTIVATIONS[name]
+    except (KeyError, TypeError):
+        raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)}, got {name!r}") from None
+
+
+def _require_16bit(t: torch.Tensor, name: str) -> int:
+    if not t.is_cuda:
+        raise _lib.StrataLibraryError(f"{name} must be a CUDA tensor: strata_b200 has no CPU path")
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{name} must be bfloat16 or float16, got {t.dtype}")
+    return code
+
+
+def _like(t: torch.Tensor, name: str, x: torch.Tensor) -> None:
+    if t.dtype != x.dtype or t.device != x.device:
+        raise TypeError(f"{name} must be {x.dtype} on {x.device}, got {t.dtype} on {t.device}")
+
+
+def _f32_like(t, name: str, shape, x: torch.Tensor):
+    if t is None:
+        return None
+    if t.dtype != torch.float32 or t.device != x.device:
+        raise TypeError(f"{name} must be float32 on {x.device}, got {t.dtype} on {t.device}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
+    return t.contiguous()
+
+
+def _packed_rows(t: torch.Tensor, cols: int, name: str):
+    """t [..., cols] as rows (tensor, row stride): unit inner stride and rows that do not overlap, copied where they do."""
+    if t.dim() < 2 or t.shape[-1] != cols:
+        raise ValueError(f"{name} must be [..., {cols}] with at least 2 dims, got {tuple(t.shape)}")
+    t = t.detach() if t.dim() == 2 else t.reshape(-1, cols)
+    if t.shape[0] > 1:
+        if (t.stride(1) != 1 and cols > 1) or t.stride(0) < cols:
+            t = t.contiguous()
+        return t, t.stride(0)
+    return (t if cols == 1 or t.stride(1) == 1 else t.contiguous()), cols
+
+
+def _aligned16(t, ld: int) -> int:
+    return int(t.data_ptr() % 16 == 0 and ld % 8 == 0)
+
+
+def _scratch(need: int, device):
+    if need < 0:
+        _lib.check(need, "workspace size")
+    return torch.empty(need, dtype=torch.uint8, device=device) if need else None
+
+
+def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, activation: str = "none",
+               residual: torch.Tensor | None = None, *, save_preact: bool = False, out: torch.Tensor | None = None):
+    """y = residual + act(z), z = x @ weight.T + bias, in one pass: x [..., K], weight [N, K], residual and y [..., N] of
+    one type (bfloat16 or float16), bias [N] fp32; activation one of "none", "gelu" (erf), "gelu_tanh", "silu", "relu".
+    Any number of rows, any widths and row strides. Sums and the epilogue are fp32, y is rounded once.
+
+    save_preact: returns (y, z); linear_act_backward needs z for any activation but "none". out: where y goes, [M, N]
+    with unit inner stride; it may be the residual, no other operand. The gradients are linear_act_backward's;
+    torch.ops.strata_b200.linear_act is the differentiable form."""
+    dtype = _require_16bit(x, "x")
+    _like(weight, "weight", x)
+    act = _activation(activation)
+    if weight.dim() != 2:
+        raise ValueError(f"weight must be [N, K], got {tuple(weight.shape)}")
+    N, K = weight.shape
+    x2, ldx = _packed_rows(x, K, "x")
+    w2, ldw = _packed_rows(weight, K, "weight")
+    M = x2.shape[0]
+    bias = _f32_like(bias, "bias", (N,), x)
+    shape = (*x.shape[:-1], N)
+    r2, ldr = None, 0
+    if residual is not None:
+        _like(residual, "residual", x)
+        if tuple(residual.shape) != shape:
+            raise ValueError(f"residual must be {shape}, got {tuple(residual.shape)}")
+        r2, ldr = _packed_rows(residual, N, "residual")
+    if out is None:
+        y, ldy = torch.empty(shape, dtype=x.dtype, device=x.device), N
+    else:
+        _like(out, "out", x)
+        if tuple(out.shape) != (M, N) or (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
+            raise ValueError(f"out must be [{M}, {N}] with unit inner stride")
+        y, ldy = out, out.stride(0) if M > 1 else N
+    z = torch.empty(shape, dtype=x.dtype, device=x.device) if save_preact else None
+    if M:
+        lib = _lib.load()
+        with _lib.on_device(x):
+            ws, need = None, 0
+            if M > 8:
+                need = lib.strata_linear_act_workspace_bytes(M, N, K, _aligned16(x2, ldx), _aligned16(w2, ldw))
+                ws = _scratch(need, x.device)
+            _lib.check(lib.strata_linear_act(
+                x2.data_ptr(), ldx, w2.data_ptr(), ldw, None if bias is None else bias.data_ptr(),
+                None if r2 is None else r2.data_ptr(), ldr, y.data_ptr(), ldy, None if z is None else z.data_ptr(), N,
+                M, N, K, act, dtype, None if ws is None else ws.data_ptr(), need, _stream_ptr(x)), "strata_linear_act")
+    if out is not None and x.dim() != 2:
+        y = out.view(shape)
+    return (y, z) if save_preact else y
+
+
+def linear_act_backward(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, activation: str = "none",
+                        preact: torch.Tensor | None = None, *, need_x: bool = True, need_weight: bool = True,
+                        need_bias: bool = True):
+    """Gradients of linear_act at dy = grad [..., N]: (dx [..., K], dweight [N, K], dbias [N] fp32), None for those not
+    needed; the residual's is grad itself. preact: the z that linear_act saved (any activation but "none"). No atomics:
+    the same call gives the same bits."""
+    dtype = _require_16bit(grad, "grad")
+    _like(x, "x", grad)
+    _like(weight, "weight", grad)
+    act = _activation(activation)
+    if weight.dim() != 2:
+        raise ValueError(f"weight must be [N, K], got {tuple(weight.shape)}")
+    N, K = weight.shape
+    if x.dim() < 2 or x.shape[-1] != K:
+        raise ValueError(f"x must be [..., {K}] with at least 2 dims, got {tuple(x.shape)}")
+    shape = (*x.shape[:-1], N)
+    if tuple(grad.shape) != shape:
+        raise ValueError(f"grad must be {shape}, got {tuple(grad.shape)}")
+    g2, ldg = _packed_rows(grad, N, "grad")
+    x2, ldx = _packed_rows(x, K, "x")
+    w2, ldw = _packed_rows(weight, K, "weight")
+    z2, ldz = None, 0
+    if act:
+        if preact is None:
+            raise ValueError(f'the gradient through "{activation}" needs preact, the z that linear_act saves')
+        _like(preact, "preact", grad)
+        if tuple(preact.shape) != shape:
+            raise ValueError(f"preact must be {shape}, got {tuple(preact.shape)}")
+        z2, ldz = _packed_rows(preact, N, "preact")
+    M, dev = x2.shape[0], x.device
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
+    dw = torch.empty((N, K), dtype=x.dtype, device=dev) if need_weight else None
+    db = torch.empty(N, dtype=torch.float32, device=dev) if need_bias else None
+    if need_x or need_weight or need_bias:
+        lib = _lib.load()
+        with _lib.on_device(x):
+            need = lib.strata_linear_act_backward_workspace_bytes(
+                M, N, K, act, _aligned16(g2, ldg), 0 if z2 is None else _aligned16(z2, ldz), _aligned16(x2, ldx),
+                _aligned16(w2, ldw), int(need_x), int(need_weight), int(need_bias))
+            ws = _scratch(need, dev)
+            _lib.check(lib.strata_linear_act_backward(
+                g2.data_ptr(), ldg, x2.data_ptr(), ldx, w2.data_ptr(), ldw, None if z2 is None else z2.data_ptr(), ldz,
+                None if dx is None else dx.data_ptr(), K, None if dw is None else dw.data_ptr(), K,
+                None if db is None else db.data_ptr(), M, N, K, act, dtype, None if ws is None else ws.data_ptr(), need,
+                _stream_ptr(x)), "strata_linear_act_backward")
+    return dx, dw, db
+
+
 def mlp(x: torch.Tensor, w1: torch.Tensor, b1: torch.Tensor | None, w2: torch.Tensor,
         b2: torch.Tensor | None, residual: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
     """residual + linear(gelu(linear(x, w1, b1)), w2, b2) of rows [M, C]: one kernel for narrow models, the two
@@ -507,6 +663,160 @@ def qk_norm_rows_(qkv: torch.Tensor, C: int, eps: float = 1e-6) -> torch.Tensor:
             qkv.data_ptr(), qkv.stride(0), qkv.shape[0], int(C), float(eps), _stream_ptr(qkv)),
             "strata_qk_norm_rows_bf16")
     return qkv
+
+
+def _heads(t: torch.Tensor, name: str, shape, like: torch.Tensor):
+    """t [..., heads, head_dim] as [tokens, heads, head_dim] for the kernels: a view where the token stride is one and
+    everything is in 16-byte pieces, else a copy."""
+    if t.dtype != like.dtype or t.device != like.device:
+        raise TypeError(f"{name} must be {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
+    t = t.detach() if t.dim() == 3 else t.detach().reshape(-1, *shape[-2:])
+    M, heads, hd = t.shape
+    # (a dimension of one has whatever stride)
+    token, head = t.stride(0) if M > 1 else heads * hd, t.stride(1) if heads > 1 else hd
+    if t.stride(2) != 1 or token % 8 or head % 8 or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+        token, head = heads * hd, hd
+    return t, _lib.Heads(t.data_ptr(), token, head)
+
+
+def _heads_out(t: torch.Tensor, name: str, shape, like: torch.Tensor):
+    t3, desc = _heads(t, name, shape, like)
+    (M, heads, hd), inner, outer = t3.shape, desc.stride_head, desc.stride_token
+    sizes = (heads, M)
+    if inner > outer:
+        inner, outer, sizes = outer, inner, (M, heads)
+    if t3.data_ptr() != t.data_ptr() or (sizes[0] > 1 and inner < hd) or (
+            sizes[1] > 1 and outer < max(inner * (sizes[0] - 1), 0) + hd):
+        raise ValueError(f"{name} must be viewable as [tokens, heads, head_dim] in 16-byte pieces that do not overlap")
+    return desc
+
+
+def _qk_arguments(q, k, q_weight, k_weight, rope_cs, positions, tokens_per_tile, hw, interleaved):
+    """What both directions check: (heads_q, heads_k, head_dim, kept tensors, the C arguments from rot to hw)."""
+    _like(k, "k", q)
+    if q.dim() < 3 or k.dim() != q.dim():
+        raise ValueError("q and k must be [..., heads, head_dim]")
+    hq, hd = q.shape[-2:]
+    hk = k.shape[-2]
+    if k.shape[:-2] != q.shape[:-2] or k.shape[-1] != hd:
+        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} must have the same tokens and head_dim")
+    if hd % 8 or not 8 <= hd <= 256 or not hq or not hk:
+        raise ValueError(f"head_dim must be a multiple of 8 up to 256 and both have heads, got {hq} + {hk} heads of {hd}")
+    M = 1
+    for n in q.shape[:-2]:
+        M *= n
+    q_weight = _f32_like(q_weight, "q_weight", (hd,), q)
+    k_weight = _f32_like(k_weight, "k_weight", (hd,), q)
+    if rope_cs is None:
+        if positions is not None:
+            raise ValueError("positions are rows of rope_cs: give both or neither")
+        return hq, hk, hd, M, (q_weight, k_weight), (0, int(interleaved), None, 0, 0, None, 0, 0, 0)
+    if rope_cs.dtype not in (torch.float16, torch.float32) or rope_cs.device != q.device:
+        raise TypeError(f"rope_cs must be float16 or float32 on {q.device}, got {rope_cs.dtype} on {rope_cs.device}")
+    if rope_cs.dim() < 3 or rope_cs.shape[-1] != 2:
+        raise ValueError(f"rope_cs must be [..., rot / 2, 2], got {tuple(rope_cs.shape)}")
+    rot = 2 * rope_cs.shape[-2]
+    unit = 8 if interleaved else 16
+    if rot % unit or not 0 < rot <= hd:
+        raise ValueError(f"rope_cs turns {rot} channels: a multiple of {unit} up to head_dim {hd} is needed")
+    cs = rope_cs.contiguous()
+    if cs.data_ptr() % 16:
+        cs = cs.clone()
+    rows = cs.numel() // rot
+    if not rows:
+        raise ValueError("rope_cs has no rows")
+    pos, wide = None, 0
+    if positions is not None:
+        if positions.dtype not in (torch.int32, torch.int64) or positions.device != q.device:
+            raise TypeError(f"positions must be int32 or int64 on {q.device}, got {positions.dtype} on {positions.device}")
+        if positions.numel() != M:
+            raise ValueError(f"positions must name a row for each of the {M} tokens, got {positions.numel()}")
+        if tokens_per_tile is not None or hw is not None:
+            raise ValueError("a token's row is given by positions or by tokens_per_tile and hw, not by both")
+        pos, wide = positions.contiguous(), int(positions.dtype == torch.int64)
+        per, hw = 0, 0
+    else:
+        per = rows if tokens_per_tile is None else int(tokens_per_tile)
+        hw = per if hw is None else int(hw)
+        if per <= 0 or hw <= 0:
+            raise ValueError("tokens_per_tile and hw must be positive")
+        if M and (M - 1) // per * hw + min(M, hw) > rows:
+            raise ValueError(f"{M} tokens, {per} a tile with {hw} rows each, need more than the {rows} rows of rope_cs")
+    return hq, hk, hd, M, (q_weight, k_weight, cs, pos), (
+        rot, int(interleaved), cs.data_ptr(), int(cs.dtype == torch.float32), rows,
+        None if pos is None else pos.data_ptr(), wide, per, hw)
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None = None,
+                 k_weight: torch.Tensor | None = None, *, rope_cs: torch.Tensor | None = None,
+                 positions: torch.Tensor | None = None, tokens_per_tile: int | None = None, hw: int | None = None,
+                 eps: float = 1e-6, interleaved: bool = True, out=None):
+    """RMS norm of every q and k head and the rotary turn behind it, in one pass over both: returns (q', k') with
+    x' = R (x * rsqrt(mean(x^2) + eps) * weight).
+
+    q [..., heads_q, head_dim], k [..., heads_k, head_dim]: bfloat16 or float16, the same tokens, views of a packed qkv
+    matrix included; head_dim a multiple of 8 up to 256. q_weight, k_weight: [head_dim] fp32, or None for a plain norm.
+    rope_cs [..., rot / 2, 2]: (cos, sin) rows, float16 (rope.pack_rope_tables) or float32, None for the norm alone; the
+    first rot <= head_dim channels turn in pairs of neighbours (interleaved, rot a multiple of 8) or of the two halves
+    of rot (a multiple of 16). A token's row: positions [tokens] (int32 / int64; negative: a padding token, its outputs
+    are zero; one behind the table gives NaN and device status 107), else as in qkv_rope
+    m // tokens_per_tile * hw + m % hw (default: token m has row m). out: (q', k') to write to, q and k themselves
+    allowed. The gradients are qk_norm_rope_backward's; torch.ops.strata_b200.qk_norm_rope is the differentiable form."""
+    dtype = _require_16bit(q, "q")
+    hq, hk, hd, M, keep, args = _qk_arguments(q, k, q_weight, k_weight, rope_cs, positions, tokens_per_tile, hw,
+                                              interleaved)
+    if out is None:
+        yq, yk = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=q.dtype, device=q.device)
+    else:
+        yq, yk = out
+    if not M:
+        return yq, yk
+    q3, q_desc = _heads(q, "q", tuple(q.shape), q)
+    k3, k_desc = _heads(k, "k", tuple(k.shape), q)
+    yq_desc, yk_desc = _heads_out(yq, "out[0]", tuple(q.shape), q), _heads_out(yk, "out[1]", tuple(k.shape), q)
+    with _lib.on_device(q):
+        _lib.check(_lib.load().strata_qk_norm_rope(
+            q_desc, k_desc, yq_desc, yk_desc, None if keep[0] is None else keep[0].data_ptr(),
+            None if keep[1] is None else keep[1].data_ptr(), hq, hk, hd, *args, M, float(eps), dtype, _stream_ptr(q)),
+            "strata_qk_norm_rope")
+    return yq, yk
+
+
+def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
+                          q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, *,
+                          rope_cs: torch.Tensor | None = None, positions: torch.Tensor | None = None,
+                          tokens_per_tile: int | None = None, hw: int | None = None, eps: float = 1e-6,
+                          interleaved: bool = True):
+    """Gradients of qk_norm_rope at (dq, dk) of its outputs: (dq_in, dk_in, dq_weight, dk_weight); q, k and the rest as
+    it was called. The weights' are fp32 [head_dim], summed over tokens and heads without atomics (None without
+    weights). A padding token has no gradient and no part in the weights'."""
+    dtype = _require_16bit(q, "q")
+    hq, hk, hd, M, keep, args = _qk_arguments(q, k, q_weight, k_weight, rope_cs, positions, tokens_per_tile, hw,
+                                              interleaved)
+    new = lambda t: torch.empty(t.shape, dtype=q.dtype, device=q.device)
+    xq, xk = new(q), new(k)
+    f32 = dict(dtype=torch.float32, device=q.device)
+    wq = None if q_weight is None else torch.empty(hd, **f32)
+    wk = None if k_weight is None else torch.empty(hd, **f32)
+    lib = _lib.load()
+    q3, q_desc = _heads(q, "q", tuple(q.shape), q)
+    k3, k_desc = _heads(k, "k", tuple(k.shape), q)
+    dq3, dq_desc = _heads(dq, "dq", tuple(q.shape), q)
+    dk3, dk_desc = _heads(dk, "dk", tuple(k.shape), q)
+    xq_desc, xk_desc = _heads(xq, "dq_in", tuple(q.shape), q)[1], _heads(xk, "dk_in", tuple(k.shape), q)[1]
+    p = lambda t: None if t is None else t.data_ptr()
+    with _lib.on_device(q):
+        need, ws = 0, None
+        if M and (wq is not None or wk is not None):
+            need = lib.strata_qk_norm_rope_backward_workspace_bytes(M, hq + hk, hd)
+            ws = _scratch(need, q.device)
+        _lib.check(lib.strata_qk_norm_rope_backward(
+            dq_desc, dk_desc, q_desc, k_desc, xq_desc, xk_desc, p(keep[0]), p(keep[1]), p(wq), p(wk), hq, hk, hd, *args,
+            M, float(eps), dtype, p(ws), need, _stream_ptr(q)), "strata_qk_norm_rope_backward")
+    return xq, xk, wq, wk
 
 
 def adaln_cond(tokens: torch.Tensor, w_dw: torch.Tensor, b_dw: torch.Tensor | None, factor: int,

@@ -15,7 +15,14 @@ references); its weights are read from the module when the operator runs, they a
 arguments (inference only: there is no backward).
 
 Finer-grained operators over the C ABI (`strata_b200::block_forward`, `::na3d`, `::linear`,
-`::layernorm`) are registered the same way for callers that assemble their own graphs.
+`::layernorm`) are registered the same way for callers that assemble their own graphs. Two of
+them have gradients, for fine-tuning: `::linear_act` (a dense layer with its activation and residual) and
+`::qk_norm_rope` (the norm and rotation of query and key heads).
+
+Capturing a training step in a CUDA graph: torch ties a leaf's gradient accumulation to the stream on which its first
+living graph was built, and a captured backward pass that meets an accumulation of another stream ends the
+process. The two operators refuse the case they can see: a forward pass under capture whose leaves still have an eager
+graph of these operators on another stream (delete the losses and outputs of warm-up steps first).
 """
 from __future__ import annotations
 
@@ -126,3 +133,146 @@ def block_forward(x: torch.Tensor, weights: Sequence[torch.Tensor], biases: Sequ
 @block_forward.register_fake
 def _block_forward_fake(x, weights, biases, grid, num_heads, kernel, rope_cs, qk_norm):
     return torch.empty_like(x)
+
+
+# ------------------------------------------------------------------ operators with gradients
+_STREAM_TAG = "strata_b200.stream"
+
+
+def claim_leaves(next_functions, stream: int, capturing: bool) -> None:
+    """next_functions: those of a node of the graph that is being built. Notes with each leaf's gradient accumulation on
+    which stream this forward pass runs, as long as a graph keeps the accumulation alive; refuses a captured pass over
+    leaves whose accumulation belongs to another stream."""
+    for node, _ in next_functions:
+        if not hasattr(node, "variable"):         # only accumulations have one
+            continue
+        if node.metadata.setdefault(_STREAM_TAG, stream) != stream and capturing:
+            raise RuntimeError(
+                "this forward pass is being captured, but an eager graph of the same leaves is alive on another stream: "
+                "its backward pass could not be captured. Delete what the eager passes returned (outputs, losses) first")
+
+
+def _claim(ctx, x) -> None:
+    from . import _lib
+    if x.is_cuda and not isinstance(x, torch._subclasses.FakeTensor):
+        claim_leaves(getattr(ctx, "next_functions", ()), _lib.stream_of(x), torch.cuda.is_current_stream_capturing())
+
+
+@torch.library.custom_op("strata_b200::linear_act", mutates_args=())
+def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: str = "none",
+               residual: Optional[torch.Tensor] = None, save_preact: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """(y, z) of ops.linear_act; z has no elements unless save_preact. Differentiable in x, weight, bias and residual;
+    without save_preact the backward pass computes z again. z itself is not differentiable."""
+    from . import ops
+    if save_preact:
+        return ops.linear_act(x, weight, bias, activation, residual, save_preact=True)
+    return ops.linear_act(x, weight, bias, activation, residual), x.new_empty(0)
+
+
+@linear_act.register_fake
+def _linear_act_fake(x, weight, bias=None, activation="none", residual=None, save_preact=False):
+    y = x.new_empty((*x.shape[:-1], weight.shape[0]))
+    return y, torch.empty_like(y) if save_preact else x.new_empty(0)
+
+
+@torch.library.custom_op("strata_b200::linear_act_backward", mutates_args=())
+def linear_act_backward(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, activation: str,
+                        preact: Optional[torch.Tensor], need_x: bool, need_weight: bool,
+                        need_bias: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """ops.linear_act_backward; gradients that are not needed have no elements."""
+    from . import ops
+    got = ops.linear_act_backward(grad, x, weight, activation, preact, need_x=need_x, need_weight=need_weight,
+                                  need_bias=need_bias)
+    return tuple(x.new_empty(0) if t is None else t for t in got)
+
+
+@linear_act_backward.register_fake
+def _linear_act_backward_fake(grad, x, weight, activation, preact, need_x, need_weight, need_bias):
+    return (x.new_empty(x.shape if need_x else 0), weight.new_empty(weight.shape if need_weight else 0),
+            weight.new_empty(weight.shape[0] if need_bias else 0, dtype=torch.float32 if need_bias else x.dtype))
+
+
+def _linear_act_context(ctx, inputs, output):
+    x, weight, bias, activation, residual, save_preact = inputs
+    _claim(ctx, x)
+    ctx.set_materialize_grads(False)
+    ctx.mark_non_differentiable(output[1])
+    again = activation != "none" and not save_preact
+    ctx.save_for_backward(x, weight, bias if again else None, output[1] if save_preact else None)
+    ctx.activation, ctx.again = activation, again
+
+
+def _each(ctx, grads):
+    """One gradient for each argument that the call gave (defaults it left out have none)."""
+    need = ctx.needs_input_grad
+    return tuple(g if n else None for g, n in zip(grads, need)) + (None,) * (len(need) - len(grads))
+
+
+def _linear_act_grad(ctx, dy, _dz):
+    if dy is None:
+        return _each(ctx, ())
+    x, weight, bias, z = ctx.saved_tensors
+    if ctx.again:
+        z = torch.ops.strata_b200.linear_act(x, weight, bias, "none", None, False)[0]
+    need = (*ctx.needs_input_grad, False)
+    dx = dw = db = None
+    if need[0] or need[1] or need[2]:
+        dx, dw, db = torch.ops.strata_b200.linear_act_backward(
+            dy, x, weight, ctx.activation, None if ctx.activation == "none" else z, need[0], need[1], need[2])
+    return _each(ctx, (dx, dw, db, None, dy))
+
+
+linear_act.register_autograd(_linear_act_grad, setup_context=_linear_act_context)
+
+
+@torch.library.custom_op("strata_b200::qk_norm_rope", mutates_args=())
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor] = None,
+                 k_weight: Optional[torch.Tensor] = None, rope_cs: Optional[torch.Tensor] = None,
+                 positions: Optional[torch.Tensor] = None, tokens_per_tile: Optional[int] = None,
+                 hw: Optional[int] = None, eps: float = 1e-6,
+                 interleaved: bool = True) -> tuple[torch.Tensor, torch.Tensor]:
+    """ops.qk_norm_rope, differentiable in q, k and the two weights."""
+    from . import ops
+    return ops.qk_norm_rope(q, k, q_weight, k_weight, rope_cs=rope_cs, positions=positions,
+                            tokens_per_tile=tokens_per_tile, hw=hw, eps=eps, interleaved=interleaved)
+
+
+@qk_norm_rope.register_fake
+def _qk_norm_rope_fake(q, k, q_weight=None, k_weight=None, rope_cs=None, positions=None, tokens_per_tile=None, hw=None,
+                       eps=1e-6, interleaved=True):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+@torch.library.custom_op("strata_b200::qk_norm_rope_backward", mutates_args=())
+def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
+                          q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
+                          rope_cs: Optional[torch.Tensor], positions: Optional[torch.Tensor],
+                          tokens_per_tile: Optional[int], hw: Optional[int], eps: float,
+                          interleaved: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """ops.qk_norm_rope_backward; the gradient of a weight that is not there has no elements."""
+    from . import ops
+    got = ops.qk_norm_rope_backward(dq, dk, q, k, q_weight, k_weight, rope_cs=rope_cs, positions=positions,
+                                    tokens_per_tile=tokens_per_tile, hw=hw, eps=eps, interleaved=interleaved)
+    return tuple(q.new_empty(0, dtype=torch.float32) if t is None else t for t in got)
+
+
+@qk_norm_rope_backward.register_fake
+def _qk_norm_rope_backward_fake(dq, dk, q, k, q_weight, k_weight, rope_cs, positions, tokens_per_tile, hw, eps,
+                                interleaved):
+    w = lambda t: q.new_empty(0 if t is None else q.shape[-1], dtype=torch.float32)
+    return q.new_empty(q.shape), k.new_empty(k.shape), w(q_weight), w(k_weight)
+
+
+def _qk_norm_rope_context(ctx, inputs, output):
+    q, k, q_weight, k_weight, rope_cs, positions, *ctx.rest = inputs
+    _claim(ctx, q)
+    ctx.save_for_backward(q, k, q_weight, k_weight, rope_cs, positions)
+
+
+def _qk_norm_rope_grad(ctx, dq, dk):
+    q, k, q_weight, k_weight, rope_cs, positions = ctx.saved_tensors
+    got = torch.ops.strata_b200.qk_norm_rope_backward(dq, dk, q, k, q_weight, k_weight, rope_cs, positions, *ctx.rest)
+    return _each(ctx, got)
+
+
+qk_norm_rope.register_autograd(_qk_norm_rope_grad, setup_context=_qk_norm_rope_context)

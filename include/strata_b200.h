@@ -300,37 +300,33 @@ int strata_adaln_rows_bf16(const void* x, int64_t ldx, const void* y, int64_t ld
  * (qk_norm_pixel of screamcast/strata_wrappers.py:437, non-affine). */
 int strata_qk_norm_rows_bf16(void* qkv, int64_t ld, int64_t M, int C, float eps, void* stream);
 
-/* q and k heads of M tokens, one entry for each: element (m, head, c) at base + m*stride_token + head*stride_head + c,
- * strides in elements, multiples of 8; bases 16-byte aligned. */
-typedef struct strata_heads {
-  void* data;
-  int64_t stride_token, stride_head;
-} strata_heads;
-
-/* Per-head RMS norm and rotation of q and k in one pass: y = R (x (mean x^2 + eps)^-1/2 w), for `heads_q` and `heads_k`
- * heads of head_dim channels (a multiple of 8, at most 256) in one 16-bit type. w_q, w_k: [head_dim] fp32 or NULL.
- * R turns the first `rot` channels of a head by the (cos, sin) pairs of the token's row of table [table_rows, rot/2]
- * (IEEE half, or float with table_f32; 16-byte aligned; NULL: no rotation): pairs (2i, 2i+1) with `adjacent`, rot a
- * multiple of 8, else (i, i + rot/2), rot a multiple of 16. The row is positions[m] (int32, or int64 with
- * positions_64); without positions m / tokens_per_tile * hw + m % hw, which has to stay below table_rows. A negative
- * position is padding: its outputs are zero. One behind the table gives NaN and device status 107. y may be x.
+/* Per-head RMS norm and rotation of q and k in one pass: y = R (x (mean x^2 + eps)^-1/2 w), for M tokens of heads_q and
+ * heads_k heads of head_dim channels (a multiple of 8, at most 256) in one 16-bit type. Element (m, head, c) of an
+ * operand lies at base + m*st + head*sh + c; strides in elements, multiples of 8, bases 16-byte aligned. w_q, w_k:
+ * [head_dim] fp32 or NULL. R turns the first `rot` channels of a head by the (cos, sin) pairs of the token's row of
+ * table [table_rows, rot/2] (IEEE half, or float with table_f32; 16-byte aligned; NULL: no rotation): pairs (2i, 2i+1)
+ * with `adjacent`, rot a multiple of 8, else (i, i + rot/2), rot a multiple of 16. The row is positions[m] (int32, or
+ * int64 with positions_64); without positions m / tokens_per_tile * hw + m % hw, which has to stay below table_rows. A
+ * negative position is padding: its outputs are zero. One behind the table gives NaN and device status 107. y may be x.
  * The q/k norm and rotation of strata_qkv_rope_bf16 and strata_qk_norm_rows_bf16 for projections made elsewhere, with
  * affine weights, shared key heads and other widths. */
-int strata_qk_norm_rope(const strata_heads* h_q, const strata_heads* h_k, const strata_heads* h_q_out,
-                        const strata_heads* h_k_out, const float* w_q, const float* w_k, int heads_q, int heads_k,
-                        int head_dim, int rot, int adjacent, const void* table, int table_f32, int table_rows,
-                        const void* positions, int positions_64, int tokens_per_tile, int hw, int64_t M, float eps,
-                        int dtype, void* stream);
-/* Its gradients from dq, dk: dx of q and k, and dw_q, dw_k [head_dim] fp32 (NULL where there are no weights). dw is
- * summed without atomics: the same bits every time. workspace: strata_qk_norm_rope_backward_workspace_bytes bytes,
- * 16-byte aligned (NULL without dw). */
+int strata_qk_norm_rope(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh, void* yq,
+                        int64_t yq_st, int64_t yq_sh, void* yk, int64_t yk_st, int64_t yk_sh, const float* w_q,
+                        const float* w_k, int heads_q, int heads_k, int head_dim, int rot, int adjacent,
+                        const void* table, int table_f32, int table_rows, const void* positions, int positions_64,
+                        int tokens_per_tile, int hw, int64_t M, float eps, int dtype, void* stream);
+/* Its gradients from those of its outputs (dyq, dyk): dxq, dxk of q and k, and dw_q, dw_k [head_dim] fp32 (NULL where
+ * there are no weights), summed without atomics: the same bits every time. workspace:
+ * strata_qk_norm_rope_backward_workspace_bytes bytes, 16-byte aligned (NULL without dw). */
 int64_t strata_qk_norm_rope_backward_workspace_bytes(int64_t M, int heads, int head_dim);
-int strata_qk_norm_rope_backward(const strata_heads* h_dq, const strata_heads* h_dk, const strata_heads* h_q,
-                                 const strata_heads* h_k, const strata_heads* h_dq_in, const strata_heads* h_dk_in,
-                                 const float* w_q, const float* w_k, float* dw_q, float* dw_k, int heads_q, int heads_k,
-                                 int head_dim, int rot, int adjacent, const void* table, int table_f32, int table_rows,
-                                 const void* positions, int positions_64, int tokens_per_tile, int hw, int64_t M,
-                                 float eps, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+int strata_qk_norm_rope_backward(const void* dyq, int64_t dyq_st, int64_t dyq_sh, const void* dyk, int64_t dyk_st,
+                                 int64_t dyk_sh, const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st,
+                                 int64_t k_sh, void* dxq, int64_t dxq_st, int64_t dxq_sh, void* dxk, int64_t dxk_st,
+                                 int64_t dxk_sh, const float* w_q, const float* w_k, float* dw_q, float* dw_k,
+                                 int heads_q, int heads_k, int head_dim, int rot, int adjacent, const void* table,
+                                 int table_f32, int table_rows, const void* positions, int positions_64,
+                                 int tokens_per_tile, int hw, int64_t M, float eps, int dtype, void* workspace,
+                                 int64_t workspace_bytes, void* stream);
 
 /* Conditioning rows of the "bilinear_dw" AdaLN mode (screamcast/strata_wrappers.py:491-495;
  * parameters adaln_bilinear_dw_conv.{weight,bias} of the parameter manifest

@@ -24,11 +24,6 @@ class BlockWeights(Structure):
                                         "w_fc1", "b_fc1", "w_fc2", "b_fc2")]
 
 
-class Heads(Structure):
-    """struct strata_heads (a device pointer and two element strides)."""
-    _fields_ = [("data", c_void_p), ("stride_token", c_int64), ("stride_head", c_int64)]
-
-
 class BackboneDesc(Structure):
     """struct strata_backbone_desc."""
     _fields_ = ([(n, c_int32) for n in ("in_channels", "out_channels", "patch_v", "patch_h", "patch_w",
@@ -117,11 +112,11 @@ _SIGNATURES = {
                                        c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p,
                                        c_int64, c_int, c_int, c_float, c_void_p]),
     "strata_qk_norm_rows_bf16": (c_int, [c_void_p, c_int64, c_int64, c_int, c_float, c_void_p]),
-    "strata_qk_norm_rope": (c_int, [POINTER(Heads)] * 4 + [c_void_p] * 2 + [c_int] * 5
+    "strata_qk_norm_rope": (c_int, [c_void_p, c_int64, c_int64] * 4 + [c_void_p] * 2 + [c_int] * 5
                             + [c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_int, c_int64, c_float, c_int,
                                c_void_p]),
     "strata_qk_norm_rope_backward_workspace_bytes": (c_int64, [c_int64, c_int, c_int]),
-    "strata_qk_norm_rope_backward": (c_int, [POINTER(Heads)] * 6 + [c_void_p] * 4 + [c_int] * 5
+    "strata_qk_norm_rope_backward": (c_int, [c_void_p, c_int64, c_int64] * 6 + [c_void_p] * 4 + [c_int] * 5
                                      + [c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_int, c_int64, c_float, c_int,
                                         c_void_p, c_int64, c_void_p]),
     "strata_adaln_cond_bf16": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,

@@ -986,16 +986,14 @@ static int strata_adaln_cond_ready_bf16(const void* tokens, int B, int D, int h,
   return r == -2 ? STRATA_ERR_ARG : r;
 }
 
-static bool qk_heads_ok(const strata_heads* t, int head_dim) {
-  return t && t->data && aligned16(t->data) && t->stride_token % 8 == 0 && t->stride_head % 8 == 0 &&
-         t->stride_token >= 0 && t->stride_head >= 0 && head_dim > 0;
+static bool qk_heads_ok(const QkTensor& t) {
+  return t.p && aligned16(t.p) && t.token >= 0 && t.head >= 0 && (t.token | t.head) % 8 == 0;
 }
 
-// Checks what both directions share and fills p; out: the tensors that are written.
-static int qk_params(QkParams& p, const strata_heads* q, const strata_heads* k, const strata_heads* yq,
-                     const strata_heads* yk, const float* w_q, const float* w_k, int heads_q, int heads_k, int head_dim,
-                     int rot, int adjacent, const void* table, int table_f32, int table_rows, const void* positions,
-                     int positions_64, int tokens_per_tile, int hw, int64_t M, float eps, int dtype) {
+// Checks what both directions share and fills in the rest of p (its tensors are set).
+static int qk_params(QkParams& p, int heads_q, int heads_k, int head_dim, int rot, int adjacent, const void* table,
+                     int table_f32, int table_rows, const void* positions, int positions_64, int tokens_per_tile, int hw,
+                     int64_t M, float eps, int dtype) {
   if (M < 0 || M > 0x7FFF0000 || heads_q <= 0 || heads_k <= 0 || heads_q > 65536 || heads_k > 65536 || head_dim <= 0 ||
       (dtype != STRATA_BF16 && dtype != STRATA_F16))
     return STRATA_ERR_ARG;
@@ -1003,21 +1001,16 @@ static int qk_params(QkParams& p, const strata_heads* q, const strata_heads* k, 
   if (table) {
     if (rot <= 0 || rot > head_dim || table_rows <= 0 || !aligned16(table)) return STRATA_ERR_ARG;
     if (rot % (adjacent ? 8 : 16) != 0) return STRATA_ERR_UNSUPPORTED;
-    if (!positions && M > 0) {
+    if (!positions) {
       if (tokens_per_tile <= 0 || hw <= 0) return STRATA_ERR_ARG;
       // the largest row of the rule
-      const int64_t tile = (M - 1) / tokens_per_tile;
-      if (tile * hw + (M < hw ? M : hw) - 1 >= table_rows) return STRATA_ERR_ARG;
+      if ((M - 1) / tokens_per_tile * hw + (M < hw ? M : hw) - 1 >= table_rows) return STRATA_ERR_ARG;
     }
     if (positions && (reinterpret_cast<uintptr_t>(positions) & (positions_64 ? 7u : 3u)) != 0) return STRATA_ERR_ARG;
   }
-  if (!qk_heads_ok(q, head_dim) || !qk_heads_ok(k, head_dim) || !qk_heads_ok(yq, head_dim) ||
-      !qk_heads_ok(yk, head_dim) || ((reinterpret_cast<uintptr_t>(w_q) | reinterpret_cast<uintptr_t>(w_k)) & 3u) != 0)
-    return STRATA_ERR_ARG;
-  auto of = [](const strata_heads* t) { return QkTensor{t->data, t->stride_token, t->stride_head}; };
-  p.x[0] = of(q); p.x[1] = of(k);
-  p.y[0] = of(yq); p.y[1] = of(yk);
-  p.w[0] = w_q; p.w[1] = w_k;
+  for (int i = 0; i < 2; ++i)
+    if (!qk_heads_ok(p.x[i]) || !qk_heads_ok(p.y[i]) || (reinterpret_cast<uintptr_t>(p.w[i]) & 3u) != 0)
+      return STRATA_ERR_ARG;
   p.heads[0] = heads_q; p.heads[1] = heads_k;
   p.head_dim = head_dim; p.rot = table ? rot : 0;
   p.table = table; p.table_f32 = table_f32; p.table_rows = table_rows;
@@ -1027,17 +1020,20 @@ static int qk_params(QkParams& p, const strata_heads* q, const strata_heads* k, 
   return STRATA_OK;
 }
 
-int strata_qk_norm_rope(const strata_heads* h_q, const strata_heads* h_k, const strata_heads* h_q_out,
-                        const strata_heads* h_k_out, const float* w_q, const float* w_k, int heads_q, int heads_k,
-                        int head_dim, int rot, int adjacent, const void* table, int table_f32, int table_rows,
-                        const void* positions, int positions_64, int tokens_per_tile, int hw, int64_t M, float eps,
-                        int dtype, void* stream) {
+int strata_qk_norm_rope(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh, void* yq,
+                        int64_t yq_st, int64_t yq_sh, void* yk, int64_t yk_st, int64_t yk_sh, const float* w_q,
+                        const float* w_k, int heads_q, int heads_k, int head_dim, int rot, int adjacent,
+                        const void* table, int table_f32, int table_rows, const void* positions, int positions_64,
+                        int tokens_per_tile, int hw, int64_t M, float eps, int dtype, void* stream) {
   const int sms = current_sm_count();
   if (sms <= 0) return STRATA_ERR_NO_DEVICE;
   if (M == 0) return STRATA_OK;
   QkParams p{};
-  const int r = qk_params(p, h_q, h_k, h_q_out, h_k_out, w_q, w_k, heads_q, heads_k, head_dim, rot, adjacent, table,
-                          table_f32, table_rows, positions, positions_64, tokens_per_tile, hw, M, eps, dtype);
+  p.x[0] = {q, q_st, q_sh}; p.x[1] = {k, k_st, k_sh};
+  p.y[0] = {yq, yq_st, yq_sh}; p.y[1] = {yk, yk_st, yk_sh};
+  p.w[0] = w_q; p.w[1] = w_k;
+  const int r = qk_params(p, heads_q, heads_k, head_dim, rot, adjacent, table, table_f32, table_rows, positions,
+                          positions_64, tokens_per_tile, hw, M, eps, dtype);
   if (r != STRATA_OK) return r;
   return launch_qk<false>(p, adjacent != 0, dtype == STRATA_F16, qk_blocks(M, heads_q + heads_k, head_dim, false, sms),
                           as_stream(stream));
@@ -1050,16 +1046,18 @@ int64_t strata_qk_norm_rope_backward_workspace_bytes(int64_t M, int heads, int h
   return qk_blocks(M, heads, head_dim, true, sms) * 2 * head_dim * 4;
 }
 
-int strata_qk_norm_rope_backward(const strata_heads* h_dq, const strata_heads* h_dk, const strata_heads* h_q,
-                                 const strata_heads* h_k, const strata_heads* h_dq_in, const strata_heads* h_dk_in,
-                                 const float* w_q, const float* w_k, float* dw_q, float* dw_k, int heads_q, int heads_k,
-                                 int head_dim, int rot, int adjacent, const void* table, int table_f32, int table_rows,
-                                 const void* positions, int positions_64, int tokens_per_tile, int hw, int64_t M,
-                                 float eps, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+int strata_qk_norm_rope_backward(const void* dyq, int64_t dyq_st, int64_t dyq_sh, const void* dyk, int64_t dyk_st,
+                                 int64_t dyk_sh, const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st,
+                                 int64_t k_sh, void* dxq, int64_t dxq_st, int64_t dxq_sh, void* dxk, int64_t dxk_st,
+                                 int64_t dxk_sh, const float* w_q, const float* w_k, float* dw_q, float* dw_k,
+                                 int heads_q, int heads_k, int head_dim, int rot, int adjacent, const void* table,
+                                 int table_f32, int table_rows, const void* positions, int positions_64,
+                                 int tokens_per_tile, int hw, int64_t M, float eps, int dtype, void* workspace,
+                                 int64_t workspace_bytes, void* stream) {
   const int sms = current_sm_count();
   if (sms <= 0) return STRATA_ERR_NO_DEVICE;
   const cudaStream_t st = as_stream(stream);
-  if (M == 0) {
+  if (M == 0) {      // sums over no tokens
     if (head_dim <= 0 || head_dim > 256) return STRATA_ERR_ARG;
     cudaError_t e = cudaSuccess;
     if (dw_q) e = cudaMemsetAsync(dw_q, 0, static_cast<size_t>(head_dim) * 4, st);
@@ -1067,12 +1065,14 @@ int strata_qk_norm_rope_backward(const strata_heads* h_dq, const strata_heads* h
     return e == cudaSuccess ? STRATA_OK : -static_cast<int>(e) - 1000;
   }
   QkParams p{};
-  int r = qk_params(p, h_q, h_k, h_dq_in, h_dk_in, w_q, w_k, heads_q, heads_k, head_dim, rot, adjacent, table, table_f32,
-                    table_rows, positions, positions_64, tokens_per_tile, hw, M, eps, dtype);
+  p.x[0] = {q, q_st, q_sh}; p.x[1] = {k, k_st, k_sh};
+  p.y[0] = {dxq, dxq_st, dxq_sh}; p.y[1] = {dxk, dxk_st, dxk_sh};
+  p.dy[0] = {dyq, dyq_st, dyq_sh}; p.dy[1] = {dyk, dyk_st, dyk_sh};
+  p.w[0] = w_q; p.w[1] = w_k;
+  int r = qk_params(p, heads_q, heads_k, head_dim, rot, adjacent, table, table_f32, table_rows, positions, positions_64,
+                    tokens_per_tile, hw, M, eps, dtype);
   if (r != STRATA_OK) return r;
-  if (!qk_heads_ok(h_dq, head_dim) || !qk_heads_ok(h_dk, head_dim)) return STRATA_ERR_ARG;
-  p.dy[0] = {h_dq->data, h_dq->stride_token, h_dq->stride_head};
-  p.dy[1] = {h_dk->data, h_dk->stride_token, h_dk->stride_head};
+  if (!qk_heads_ok(p.dy[0]) || !qk_heads_ok(p.dy[1])) return STRATA_ERR_ARG;
   const long long blocks = qk_blocks(M, heads_q + heads_k, head_dim, true, sms);
   if (dw_q || dw_k) {
     if (!workspace || !aligned16(workspace) || workspace_bytes < blocks * 2 * head_dim * 4) return STRATA_ERR_ARG;

@@ -26,8 +26,8 @@ inline int dense_pairs(int sms) {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return sms / 2;
   int fit = cached[dev].load(std::memory_order_relaxed);
   if (fit != 0) return fit;
-  using S = DenseSmem<256, true, DENSE_Y>;
-  auto kern = dense_tcgen05_kernel<256, true, DENSE_NT, DENSE_Y, __nv_bfloat16>;
+  using S = DenseSmem<256, true, DENSE_Y, false>;
+  auto kern = dense_tcgen05_kernel<256, true, DENSE_NT, DENSE_Y, __nv_bfloat16, ACT_ANY, false>;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(sms & ~1));
   cfg.blockDim = dim3(GEMM_THREADS);
@@ -85,7 +85,7 @@ inline DenseChoice dense_choice(int M, int N, int K, int sms) {
 // ---------------------------------------------------------------- launches
 struct DenseOperand { const void* p; long long ld; };
 
-template <int BN, bool PAIR, int LAY, int EPI, typename T>
+template <int BN, bool PAIR, int LAY, int EPI, typename T, int ACT = ACT_ANY, bool AUX = false>
 inline int launch_dense_t(const DenseOperand& A, const DenseOperand& B, const DenseParams& p, int units, cudaStream_t st) {
   const bool a_mn = LAY == DENSE_TN, b_mn = LAY != DENSE_NT;
   constexpr int TILE_M = PAIR ? 2 * GEMM_BM : GEMM_BM;
@@ -100,13 +100,14 @@ inline int launch_dense_t(const DenseOperand& A, const DenseOperand& B, const De
   if (map(&tmB, B, b_mn ? p.K : p.N, b_mn ? p.N : p.K, 64, b_mn ? 64 : (PAIR ? BN / 2 : BN), TMAP_SWIZZLE_128B) != 0)
     return -21;
   tmOut = tmKeep = tmAux = tmA;
+  using S = DenseSmem<BN, PAIR, EPI, AUX && EPI == DENSE_Y>;
+  constexpr TmapSwizzle sw = S::BOX_COLS == 64 ? TMAP_SWIZZLE_128B : TMAP_SWIZZLE_64B;
   if (EPI != DENSE_PART && !p.direct) {
-    if (map(&tmOut, {p.out, p.ldo}, p.M, p.N, 32, 32, TMAP_SWIZZLE_64B) != 0) return -22;
-    if (p.aux && map(&tmAux, {p.aux, p.ldaux}, p.M, p.N, 32, 32, TMAP_SWIZZLE_64B) != 0) return -23;
-    if (p.keep && map(&tmKeep, {p.keep, p.ldk}, p.M, p.N, 32, 32, TMAP_SWIZZLE_64B) != 0) return -25;
+    if (map(&tmOut, {p.out, p.ldo}, p.M, p.N, S::BOX_COLS, 32, sw) != 0) return -22;
+    if (p.aux && map(&tmAux, {p.aux, p.ldaux}, p.M, p.N, S::BOX_COLS, 32, sw) != 0) return -23;
+    if (p.keep && map(&tmKeep, {p.keep, p.ldk}, p.M, p.N, S::BOX_COLS, 32, sw) != 0) return -25;
   }
-  using S = DenseSmem<BN, PAIR, EPI>;
-  auto kern = dense_tcgen05_kernel<BN, PAIR, LAY, EPI, T>;
+  auto kern = dense_tcgen05_kernel<BN, PAIR, LAY, EPI, T, ACT, AUX>;
   static std::atomic<uint64_t> smem_set;
   if (const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), S::TOTAL, smem_set); e != cudaSuccess)
     return -static_cast<int>(e) - 1000;
@@ -118,9 +119,28 @@ inline int launch_dense_t(const DenseOperand& A, const DenseOperand& B, const De
                         PAIR ? 2 : 1, tmA, tmB, tmOut, tmKeep, tmAux, p);
 }
 
+// Forward pass on pairs of CTAs: a kernel for each activation, with and without a residual. One kernel that reads both
+// from its parameters keeps the registers of all of them (TODO figures).
+template <int EPI, typename T, bool AUX>
+inline int launch_dense_pair(const DenseOperand& A, const DenseOperand& B, const DenseParams& p, int units,
+                             cudaStream_t st) {
+  switch (p.act) {
+    case ACT_GELU: return launch_dense_t<256, true, DENSE_NT, EPI, T, ACT_GELU, AUX>(A, B, p, units, st);
+    case ACT_GELU_TANH: return launch_dense_t<256, true, DENSE_NT, EPI, T, ACT_GELU_TANH, AUX>(A, B, p, units, st);
+    case ACT_SILU: return launch_dense_t<256, true, DENSE_NT, EPI, T, ACT_SILU, AUX>(A, B, p, units, st);
+    case ACT_RELU: return launch_dense_t<256, true, DENSE_NT, EPI, T, ACT_RELU, AUX>(A, B, p, units, st);
+    default: return launch_dense_t<256, true, DENSE_NT, EPI, T, ACT_NONE, AUX>(A, B, p, units, st);
+  }
+}
+
 template <int LAY, int EPI, typename T>
 inline int launch_dense_bn(int bn, const DenseOperand& A, const DenseOperand& B, const DenseParams& p, int units,
                            cudaStream_t st) {
+  if constexpr (LAY == DENSE_NT && EPI != DENSE_PART) {
+    if (bn == 256 && !p.direct)
+      return p.aux ? launch_dense_pair<EPI, T, true>(A, B, p, units, st)
+                   : launch_dense_pair<EPI, T, false>(A, B, p, units, st);
+  }
   if (bn == 256) return launch_dense_t<256, true, LAY, EPI, T>(A, B, p, units, st);
   if (bn == 128) return launch_dense_t<128, false, LAY, EPI, T>(A, B, p, units, st);
   return launch_dense_t<64, false, LAY, EPI, T>(A, B, p, units, st);

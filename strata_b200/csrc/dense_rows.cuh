@@ -96,7 +96,7 @@ __global__ void __launch_bounds__(256) dense_few_rows_kernel(const T* __restrict
   if (p.bias != nullptr) z += __ldg(p.bias + col);
   if (p.keep != nullptr) static_cast<T*>(p.keep)[row * p.ldk + col] = from_f32<T>(z);
   uint64_t y[1] = {pack2(z, 0.f)};
-  dense_act(p.act, y);
+  dense_act<T>(p.act, y);
   float a, b;
   unpack2(y[0], a, b);
   if (p.aux != nullptr) a += to_f32<T>(static_cast<const T*>(p.aux)[row * p.ldaux + col]);

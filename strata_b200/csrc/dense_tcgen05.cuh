@@ -39,14 +39,17 @@ struct DenseParams {
   DensePlan plan;
 };
 
-template <int BN, bool PAIR, int EPI>
+// AHEAD: the residual of the next tile is loaded while this one is computed.
+template <int BN, bool PAIR, int EPI, bool AHEAD>
 struct DenseSmem {
   static constexpr int A_BYTES = GEMM_BM * GEMM_BK * 2;
   static constexpr int B_BYTES = (PAIR ? BN / 2 : BN) * GEMM_BK * 2;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int BOX_BYTES = 32 * 32 * 2;
-  static constexpr int BOXES = EPI == DENSE_PART ? 0 : EPI == DENSE_Y_KEEP ? 2 : 1;   // staging boxes of a warp
-  static constexpr int STAGES = BOXES == 2 ? 5 : 6;
+  // staging boxes of a warp: 32 rows of 32 columns, or of all its columns of a tile
+  static constexpr int BOX_COLS = AHEAD && BN == 256 ? 64 : 32;
+  static constexpr int BOX_BYTES = 32 * BOX_COLS * 2;
+  static constexpr int BOXES = EPI == DENSE_PART ? 0 : EPI == DENSE_Y_KEEP ? 2 : 1;
+  static constexpr int STAGES = BN > 64 && BOXES * BOX_BYTES > 2048 ? 5 : 6;
   static constexpr int STAGING_OFF = STAGES * STAGE_BYTES;
   static constexpr int BAR_OFF = STAGING_OFF + GEMM_EPI_WARPS * BOXES * BOX_BYTES;
   static constexpr int TOTAL = BAR_OFF + 512 + 1024;            // + alignment slack
@@ -94,15 +97,19 @@ __device__ __forceinline__ void dense_lane_bias(const DenseParams& p, int n0, in
   }
 }
 
-template <int BN, bool PAIR, int LAY, int EPI, typename T>
+// ACT: the activation, AUX: whether there is a residual; ACT_ANY: both, and how the rows are stored, are read from p.
+template <int BN, bool PAIR, int LAY, int EPI, typename T, int ACT, bool AUX>
 __global__ void __launch_bounds__(GEMM_THREADS, 1)
 dense_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                      const __grid_constant__ CUtensorMap tmOut, const __grid_constant__ CUtensorMap tmKeep,
                      const __grid_constant__ CUtensorMap tmAux, const DenseParams p) {
-  using S = DenseSmem<BN, PAIR, EPI>;
+  constexpr bool AHEAD = AUX && EPI == DENSE_Y;
+  using S = DenseSmem<BN, PAIR, EPI, AHEAD>;
   using P16 = Pair16<T>;
   constexpr bool A_MN = LAY == DENSE_TN, B_MN = LAY != DENSE_NT, PART = EPI == DENSE_PART, KEEP = EPI == DENSE_Y_KEEP;
   constexpr int TILE_M = PAIR ? 2 * GEMM_BM : GEMM_BM;
+  constexpr bool ANY = ACT == ACT_ANY;
+  const bool has_aux = ANY ? p.aux != nullptr : AUX, direct = ANY && p.direct;
   constexpr int BOX = 8192;                                // an MN-major box: 64 contraction rows of 128 bytes
   const uint32_t pair_rank = PAIR ? cluster_ctarank() : 0u;
   const int unit = PAIR ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
@@ -265,49 +272,67 @@ dense_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
     }
   } else {
     // ------------------------------------------------------------ epilogue warps
-    // Warp e has the 32 rows of its lane quarter and a quarter of the tile's columns, 32 at a time, as matrix
-    // fragments (tmem_ld_16x256_x4): registers -> math -> 32 x 32 staging box (64-byte rows, 64-byte swizzle) -> TMA
-    // store, clipped at the matrix's edge. The residual is loaded into the box before.
+    // Warp e has the 32 rows of its lane quarter and a quarter of the tile's columns, 32 at a time, as matrix fragments
+    // (tmem_ld_16x256_x4): registers -> math -> staging box (swizzled) -> TMA store, clipped at the matrix's edge. The
+    // residual is loaded into the box before; AHEAD, the box has all the warp's columns, and the next tile's residual
+    // comes as soon as this tile's store has been read.
     const int e = warp - 2;
     const int quarter = warp & 3;
     const int cg = e >> 2;
     constexpr int WARP_COLS = BN < 128 ? 32 : BN / 4;
-    constexpr int NSUB = WARP_COLS / 32;
-    [[maybe_unused]] const uint32_t box = smem_base + S::STAGING_OFF + e * S::BOXES * S::BOX_BYTES;
-    [[maybe_unused]] const uint32_t zbox = box + S::BOX_BYTES;      // KEEP
-    const uint32_t in_box = static_cast<uint32_t>(((lane >> 3) & 1) * 8 + (lane & 7)) * 64u;
-    [[maybe_unused]] auto box_addr = [&](uint32_t b, int hf, int q) -> uint32_t {
-      return b + in_box + hf * 1024u +
-             ((static_cast<uint32_t>(2 * q + (lane >> 4)) ^ static_cast<uint32_t>((lane >> 1) & 3)) << 4);
-    };
+    constexpr int BC = S::BOX_COLS;
     const uint32_t acce_remote0 = PAIR ? map_to_cta(acce_bar(0), 0) : 0u;
     const uint32_t acce_remote1 = PAIR ? map_to_cta(acce_bar(1), 0) : 0u;
-    [[maybe_unused]] const bool fetch = p.aux != nullptr && !p.direct;
+    [[maybe_unused]] const uint32_t box = smem_base + S::STAGING_OFF + e * S::BOXES * S::BOX_BYTES;
+    [[maybe_unused]] const uint32_t zbox = box + S::BOX_BYTES;      // KEEP
+    // this lane's row of the 8 x 8 pieces (rows 16 hf + {0, 8}, columns 32 c + 16 q + {0, 8}) of a box
+    [[maybe_unused]] auto box_addr = [&](uint32_t b, int hf, int c, int q) -> uint32_t {
+      const uint32_t r = ((lane >> 3) & 1) * 8 + (lane & 7), piece = 4 * c + 2 * q + (lane >> 4);
+      return b + (16 * hf + r) * (BC * 2u) + ((BC == 64 ? piece ^ (r & 7) : piece ^ ((r >> 1) & 3)) << 4);
+    };
+    const bool fetch = !PART && has_aux && !direct;
     [[maybe_unused]] uint32_t aux_phase = 0;
+    // first row and column of this warp's part of a tile; whether there is anything of it
+    auto part_of = [&](int tile, int& m, int& n) -> bool {
+      int mt, jt;
+      tile_of(tile, mt, jt);
+      m = mt * TILE_M + static_cast<int>(pair_rank) * GEMM_BM + quarter * 32;
+      n = jt * BN + cg * WARP_COLS;
+      return n < p.N && m < p.M && cg * WARP_COLS < BN;     // warp-uniform
+    };
+    [[maybe_unused]] auto fetch_aux = [&](int m, int n) {
+      if (elect_one()) {
+        tma_store_wait_read0();        // the box's last store has been read
+        mbar_expect_tx(aux_bar(e), S::BOX_BYTES);
+        tma_load_2d(box, &tmAux, n, m, aux_bar(e));
+      }
+    };
     int it = 0;
     bool ok = true;
     DenseWalk walk(unit);
     DenseSegment g;
+    if constexpr (AHEAD) {
+      int m, n;
+      if (unit < num_tiles && part_of(unit, m, n)) fetch_aux(m, n);
+    }
     for (; ok && next(walk, g); ++it) {
       const int buf = it & 1;
-      int mt, jt;
-      tile_of(g.tile, mt, jt);
-      const int m_warp = mt * TILE_M + static_cast<int>(pair_rank) * GEMM_BM + quarter * 32;
-      const int n_warp0 = jt * BN + cg * WARP_COLS;
+      int m_warp, n_warp0;
+      const bool live = part_of(g.tile, m_warp, n_warp0);
+      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
+                             static_cast<uint32_t>(buf * BN + cg * WARP_COLS);
+      [[maybe_unused]] float* slab = nullptr;
+      if constexpr (PART) {
+        int mt, jt;
+        tile_of(g.tile, mt, jt);
+        slab = p.part + static_cast<long long>(g.slot) * (TILE_M * BN) +
+               static_cast<long long>(m_warp - mt * TILE_M) * BN + (n_warp0 - jt * BN) + 2 * (lane & 3);
+      }
       bool acc_ready = false;
 #pragma unroll 1
-      for (int c = 0; c < NSUB; ++c) {
-        const int n0 = n_warp0 + c * 32;
-        const bool live = n0 < p.N && m_warp < p.M && cg * WARP_COLS < BN;   // warp-uniform
-        [[maybe_unused]] uint64_t bias[4];
-        if constexpr (!PART) {
-          dense_lane_bias(p, n0, lane, bias);
-          if (fetch && live && elect_one()) {
-            tma_store_wait_read0();        // the box's last store has been read
-            mbar_expect_tx(aux_bar(e), S::BOX_BYTES);
-            tma_load_2d(box, &tmAux, n0, m_warp, aux_bar(e));
-          }
-        }
+      for (int c0 = 0; c0 < WARP_COLS; c0 += BC) {              // a box
+        const bool box_live = live && n_warp0 + c0 < p.N;
+        if (!AHEAD && fetch && box_live) fetch_aux(m_warp, n_warp0 + c0);
         if (!acc_ready) {
           if (!gemm_wait(accf_bar(buf), (it >> 1) & 1u, abort_flag, ST_TIMEOUT_EPILOGUE)) {
             ok = false;
@@ -316,110 +341,115 @@ dense_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
           tc_fence_after();
           acc_ready = true;
         }
-        if constexpr (!PART) {
-          if (fetch && live) {
-            if (!gemm_wait(aux_bar(e), aux_phase, abort_flag, ST_TIMEOUT_EPILOGUE)) {
-              ok = false;
-              break;
-            }
-            aux_phase ^= 1u;
+        if (fetch && box_live) {
+          if (!gemm_wait(aux_bar(e), aux_phase, abort_flag, ST_TIMEOUT_EPILOGUE)) {
+            ok = false;
+            break;
           }
+          aux_phase ^= 1u;
         }
-        uint32_t acc[2][16];
-        if (live) {
-          const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
-                                 static_cast<uint32_t>(buf * BN + cg * WARP_COLS + c * 32);
-          tmem_ld_16x256_x4(taddr, acc[0]);
-          tmem_ld_16x256_x4(taddr + (16u << 16), acc[1]);
-          tmem_ld_wait();
-        }
-        if (c == NSUB - 1) {
-          // the accumulator is in registers (or not needed): hand it back to the MMA warp
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) {
-            if constexpr (PAIR) mbar_arrive_cluster(buf ? acce_remote1 : acce_remote0);
-            else mbar_arrive(acce_bar(buf));
+#pragma unroll 1
+        for (int c = 0; c < BC / 32; ++c) {
+          const int n0 = n_warp0 + c0 + 32 * c;
+          const bool on = live && n0 < p.N;
+          [[maybe_unused]] uint64_t bias[4];
+          if constexpr (!PART) dense_lane_bias(p, n0, lane, bias);
+          uint32_t acc[2][16];
+          if (on) {
+            tmem_ld_16x256_x4(taddr + c0 + 32 * c, acc[0]);
+            tmem_ld_16x256_x4(taddr + c0 + 32 * c + (16u << 16), acc[1]);
+            tmem_ld_wait();
           }
-        }
-        if (!live) continue;
-        // the fragment: pair i of half hf is row 16 hf + 8 (i % 2) + lane / 4, columns 8 (i / 2) + 2 (lane % 4)
-        if constexpr (PART) {
-          float* slab = p.part + static_cast<long long>(g.slot) * (TILE_M * BN) +
-                        static_cast<long long>(m_warp - mt * TILE_M) * BN + (n0 - jt * BN) + 2 * (lane & 3);
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int r = 16 * hf + 8 * (i & 1) + (lane >> 2);
-              if (m_warp + r < p.M)
-                *reinterpret_cast<uint2*>(slab + r * BN + 8 * (i >> 1)) = make_uint2(acc[hf][2 * i], acc[hf][2 * i + 1]);
+          if (c0 + 32 * c + 32 == WARP_COLS) {
+            // the accumulator is in registers (or not needed): hand it back to the MMA warp
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              if constexpr (PAIR) mbar_arrive_cluster(buf ? acce_remote1 : acce_remote0);
+              else mbar_arrive(acce_bar(buf));
             }
-        } else {
+          }
+          if (!on) continue;
+          // the fragment: pair i of half hf is row 16 hf + 8 (i % 2) + lane / 4, columns 8 (i / 2) + 2 (lane % 4)
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf) {
-            uint64_t v[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = fadd2(pack2u(acc[hf][2 * i], acc[hf][2 * i + 1]), bias[i >> 1]);
-            uint32_t aux[8];
-            if (p.aux != nullptr) {
-              if (!p.direct) {
-#pragma unroll
-                for (int q = 0; q < 2; ++q) ldmatrix_x4(box_addr(box, hf, q), &aux[4 * q]);
-              } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                  const int row = m_warp + 16 * hf + 8 * (i & 1) + (lane >> 2), col = n0 + 8 * (i >> 1) + 2 * (lane & 3);
-                  aux[i] = row < p.M && col < p.N
-                               ? dense_load_pair(p.aux, static_cast<long long>(row) * p.ldaux + col, col + 1 < p.N)
-                               : 0u;
-                }
-              }
-            }
-            auto put = [&](uint32_t b, void* base, long long ld, bool wait) {
-              uint32_t w[8];
+            if constexpr (PART) {
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
-                float lo, hi;
-                unpack2(v[i], lo, hi);
-                w[i] = P16::pack(lo, hi);
+                const int r = 16 * hf + 8 * (i & 1) + (lane >> 2);
+                if (m_warp + r < p.M)
+                  *reinterpret_cast<uint2*>(slab + r * BN + c0 + 32 * c + 8 * (i >> 1)) =
+                      make_uint2(acc[hf][2 * i], acc[hf][2 * i + 1]);
               }
-              if (!p.direct) {
-                if (wait) {      // as late as possible: the last sub-chunk's stores drain meanwhile
-                  if (elect_one()) tma_store_wait_read0();
-                  __syncwarp();
-                }
+            } else {
+              uint64_t v[8];
 #pragma unroll
-                for (int q = 0; q < 2; ++q) stmatrix_x4(box_addr(b, hf, q), &w[4 * q]);
-              } else {
+              for (int i = 0; i < 8; ++i) v[i] = fadd2(pack2u(acc[hf][2 * i], acc[hf][2 * i + 1]), bias[i >> 1]);
+              const int row0 = m_warp + 16 * hf + (lane >> 2), col0 = n0 + 2 * (lane & 3);
+              auto put = [&](uint32_t b, void* to, long long ld, bool wait) {
+                uint32_t w[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                  const int row = m_warp + 16 * hf + 8 * (i & 1) + (lane >> 2), col = n0 + 8 * (i >> 1) + 2 * (lane & 3);
-                  if (row < p.M && col < p.N)
-                    dense_store_pair<T>(base, static_cast<long long>(row) * ld + col, w[i], col + 1 < p.N);
+                  float lo, hi;
+                  unpack2(v[i], lo, hi);
+                  w[i] = P16::pack(lo, hi);
+                }
+                if (!direct) {
+                  if (wait) {      // as late as possible: the box's last store drains meanwhile
+                    if (elect_one()) tma_store_wait_read0();
+                    __syncwarp();
+                  }
+#pragma unroll
+                  for (int q = 0; q < 2; ++q) stmatrix_x4(box_addr(b, hf, c, q), &w[4 * q]);
+                } else {
+#pragma unroll
+                  for (int i = 0; i < 8; ++i) {
+                    const int row = row0 + 8 * (i & 1), col = col0 + 8 * (i >> 1);
+                    if (row < p.M && col < p.N)
+                      dense_store_pair<T>(to, static_cast<long long>(row) * ld + col, w[i], col + 1 < p.N);
+                  }
+                }
+              };
+              if constexpr (KEEP) put(zbox, p.keep, p.ldk, c == 0 && hf == 0 && !fetch);
+              if constexpr (LAY == DENSE_NT) {
+                uint32_t aux[8];
+                if (has_aux) {
+                  if (!direct) {
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) ldmatrix_x4(box_addr(box, hf, c, q), &aux[4 * q]);
+                  } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                      const int row = row0 + 8 * (i & 1), col = col0 + 8 * (i >> 1);
+                      aux[i] = row < p.M && col < p.N
+                                   ? dense_load_pair(p.aux, static_cast<long long>(row) * p.ldaux + col, col + 1 < p.N)
+                                   : 0u;
+                    }
+                  }
+                }
+                if constexpr (ANY) dense_act<T>(p.act, v); else dense_act_all<T, ACT>(v);
+                if (has_aux) {
+#pragma unroll
+                  for (int i = 0; i < 8; ++i) v[i] = fadd2(v[i], pack2(P16::lo(aux[i]), P16::hi(aux[i])));
                 }
               }
-            };
-            if constexpr (KEEP) put(zbox, p.keep, p.ldk, hf == 0 && !fetch);
-            if constexpr (LAY == DENSE_NT) {
-              dense_act(p.act, v);
-              if (p.aux != nullptr) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = fadd2(v[i], pack2(P16::lo(aux[i]), P16::hi(aux[i])));
-              }
-            }
-            put(box, p.out, p.ldo, !KEEP && hf == 0 && !fetch);
-          }
-          if (!p.direct) {
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (elect_one()) {
-              if constexpr (KEEP) tma_store_2d(&tmKeep, zbox, n0, m_warp);
-              tma_store_2d(&tmOut, box, n0, m_warp);
-              tma_store_commit();
+              put(box, p.out, p.ldo, !KEEP && c == 0 && hf == 0 && !fetch);
             }
           }
         }
+        if (!PART && !direct && box_live) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (elect_one()) {
+            if constexpr (KEEP) tma_store_2d(&tmKeep, zbox, n_warp0 + c0, m_warp);
+            tma_store_2d(&tmOut, box, n_warp0 + c0, m_warp);
+            tma_store_commit();
+          }
+        }
+      }
+      if constexpr (AHEAD) {
+        int m, n;
+        if (ok && g.tile + n_units < num_tiles && part_of(g.tile + n_units, m, n)) fetch_aux(m, n);
       }
     }
     if (elect_one()) tma_store_wait_all();
@@ -525,7 +555,7 @@ __global__ void __launch_bounds__(FINISH_THREADS) dense_finish_kernel(const Dens
     }
   };
   if (p.keep != nullptr) put(p.keep, p.ldk);
-  dense_act(p.act, v);
+  dense_act<T>(p.act, v);
   if (p.aux != nullptr) {
 #pragma unroll
     for (int k = 0; k < 2; ++k)

@@ -119,10 +119,10 @@ _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 
 
 def _activation(name: str) -> int:
-    try:
-        return ACTIVATIONS[name]
-    except (KeyError, TypeError):
-        raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)}, got {name!r}") from None
+    act = ACTIVATIONS.get(name) if isinstance(name, str) else None
+    if act is None:
+        raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)}, got {name!r}")
+    return act
 
 
 def _require_16bit(t: torch.Tensor, name: str) -> int:
@@ -139,36 +139,40 @@ def _like(t: torch.Tensor, name: str, x: torch.Tensor) -> None:
         raise TypeError(f"{name} must be {x.dtype} on {x.device}, got {t.dtype} on {t.device}")
 
 
-def _f32_like(t, name: str, shape, x: torch.Tensor):
+def _f32_like(t, name: str, size: int, x: torch.Tensor):
+    """An fp32 vector of `size` values on x's device, packed; None stays None."""
     if t is None:
         return None
     if t.dtype != torch.float32 or t.device != x.device:
         raise TypeError(f"{name} must be float32 on {x.device}, got {t.dtype} on {t.device}")
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
+    if t.dim() != 1 or t.shape[0] != size:
+        raise ValueError(f"{name} must have shape ({size},), got {tuple(t.shape)}")
     return t.contiguous()
 
 
 def _packed_rows(t: torch.Tensor, cols: int, name: str):
-    """t [..., cols] as rows (tensor, row stride): unit inner stride and rows that do not overlap, copied where they do."""
-    if t.dim() < 2 or t.shape[-1] != cols:
-        raise ValueError(f"{name} must be [..., {cols}] with at least 2 dims, got {tuple(t.shape)}")
-    t = t.detach() if t.dim() == 2 else t.reshape(-1, cols)
-    if t.shape[0] > 1:
-        if (t.stride(1) != 1 and cols > 1) or t.stride(0) < cols:
-            t = t.contiguous()
-        return t, t.stride(0)
-    return (t if cols == 1 or t.stride(1) == 1 else t.contiguous()), cols
+    """t [..., cols] as rows: (tensor, rows, row stride), of unit inner stride and not overlapping; copied where they are
+    not. (Attribute reads are what such a call costs on the host: the common case comes first.)"""
+    shape = t.shape
+    if len(shape) == 2 and shape[1] == cols and shape[0] > 1:
+        row, inner = t.stride()
+        if inner == 1 and row >= cols:
+            return t, shape[0], row
+    if len(shape) < 2 or shape[-1] != cols:
+        raise ValueError(f"{name} must be [..., {cols}] with at least 2 dims, got {tuple(shape)}")
+    if len(shape) != 2:
+        t = t.reshape(-1, cols)
+    rows = t.shape[0]
+    row, inner = t.stride()
+    if (inner != 1 and cols > 1) or (rows > 1 and row < cols):
+        t, row = t.contiguous(), cols
+    return t, rows, row if rows > 1 else cols
 
 
-def _aligned16(t, ld: int) -> int:
-    return int(t.data_ptr() % 16 == 0 and ld % 8 == 0)
-
-
-def _scratch(need: int, device):
+def _scratch(need: int, x):
     if need < 0:
         _lib.check(need, "workspace size")
-    return torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    return x.new_empty(need, dtype=torch.uint8) if need else None
 
 
 def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, activation: str = "none",
@@ -181,41 +185,43 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     with unit inner stride; it may be the residual, no other operand. The gradients are linear_act_backward's;
     torch.ops.strata_b200.linear_act is the differentiable form."""
     dtype = _require_16bit(x, "x")
-    _like(weight, "weight", x)
     act = _activation(activation)
+    _like(weight, "weight", x)
     if weight.dim() != 2:
         raise ValueError(f"weight must be [N, K], got {tuple(weight.shape)}")
     N, K = weight.shape
-    x2, ldx = _packed_rows(x, K, "x")
-    w2, ldw = _packed_rows(weight, K, "weight")
-    M = x2.shape[0]
-    bias = _f32_like(bias, "bias", (N,), x)
-    shape = (*x.shape[:-1], N)
+    x2, M, ldx = _packed_rows(x, K, "x")
+    w2, _, ldw = _packed_rows(weight, K, "weight")
+    bias = _f32_like(bias, "bias", N, x)
+    shape = x.shape[:-1] + (N,)
     r2, ldr = None, 0
     if residual is not None:
         _like(residual, "residual", x)
-        if tuple(residual.shape) != shape:
-            raise ValueError(f"residual must be {shape}, got {tuple(residual.shape)}")
-        r2, ldr = _packed_rows(residual, N, "residual")
+        if residual.shape != shape:
+            raise ValueError(f"residual must be {tuple(shape)}, got {tuple(residual.shape)}")
+        r2, _, ldr = _packed_rows(residual, N, "residual")
     if out is None:
-        y, ldy = torch.empty(shape, dtype=x.dtype, device=x.device), N
+        y, ldy = x.new_empty(shape), N
     else:
         _like(out, "out", x)
-        if tuple(out.shape) != (M, N) or (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
+        if out.shape != (M, N) or (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
             raise ValueError(f"out must be [{M}, {N}] with unit inner stride")
         y, ldy = out, out.stride(0) if M > 1 else N
-    z = torch.empty(shape, dtype=x.dtype, device=x.device) if save_preact else None
+    z = x.new_empty(shape) if save_preact else None
     if M:
         lib = _lib.load()
         with _lib.on_device(x):
-            ws, need = None, 0
-            if M > 8:
-                need = lib.strata_linear_act_workspace_bytes(M, N, K, _aligned16(x2, ldx), _aligned16(w2, ldw))
-                ws = _scratch(need, x.device)
-            _lib.check(lib.strata_linear_act(
-                x2.data_ptr(), ldx, w2.data_ptr(), ldw, None if bias is None else bias.data_ptr(),
-                None if r2 is None else r2.data_ptr(), ldr, y.data_ptr(), ldy, None if z is None else z.data_ptr(), N,
-                M, N, K, act, dtype, None if ws is None else ws.data_ptr(), need, _stream_ptr(x)), "strata_linear_act")
+            xp, wp = x2.data_ptr(), w2.data_ptr()
+            need, ws = 0, None
+            if M > 8:       # (fewer rows take no workspace)
+                need = lib.strata_linear_act_workspace_bytes(M, N, K, not (xp & 15 or ldx & 7), not (wp & 15 or ldw & 7))
+                ws = _scratch(need, x)
+            code = lib.strata_linear_act(
+                xp, ldx, wp, ldw, None if bias is None else bias.data_ptr(), None if r2 is None else r2.data_ptr(), ldr,
+                y.data_ptr(), ldy, None if z is None else z.data_ptr(), N, M, N, K, act, dtype,
+                None if ws is None else ws.data_ptr(), need, _stream_ptr(x))
+            if code:
+                _lib.check(code, "strata_linear_act")
     if out is not None and x.dim() != 2:
         y = out.view(shape)
     return (y, z) if save_preact else y
@@ -228,44 +234,44 @@ def linear_act_backward(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tenso
     needed; the residual's is grad itself. preact: the z that linear_act saved (any activation but "none"). No atomics:
     the same call gives the same bits."""
     dtype = _require_16bit(grad, "grad")
+    act = _activation(activation)
     _like(x, "x", grad)
     _like(weight, "weight", grad)
-    act = _activation(activation)
     if weight.dim() != 2:
         raise ValueError(f"weight must be [N, K], got {tuple(weight.shape)}")
     N, K = weight.shape
-    if x.dim() < 2 or x.shape[-1] != K:
-        raise ValueError(f"x must be [..., {K}] with at least 2 dims, got {tuple(x.shape)}")
-    shape = (*x.shape[:-1], N)
-    if tuple(grad.shape) != shape:
-        raise ValueError(f"grad must be {shape}, got {tuple(grad.shape)}")
-    g2, ldg = _packed_rows(grad, N, "grad")
-    x2, ldx = _packed_rows(x, K, "x")
-    w2, ldw = _packed_rows(weight, K, "weight")
-    z2, ldz = None, 0
+    x2, M, ldx = _packed_rows(x, K, "x")
+    w2, _, ldw = _packed_rows(weight, K, "weight")
+    shape = x.shape[:-1] + (N,)
+    if grad.shape != shape:
+        raise ValueError(f"grad must be {tuple(shape)}, got {tuple(grad.shape)}")
+    g2, _, ldg = _packed_rows(grad, N, "grad")
+    zp, ldz = None, 0
     if act:
         if preact is None:
             raise ValueError(f'the gradient through "{activation}" needs preact, the z that linear_act saves')
         _like(preact, "preact", grad)
-        if tuple(preact.shape) != shape:
-            raise ValueError(f"preact must be {shape}, got {tuple(preact.shape)}")
-        z2, ldz = _packed_rows(preact, N, "preact")
-    M, dev = x2.shape[0], x.device
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
-    dw = torch.empty((N, K), dtype=x.dtype, device=dev) if need_weight else None
-    db = torch.empty(N, dtype=torch.float32, device=dev) if need_bias else None
+        if preact.shape != shape:
+            raise ValueError(f"preact must be {tuple(shape)}, got {tuple(preact.shape)}")
+        z2, _, ldz = _packed_rows(preact, N, "preact")
+        zp = z2.data_ptr()
+    dx = x.new_empty(x.shape) if need_x else None
+    dw = x.new_empty((N, K)) if need_weight else None
+    db = x.new_empty(N, dtype=torch.float32) if need_bias else None
     if need_x or need_weight or need_bias:
         lib = _lib.load()
         with _lib.on_device(x):
+            gp, xp, wp = g2.data_ptr(), x2.data_ptr(), w2.data_ptr()
             need = lib.strata_linear_act_backward_workspace_bytes(
-                M, N, K, act, _aligned16(g2, ldg), 0 if z2 is None else _aligned16(z2, ldz), _aligned16(x2, ldx),
-                _aligned16(w2, ldw), int(need_x), int(need_weight), int(need_bias))
-            ws = _scratch(need, dev)
-            _lib.check(lib.strata_linear_act_backward(
-                g2.data_ptr(), ldg, x2.data_ptr(), ldx, w2.data_ptr(), ldw, None if z2 is None else z2.data_ptr(), ldz,
-                None if dx is None else dx.data_ptr(), K, None if dw is None else dw.data_ptr(), K,
-                None if db is None else db.data_ptr(), M, N, K, act, dtype, None if ws is None else ws.data_ptr(), need,
-                _stream_ptr(x)), "strata_linear_act_backward")
+                M, N, K, act, not (gp & 15 or ldg & 7), not (zp is None or zp & 15 or ldz & 7),
+                not (xp & 15 or ldx & 7), not (wp & 15 or ldw & 7), need_x, need_weight, need_bias)
+            ws = _scratch(need, x)
+            code = lib.strata_linear_act_backward(
+                gp, ldg, xp, ldx, wp, ldw, zp, ldz, None if dx is None else dx.data_ptr(), K,
+                None if dw is None else dw.data_ptr(), K, None if db is None else db.data_ptr(), M, N, K, act, dtype,
+                None if ws is None else ws.data_ptr(), need, _stream_ptr(x))
+            if code:
+                _lib.check(code, "strata_linear_act_backward")
     return dx, dw, db
 
 
@@ -665,65 +671,66 @@ def qk_norm_rows_(qkv: torch.Tensor, C: int, eps: float = 1e-6) -> torch.Tensor:
     return qkv
 
 
-def _heads(t: torch.Tensor, name: str, shape, like: torch.Tensor):
-    """t [..., heads, head_dim] as [tokens, heads, head_dim] for the kernels: a view where the token stride is one and
-    everything is in 16-byte pieces, else a copy."""
-    if t.dtype != like.dtype or t.device != like.device:
-        raise TypeError(f"{name} must be {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
-    t = t.detach() if t.dim() == 3 else t.detach().reshape(-1, *shape[-2:])
-    M, heads, hd = t.shape
-    # (a dimension of one has whatever stride)
-    token, head = t.stride(0) if M > 1 else heads * hd, t.stride(1) if heads > 1 else hd
-    if t.stride(2) != 1 or token % 8 or head % 8 or t.data_ptr() % 16:
+def _heads(t: torch.Tensor, name: str, like: torch.Tensor):
+    """t [..., heads, head_dim] of like's shape for the kernels: (tensor, token stride, head stride) of a view as [tokens,
+    heads, head_dim] where there is one in 16-byte pieces, else of a copy."""
+    if t is not like:
+        _like(t, name, like)
+        if t.shape != like.shape:
+            raise ValueError(f"{name} must be {tuple(like.shape)}, got {tuple(t.shape)}")
+    if t.dim() != 3:
+        t = t.reshape(-1, *t.shape[-2:])
+    tokens, heads, hd = t.shape
+    token, head, inner = t.stride()
+    if tokens == 1 or heads == 1:      # (a dimension of one has whatever stride)
+        token, head = token if tokens > 1 else heads * hd, head if heads > 1 else hd
+    if inner != 1 or (token | head) & 7 or t.data_ptr() & 15:
         t = t.clone(memory_format=torch.contiguous_format)
         token, head = heads * hd, hd
-    return t, _lib.Heads(t.data_ptr(), token, head)
+    return t, token, head
 
 
-def _heads_out(t: torch.Tensor, name: str, shape, like: torch.Tensor):
-    t3, desc = _heads(t, name, shape, like)
-    (M, heads, hd), inner, outer = t3.shape, desc.stride_head, desc.stride_token
-    sizes = (heads, M)
-    if inner > outer:
-        inner, outer, sizes = outer, inner, (M, heads)
-    if t3.data_ptr() != t.data_ptr() or (sizes[0] > 1 and inner < hd) or (
-            sizes[1] > 1 and outer < max(inner * (sizes[0] - 1), 0) + hd):
+def _heads_out(t: torch.Tensor, name: str, like: torch.Tensor):
+    t3, token, head = _heads(t, name, like)
+    (tokens, heads, hd), ok = t3.shape, t3.data_ptr() == t.data_ptr()
+    for (inner, n), (outer, m) in (((head, heads), (token, tokens)), ((token, tokens), (head, heads))):
+        if inner <= outer or m == 1:
+            ok = ok and (n == 1 or inner >= hd) and (m == 1 or outer >= inner * (n - 1) + hd)
+            break
+    if not ok:
         raise ValueError(f"{name} must be viewable as [tokens, heads, head_dim] in 16-byte pieces that do not overlap")
-    return desc
+    return t3, token, head
 
 
 def _qk_arguments(q, k, q_weight, k_weight, rope_cs, positions, tokens_per_tile, hw, interleaved):
-    """What both directions check: (heads_q, heads_k, head_dim, kept tensors, the C arguments from rot to hw)."""
+    """What both directions check: (heads_q, heads_k, head_dim, tokens, tensors, the C arguments from rot to hw)."""
     _like(k, "k", q)
-    if q.dim() < 3 or k.dim() != q.dim():
+    qs, ks = q.shape, k.shape
+    if len(qs) < 3 or len(ks) != len(qs):
         raise ValueError("q and k must be [..., heads, head_dim]")
-    hq, hd = q.shape[-2:]
-    hk = k.shape[-2]
-    if k.shape[:-2] != q.shape[:-2] or k.shape[-1] != hd:
-        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} must have the same tokens and head_dim")
+    hq, hd = qs[-2:]
+    hk = ks[-2]
+    if ks[:-2] != qs[:-2] or ks[-1] != hd:
+        raise ValueError(f"q {tuple(qs)} and k {tuple(ks)} must have the same tokens and head_dim")
     if hd % 8 or not 8 <= hd <= 256 or not hq or not hk:
         raise ValueError(f"head_dim must be a multiple of 8 up to 256 and both have heads, got {hq} + {hk} heads of {hd}")
-    M = 1
-    for n in q.shape[:-2]:
-        M *= n
-    q_weight = _f32_like(q_weight, "q_weight", (hd,), q)
-    k_weight = _f32_like(k_weight, "k_weight", (hd,), q)
+    M = qs[0] if len(qs) == 3 else qs[:-2].numel()
+    wq, wk = _f32_like(q_weight, "q_weight", hd, q), _f32_like(k_weight, "k_weight", hd, q)
     if rope_cs is None:
         if positions is not None:
             raise ValueError("positions are rows of rope_cs: give both or neither")
-        return hq, hk, hd, M, (q_weight, k_weight), (0, int(interleaved), None, 0, 0, None, 0, 0, 0)
+        return hq, hk, hd, M, (wq, wk), (0, interleaved, None, 0, 0, None, 0, 0, 0)
     if rope_cs.dtype not in (torch.float16, torch.float32) or rope_cs.device != q.device:
         raise TypeError(f"rope_cs must be float16 or float32 on {q.device}, got {rope_cs.dtype} on {rope_cs.device}")
-    if rope_cs.dim() < 3 or rope_cs.shape[-1] != 2:
-        raise ValueError(f"rope_cs must be [..., rot / 2, 2], got {tuple(rope_cs.shape)}")
-    rot = 2 * rope_cs.shape[-2]
+    cshape = rope_cs.shape
+    if len(cshape) < 3 or cshape[-1] != 2:
+        raise ValueError(f"rope_cs must be [..., rot / 2, 2], got {tuple(cshape)}")
+    rot = 2 * cshape[-2]
     unit = 8 if interleaved else 16
     if rot % unit or not 0 < rot <= hd:
         raise ValueError(f"rope_cs turns {rot} channels: a multiple of {unit} up to head_dim {hd} is needed")
     cs = rope_cs.contiguous()
-    if cs.data_ptr() % 16:
+    if cs.data_ptr() & 15:
         cs = cs.clone()
     rows = cs.numel() // rot
     if not rows:
@@ -736,8 +743,8 @@ def _qk_arguments(q, k, q_weight, k_weight, rope_cs, positions, tokens_per_tile,
             raise ValueError(f"positions must name a row for each of the {M} tokens, got {positions.numel()}")
         if tokens_per_tile is not None or hw is not None:
             raise ValueError("a token's row is given by positions or by tokens_per_tile and hw, not by both")
-        pos, wide = positions.contiguous(), int(positions.dtype == torch.int64)
-        per, hw = 0, 0
+        pos, wide = positions.contiguous(), positions.dtype == torch.int64
+        per = hw = 0
     else:
         per = rows if tokens_per_tile is None else int(tokens_per_tile)
         hw = per if hw is None else int(hw)
@@ -745,9 +752,9 @@ def _qk_arguments(q, k, q_weight, k_weight, rope_cs, positions, tokens_per_tile,
             raise ValueError("tokens_per_tile and hw must be positive")
         if M and (M - 1) // per * hw + min(M, hw) > rows:
             raise ValueError(f"{M} tokens, {per} a tile with {hw} rows each, need more than the {rows} rows of rope_cs")
-    return hq, hk, hd, M, (q_weight, k_weight, cs, pos), (
-        rot, int(interleaved), cs.data_ptr(), int(cs.dtype == torch.float32), rows,
-        None if pos is None else pos.data_ptr(), wide, per, hw)
+    return hq, hk, hd, M, (wq, wk, cs, pos), (
+        rot, interleaved, cs.data_ptr(), cs.dtype == torch.float32, rows, None if pos is None else pos.data_ptr(), wide,
+        per, hw)
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None = None,
@@ -768,20 +775,23 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
     dtype = _require_16bit(q, "q")
     hq, hk, hd, M, keep, args = _qk_arguments(q, k, q_weight, k_weight, rope_cs, positions, tokens_per_tile, hw,
                                               interleaved)
-    if out is None:
-        yq, yk = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=q.dtype, device=q.device)
-    else:
-        yq, yk = out
+    yq, yk = (q.new_empty(q.shape), k.new_empty(k.shape)) if out is None else out
     if not M:
         return yq, yk
-    q3, q_desc = _heads(q, "q", tuple(q.shape), q)
-    k3, k_desc = _heads(k, "k", tuple(k.shape), q)
-    yq_desc, yk_desc = _heads_out(yq, "out[0]", tuple(q.shape), q), _heads_out(yk, "out[1]", tuple(k.shape), q)
+    q3, q_token, q_head = _heads(q, "q", q)
+    k3, k_token, k_head = _heads(k, "k", k)
+    if out is None:
+        yq_token, yq_head, yk_token, yk_head = hq * hd, hd, hk * hd, hd
+    else:
+        (_, yq_token, yq_head), (_, yk_token, yk_head) = _heads_out(yq, "out[0]", q), _heads_out(yk, "out[1]", k)
+    wq, wk = keep[:2]
     with _lib.on_device(q):
-        _lib.check(_lib.load().strata_qk_norm_rope(
-            q_desc, k_desc, yq_desc, yk_desc, None if keep[0] is None else keep[0].data_ptr(),
-            None if keep[1] is None else keep[1].data_ptr(), hq, hk, hd, *args, M, float(eps), dtype, _stream_ptr(q)),
-            "strata_qk_norm_rope")
+        code = _lib.load().strata_qk_norm_rope(
+            q3.data_ptr(), q_token, q_head, k3.data_ptr(), k_token, k_head, yq.data_ptr(), yq_token, yq_head,
+            yk.data_ptr(), yk_token, yk_head, None if wq is None else wq.data_ptr(),
+            None if wk is None else wk.data_ptr(), hq, hk, hd, *args, M, eps, dtype, _stream_ptr(q))
+        if code:
+            _lib.check(code, "strata_qk_norm_rope")
     return yq, yk
 
 
@@ -796,27 +806,29 @@ def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k
     dtype = _require_16bit(q, "q")
     hq, hk, hd, M, keep, args = _qk_arguments(q, k, q_weight, k_weight, rope_cs, positions, tokens_per_tile, hw,
                                               interleaved)
-    new = lambda t: torch.empty(t.shape, dtype=q.dtype, device=q.device)
-    xq, xk = new(q), new(k)
-    f32 = dict(dtype=torch.float32, device=q.device)
-    wq = None if q_weight is None else torch.empty(hd, **f32)
-    wk = None if k_weight is None else torch.empty(hd, **f32)
+    xq, xk = q.new_empty(q.shape), k.new_empty(k.shape)
+    wq, wk = keep[:2]
+    dwq = None if wq is None else wq.new_empty(hd)
+    dwk = None if wk is None else wk.new_empty(hd)
+    q3, q_token, q_head = _heads(q, "q", q)
+    k3, k_token, k_head = _heads(k, "k", k)
+    dq3, dq_token, dq_head = _heads(dq, "dq", q)
+    dk3, dk_token, dk_head = _heads(dk, "dk", k)
     lib = _lib.load()
-    q3, q_desc = _heads(q, "q", tuple(q.shape), q)
-    k3, k_desc = _heads(k, "k", tuple(k.shape), q)
-    dq3, dq_desc = _heads(dq, "dq", tuple(q.shape), q)
-    dk3, dk_desc = _heads(dk, "dk", tuple(k.shape), q)
-    xq_desc, xk_desc = _heads(xq, "dq_in", tuple(q.shape), q)[1], _heads(xk, "dk_in", tuple(k.shape), q)[1]
-    p = lambda t: None if t is None else t.data_ptr()
     with _lib.on_device(q):
         need, ws = 0, None
         if M and (wq is not None or wk is not None):
             need = lib.strata_qk_norm_rope_backward_workspace_bytes(M, hq + hk, hd)
-            ws = _scratch(need, q.device)
-        _lib.check(lib.strata_qk_norm_rope_backward(
-            dq_desc, dk_desc, q_desc, k_desc, xq_desc, xk_desc, p(keep[0]), p(keep[1]), p(wq), p(wk), hq, hk, hd, *args,
-            M, float(eps), dtype, p(ws), need, _stream_ptr(q)), "strata_qk_norm_rope_backward")
-    return xq, xk, wq, wk
+            ws = _scratch(need, q)
+        code = lib.strata_qk_norm_rope_backward(
+            dq3.data_ptr(), dq_token, dq_head, dk3.data_ptr(), dk_token, dk_head, q3.data_ptr(), q_token, q_head,
+            k3.data_ptr(), k_token, k_head, xq.data_ptr(), hq * hd, hd, xk.data_ptr(), hk * hd, hd,
+            None if wq is None else wq.data_ptr(), None if wk is None else wk.data_ptr(),
+            None if dwq is None else dwq.data_ptr(), None if dwk is None else dwk.data_ptr(), hq, hk, hd, *args, M, eps,
+            dtype, None if ws is None else ws.data_ptr(), need, _stream_ptr(q))
+        if code:
+            _lib.check(code, "strata_qk_norm_rope_backward")
+    return xq, xk, dwq, dwk
 
 
 def adaln_cond(tokens: torch.Tensor, w_dw: torch.Tensor, b_dw: torch.Tensor | None, factor: int,

@@ -303,7 +303,7 @@ int strata_qk_norm_rows_bf16(void* qkv, int64_t ld, int64_t M, int C, float eps,
 /* Per-head RMS norm and rotation of q and k in one pass: y = R (x (mean x^2 + eps)^-1/2 w), for M tokens of heads_q and
  * heads_k heads of head_dim channels (a multiple of 8, at most 256) in one 16-bit type. Element (m, head, c) of an
  * operand lies at base + m*st + head*sh + c; strides in elements, multiples of 8, bases 16-byte aligned. w_q, w_k:
- * [head_dim] fp32 or NULL. R turns the first `rot` channels of a head by the (cos, sin) pairs of the token's row of
+ * [head_dim] fp32, 16-byte aligned, or NULL. R turns the first `rot` channels of a head by the (cos, sin) pairs of the token's row of
  * table [table_rows, rot/2] (IEEE half, or float with table_f32; 16-byte aligned; NULL: no rotation): pairs (2i, 2i+1)
  * with `adjacent`, rot a multiple of 8, else (i, i + rot/2), rot a multiple of 16. The row is positions[m] (int32, or
  * int64 with positions_64); without positions m / tokens_per_tile * hw + m % hw, which has to stay below table_rows. A
@@ -318,7 +318,7 @@ int strata_qk_norm_rope(const void* q, int64_t q_st, int64_t q_sh, const void* k
 /* Its gradients from those of its outputs (dyq, dyk): dxq, dxk of q and k, and dw_q, dw_k [head_dim] fp32 (NULL where
  * there are no weights), summed without atomics: the same bits every time. workspace:
  * strata_qk_norm_rope_backward_workspace_bytes bytes, 16-byte aligned (NULL without dw). */
-int64_t strata_qk_norm_rope_backward_workspace_bytes(int64_t M, int heads, int head_dim);
+int64_t strata_qk_norm_rope_backward_workspace_bytes(int64_t M, int head_dim);
 int strata_qk_norm_rope_backward(const void* dyq, int64_t dyq_st, int64_t dyq_sh, const void* dyk, int64_t dyk_st,
                                  int64_t dyk_sh, const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st,
                                  int64_t k_sh, void* dxq, int64_t dxq_st, int64_t dxq_sh, void* dxk, int64_t dxk_st,

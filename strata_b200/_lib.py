@@ -115,7 +115,7 @@ _SIGNATURES = {
     "strata_qk_norm_rope": (c_int, [c_void_p, c_int64, c_int64] * 4 + [c_void_p] * 2 + [c_int] * 5
                             + [c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_int, c_int64, c_float, c_int,
                                c_void_p]),
-    "strata_qk_norm_rope_backward_workspace_bytes": (c_int64, [c_int64, c_int, c_int]),
+    "strata_qk_norm_rope_backward_workspace_bytes": (c_int64, [c_int64, c_int]),
     "strata_qk_norm_rope_backward": (c_int, [c_void_p, c_int64, c_int64] * 6 + [c_void_p] * 4 + [c_int] * 5
                                      + [c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_int, c_int64, c_float, c_int,
                                         c_void_p, c_int64, c_void_p]),

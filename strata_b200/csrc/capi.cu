@@ -1009,13 +1009,13 @@ static int qk_params(QkParams& p, int heads_q, int heads_k, int head_dim, int ro
     if (positions && (reinterpret_cast<uintptr_t>(positions) & (positions_64 ? 7u : 3u)) != 0) return STRATA_ERR_ARG;
   }
   for (int i = 0; i < 2; ++i)
-    if (!qk_heads_ok(p.x[i]) || !qk_heads_ok(p.y[i]) || (reinterpret_cast<uintptr_t>(p.w[i]) & 3u) != 0)
+    if (!qk_heads_ok(p.x[i]) || !qk_heads_ok(p.y[i]) || (p.w[i] && !aligned16(p.w[i])))
       return STRATA_ERR_ARG;
   p.heads[0] = heads_q; p.heads[1] = heads_k;
   p.head_dim = head_dim; p.rot = table ? rot : 0;
   p.table = table; p.table_f32 = table_f32; p.table_rows = table_rows;
   p.positions = positions; p.positions_64 = positions_64;
-  p.tokens_per_tile = tokens_per_tile; p.hw = hw;
+  p.tokens_per_tile = qk_div(tokens_per_tile); p.hw = qk_div(hw);
   p.M = M; p.eps = eps;
   return STRATA_OK;
 }
@@ -1035,15 +1035,15 @@ int strata_qk_norm_rope(const void* q, int64_t q_st, int64_t q_sh, const void* k
   const int r = qk_params(p, heads_q, heads_k, head_dim, rot, adjacent, table, table_f32, table_rows, positions,
                           positions_64, tokens_per_tile, hw, M, eps, dtype);
   if (r != STRATA_OK) return r;
-  return launch_qk<false>(p, adjacent != 0, dtype == STRATA_F16, qk_blocks(M, heads_q + heads_k, head_dim, false, sms),
+  return launch_qk<false>(p, adjacent != 0, dtype == STRATA_F16, qk_blocks(M, false, sms),
                           as_stream(stream));
 }
 
-int64_t strata_qk_norm_rope_backward_workspace_bytes(int64_t M, int heads, int head_dim) {
+int64_t strata_qk_norm_rope_backward_workspace_bytes(int64_t M, int head_dim) {
   const int sms = current_sm_count();
   if (sms <= 0) return STRATA_ERR_NO_DEVICE;
-  if (M < 0 || M > 0x7FFF0000 || heads <= 0 || head_dim <= 0 || head_dim > 256) return STRATA_ERR_ARG;
-  return qk_blocks(M, heads, head_dim, true, sms) * 2 * head_dim * 4;
+  if (M < 0 || M > 0x7FFF0000 || head_dim <= 0 || head_dim > 256) return STRATA_ERR_ARG;
+  return static_cast<int64_t>(qk_blocks(M, true, sms)) * 2 * head_dim * 4;
 }
 
 int strata_qk_norm_rope_backward(const void* dyq, int64_t dyq_st, int64_t dyq_sh, const void* dyk, int64_t dyk_st,
@@ -1073,15 +1073,16 @@ int strata_qk_norm_rope_backward(const void* dyq, int64_t dyq_st, int64_t dyq_sh
                     tokens_per_tile, hw, M, eps, dtype);
   if (r != STRATA_OK) return r;
   if (!qk_heads_ok(p.dy[0]) || !qk_heads_ok(p.dy[1])) return STRATA_ERR_ARG;
-  const long long blocks = qk_blocks(M, heads_q + heads_k, head_dim, true, sms);
+  const int blocks = qk_blocks(M, true, sms);
   if (dw_q || dw_k) {
-    if (!workspace || !aligned16(workspace) || workspace_bytes < blocks * 2 * head_dim * 4) return STRATA_ERR_ARG;
+    if (!workspace || !aligned16(workspace) || workspace_bytes < static_cast<int64_t>(blocks) * 2 * head_dim * 4)
+       return STRATA_ERR_ARG;
     p.partial = static_cast<float*>(workspace);
   }
   r = launch_qk<true>(p, adjacent != 0, dtype == STRATA_F16, blocks, st);
   if (r != 0 || !p.partial) return r;
-  return launch_chained(qk_weight_grad_kernel, dim3((2 * head_dim + 31) / 32), 256, 0, st, 1,
-                        static_cast<const float*>(p.partial), static_cast<int>(blocks), head_dim, dw_q, dw_k);
+  return launch_chained(qk_weight_grad_kernel, dim3(2 * head_dim / 8), 256, 0, st, 1,
+                        static_cast<const float*>(p.partial), blocks, head_dim, dw_q, dw_k);
 }
 
 int strata_adaln_cond_bf16(const void* tokens, int B, int D, int h, int w, int Cb, int factor,

@@ -148,7 +148,7 @@ inline int launch_dense_bn(int bn, const DenseOperand& A, const DenseOperand& B,
 
 inline int launch_dense_finish(const DenseFinish& f, cudaStream_t st) {
   const DensePlan& s = f.p.plan;
-  const int blocks = (f.p.part ? s.tiles * f.blocks_per_tile : 0) + (f.db ? (f.sum_cols + 31) / 32 : 0);
+  const int blocks = (f.p.part ? s.tiles * f.blocks_per_tile : 0) + (f.db ? (f.sum_cols + 7) / 8 : 0);
   if (blocks == 0) return 0;
   if (f.p.fp16)
     return launch_chained(dense_finish_kernel<__half>, dim3(blocks), FINISH_THREADS, 0, st, 1, f);

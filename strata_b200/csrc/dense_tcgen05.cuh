@@ -486,19 +486,19 @@ __global__ void __launch_bounds__(FINISH_THREADS) dense_finish_kernel(const Dens
   const DensePlan& s = p.plan;
   const int tile_blocks = p.part != nullptr ? s.tiles * f.blocks_per_tile : 0;
   if (static_cast<int>(blockIdx.x) >= tile_blocks) {
-    // 32 columns a block, eight rows of sums side by side
-    __shared__ float red[8][33];
-    const int col = (blockIdx.x - tile_blocks) * 32 + (threadIdx.x & 31), r0 = threadIdx.x >> 5;
+    // eight columns a block, 32 rows of sums side by side
+    __shared__ float red[32][9];
+    const int col = (blockIdx.x - tile_blocks) * 8 + (threadIdx.x & 7), r0 = threadIdx.x >> 3;
     float a = 0.f;
     if (col < f.sum_cols) {
 #pragma unroll 8
-      for (int r = r0; r < f.sum_rows; r += 8) a += f.sums[static_cast<long long>(r) * f.sum_cols + col];
+      for (int r = r0; r < f.sum_rows; r += 32) a += f.sums[static_cast<long long>(r) * f.sum_cols + col];
     }
-    red[r0][threadIdx.x & 31] = a;
+    red[r0][threadIdx.x & 7] = a;
     __syncthreads();
     if (r0 == 0 && col < f.sum_cols) {
 #pragma unroll
-      for (int i = 1; i < 8; ++i) a += red[i][threadIdx.x & 31];
+      for (int i = 1; i < 32; ++i) a += red[i][threadIdx.x & 7];
       f.db[col] = a;
     }
     return;

@@ -7,21 +7,40 @@
 // (cos, sin) pairs of the token's table row. Both directions are bound by HBM: a head is read once (twice backward: x
 // and dy) and written once, in 16 bits; all arithmetic is fp32.
 //
-// A group of G lanes (a power of two, 8 channels each) has a head, a warp 32 / G heads at a time; an item of work is
-// one token's next U rounds of heads, whose loads are all in flight together. The table row is read once per item
-// and not per head: the lanes of a group need the same channels of every head. A head whose width is no power of two
-// leaves the group's last lanes idle. Pairs of the two halves meet through a shuffle within the group.
+// A group of G lanes (a power of two, 8 channels each) has a head; a warp has a token, S = 32 / G heads of it at a time
+// (several tokens where both q and k have fewer heads than that), in steps of two rounds of q heads or of k heads. So the
+// token's table row is read and unpacked once for all its heads. A head whose width is no power of two leaves the group's
+// last lanes idle. What a step reads is asked for two steps ahead with cp.async into slots of shared memory that only the
+// asking lane reads: bytes in flight that cost no registers, and no barrier. Divisions by launch constants are
+// multiplications; arithmetic runs on fp32 pairs.
+// Measured (8 + 8 heads of 64, 262144 tokens, bf16, half table; the bytes alone take 166 us forward, 250 backward):
+// forward 198 us, backward 292 (178 and 263 without rotation). With the loads straight into registers, two rounds of q
+// and two of k at a time: 190 and 355 (16 + 4 heads of 128: 303 against 248, 370 against 323); more blocks per SM at
+// fewer registers spill (backward, three blocks: 353).
 #pragma once
 #include "dense_common.cuh"
 
 namespace strata {
 
-constexpr int QK_ROUNDS = 4;          // U
+constexpr int QK_ROUNDS = 2;          // rounds of q heads, and of k heads, in flight
 
 struct QkTensor {                     // [tokens, heads, head_dim], unit channel stride, 16-byte pieces
   const void* p;
   long long token, head;              // strides in elements
 };
+// Division by a number that the host knows: n / d = (n mul) >> 32 >> shift for n < 2^31 (Granlund and Montgomery 1994).
+struct QkDiv {
+  uint32_t d, mul, shift;
+  __device__ __forceinline__ uint32_t div(uint32_t n) const { return d == 1 ? n : __umulhi(n, mul) >> shift; }
+};
+inline QkDiv qk_div(uint32_t d) {      // 2^31 > d >= 1
+  QkDiv q{d, 0, 0};
+  if (d <= 1) return q;
+  while ((1ull << (q.shift + 1)) < d) ++q.shift;            // 2^shift < d <= 2^(shift + 1)
+  q.mul = static_cast<uint32_t>(((1ull << (32 + q.shift)) + d - 1) / d);
+  return q;
+}
+
 struct QkParams {
   QkTensor x[2];                      // q, k
   QkTensor y[2];                      // outputs (of the backward pass: dx)
@@ -33,99 +52,119 @@ struct QkParams {
   int table_f32, table_rows;
   const void* positions;              // [M] int32 or int64, or nullptr: row m / tokens_per_tile * hw + m % hw
   int positions_64;
-  int tokens_per_tile, hw;
+  QkDiv tokens_per_tile, hw;
   long long M;
   float eps;
   float* partial;                     // backward: [grid, 2, head_dim] sums of dw, or nullptr
 };
 
+enum QkTable : int { QK_NO_TABLE = 0, QK_HALF_TABLE = 1, QK_F32_TABLE = 2 };
+
 // Table row of token m; -1: a padding token, -2: no such row.
 __device__ __forceinline__ int qk_row(const QkParams& p, long long m) {
-  if (p.table == nullptr) return 0;
-  if (p.positions == nullptr) return static_cast<int>(m / p.tokens_per_tile * p.hw + m % p.hw);
+  if (p.positions == nullptr) {
+    const unsigned t = static_cast<unsigned>(m);
+    return static_cast<int>(p.tokens_per_tile.div(t) * p.hw.d + t - p.hw.div(t) * p.hw.d);
+  }
   const long long r = p.positions_64 ? __ldg(static_cast<const long long*>(p.positions) + m)
                                      : __ldg(static_cast<const int*>(p.positions) + m);
   if (r >= p.table_rows) return -2;
   return r < 0 ? -1 : static_cast<int>(r);
 }
 
-// The (cos, sin) of this lane's channels 8 v .. 8 v + 7: of four neighbour pairs, or of eight pairs of the two halves
-// (the same ones for both partners). One of c, s for each channel; c = 1, s = 0 where nothing turns. Neighbours: s has
-// the sign with which the partner enters (-sin for the even channel), so that y_i = x_i c_i + x_partner s_i.
+// (cos, sin) for this lane's channels 8 v .. 8 v + 7: four pairs where neighbours turn, else one for each channel; (1, 0)
+// where nothing turns. sin has the sign with which a pair's second channel enters its first: -1 forward, +1 for the
+// inverse turn; for channels of the second half the other sign.
+// raw: the lane's part of the table row, TV 16-byte vectors.
+template <int TAB, bool ADJ>
+struct QkTab {
+  static constexpr int N = ADJ ? 4 : 8;
+  static constexpr int TV = TAB == QK_NO_TABLE ? 0 : (TAB == QK_F32_TABLE ? 2 : 1) * (ADJ ? 1 : 2);
+};
+// First table entry of this lane in a row of rot / 2.
 template <bool ADJ>
-__device__ __forceinline__ void qk_table(const QkParams& p, int row, int v, float (&c)[8], float (&s)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) { c[i] = 1.f; s[i] = 0.f; }
-  if (p.table == nullptr || row < 0 || 8 * v >= p.rot) return;
+__device__ __forceinline__ int qk_entry(const QkParams& p, int v) {
   const int half = p.rot >> 1;
-  const int pair0 = ADJ ? 4 * v : (8 * v < half ? 8 * v : 8 * v - half);
-  constexpr int N = ADJ ? 4 : 8;
-  float cc[N], ss[N];
-  const long long at = static_cast<long long>(row) * half + pair0;
-  if (p.table_f32) {
-    const float4* t = reinterpret_cast<const float4*>(static_cast<const float2*>(p.table) + at);
+  return ADJ ? 4 * v : 8 * v >= half ? 8 * v - half : 8 * v;
+}
+template <int TAB, bool ADJ, int N, int TV>
+__device__ __forceinline__ void qk_table(const QkParams& p, const uint4 (&raw)[TV], bool turns, int v, float sign,
+                                         float (&c)[N], float (&s)[N]) {
 #pragma unroll
-    for (int i = 0; i < N / 2; ++i) {
-      const float4 f = __ldg(t + i);
-      cc[2 * i] = f.x; ss[2 * i] = f.y; cc[2 * i + 1] = f.z; ss[2 * i + 1] = f.w;
-    }
-  } else {
-    const uint4* t = reinterpret_cast<const uint4*>(static_cast<const uint32_t*>(p.table) + at);
+  for (int i = 0; i < TV; ++i) {
+    const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
-    for (int i = 0; i < N / 4; ++i) {
-      const uint4 u = __ldg(t + i);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (TAB == QK_F32_TABLE) {
+        if (k & 1) s[2 * i + k / 2] = __uint_as_float(w[k]); else c[2 * i + k / 2] = __uint_as_float(w[k]);
+      } else {
         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
-        cc[4 * i + k] = f.x; ss[4 * i + k] = f.y;
+        c[4 * i + k] = f.x; s[4 * i + k] = f.y;
       }
     }
   }
+  if (!ADJ && 8 * v >= p.rot >> 1) sign = -sign;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if constexpr (ADJ) {
-      c[i] = cc[i >> 1];
-      s[i] = i & 1 ? ss[i >> 1] : -ss[i >> 1];
-    } else {
-      c[i] = cc[i];
-      s[i] = 8 * v < half ? -ss[i] : ss[i];
+  for (int i = 0; i < N; ++i) {
+    c[i] = turns ? c[i] : 1.f;
+    s[i] = turns ? sign * s[i] : 0.f;
+  }
+}
+
+// A lane's eight channels as four fp32 pairs. Where neighbours turn the pairs are (0, 2), (4, 6), (1, 3), (5, 7), so that the
+// rotation multiplies whole pairs: even' = even c + odd s, odd' = odd c - even s; else (0, 1), (2, 3), ...
+template <bool ADJ>
+__device__ constexpr int qk_first(int i) { return ADJ ? (i & 1) * 4 + (i >> 1) : 2 * i; }
+template <bool ADJ>
+__device__ constexpr int qk_second(int i) { return qk_first<ADJ>(i) + (ADJ ? 2 : 1); }
+
+template <typename T, bool ADJ>
+__device__ __forceinline__ void qk_unpack(const uint4& u, uint64_t (&x)[4]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  auto at = [&](int ch) { return ch & 1 ? Pair16<T>::hi(w[ch >> 1]) : Pair16<T>::lo(w[ch >> 1]); };
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = pack2(at(qk_first<ADJ>(i)), at(qk_second<ADJ>(i)));
+}
+template <typename T, bool ADJ>
+__device__ __forceinline__ uint4 qk_pack(const uint64_t (&x)[4]) {
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) unpack2(x[i], f[qk_first<ADJ>(i)], f[qk_second<ADJ>(i)]);
+  return make_uint4(Pair16<T>::pack(f[0], f[1]), Pair16<T>::pack(f[2], f[3]), Pair16<T>::pack(f[4], f[5]),
+                    Pair16<T>::pack(f[6], f[7]));
+}
+
+// Turns a lane's channels. partner: the lane that has their partners (halves; all lanes of the warp take part).
+template <bool ADJ, int N>
+__device__ __forceinline__ void qk_turn(const float (&c)[N], const float (&s)[N], int partner, uint64_t (&x)[4]) {
+  if constexpr (ADJ) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {      // pairs (0, 2) with (1, 3), (4, 6) with (5, 7)
+      const uint64_t c2 = pack2(c[2 * i], c[2 * i + 1]), s2 = pack2(s[2 * i], s[2 * i + 1]),
+                     n2 = pack2(-s[2 * i], -s[2 * i + 1]);
+      const uint64_t e = x[i], o = x[i + 2];
+      x[i] = ffma2(o, s2, fmul2(e, c2));
+      x[i + 2] = ffma2(e, n2, fmul2(o, c2));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float a, b;
+      unpack2(x[i], a, b);
+      a = __shfl_sync(0xffffffffu, a, partner);
+      b = __shfl_sync(0xffffffffu, b, partner);
+      x[i] = ffma2(pack2(a, b), pack2(s[2 * i], s[2 * i + 1]), fmul2(x[i], pack2(c[2 * i], c[2 * i + 1])));
     }
   }
 }
 
-// x <- x c + partner s, in the group (all lanes of the warp take part in the shuffles). sign -1: the inverse turn.
-template <bool ADJ>
-__device__ __forceinline__ void qk_turn(const QkParams& p, int v, const float (&c)[8], const float (&s)[8], float sign,
-                                        float (&x)[8]) {
-  float o[8];
-  if constexpr (ADJ) {
+__device__ __forceinline__ float qk_dot(const uint64_t (&a)[4], const uint64_t (&b)[4]) {
+  uint64_t t = fmul2(a[0], b[0]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = x[i ^ 1];
-  } else {
-    const int hv = p.rot >> 4;                             // vectors in half the turned channels
-    const int lane = threadIdx.x & 31;
-    const int from = v < hv ? lane + hv : v < 2 * hv ? lane - hv : lane;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = __shfl_sync(0xffffffffu, x[i], from);
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = fmaf(x[i], c[i], sign * s[i] * o[i]);
-}
-
-template <typename T>
-__device__ __forceinline__ void qk_unpack(const uint4& u, float (&x)[8]) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = Pair16<T>::lo(w[i]);
-    x[2 * i + 1] = Pair16<T>::hi(w[i]);
-  }
-}
-template <typename T>
-__device__ __forceinline__ uint4 qk_pack(const float (&x)[8]) {
-  return make_uint4(Pair16<T>::pack(x[0], x[1]), Pair16<T>::pack(x[2], x[3]), Pair16<T>::pack(x[4], x[5]),
-                    Pair16<T>::pack(x[6], x[7]));
+  for (int i = 1; i < 4; ++i) t = ffma2(a[i], b[i], t);
+  float lo, hi;
+  unpack2(t, lo, hi);
+  return lo + hi;
 }
 template <int G>
 __device__ __forceinline__ float qk_group_sum(float v) {
@@ -133,142 +172,233 @@ __device__ __forceinline__ float qk_group_sum(float v) {
   for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-__device__ __forceinline__ uint4 qk_load(const QkTensor& t, long long m, int head, int v) {
-  // (a plain load: y may be x)
-  return reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(t.p) + m * t.token + head * t.head)[v];
-}
-__device__ __forceinline__ void qk_store(const QkTensor& t, long long m, int head, int v, const uint4& u) {
-  reinterpret_cast<uint4*>(const_cast<uint16_t*>(static_cast<const uint16_t*>(t.p)) + m * t.token + head * t.head)[v] = u;
-}
-__device__ __forceinline__ void qk_weights(const float* w, int v, bool live, float (&o)[8]) {
+
+// One head's vector of this lane: y of x, or dx of x and dy = gr and its part of dw (if it counts: not padding).
+template <typename T, int G, int TAB, bool ADJ, bool GRAD, int N>
+__device__ __forceinline__ uint4 qk_vector(const uint4& xr, const uint4& gr, const float (&w)[8], const float (&c)[N],
+                                           const float (&s)[N], int partner, bool counts, float inv, float eps,
+                                           uint64_t (&sums)[4]) {
+  uint64_t x[4], h[4];
+  qk_unpack<T, ADJ>(xr, x);
+  auto weighted = [&](uint64_t v, int i) {
+    float a, b;
+    unpack2(v, a, b);
+    return pack2(a * w[qk_first<ADJ>(i)], b * w[qk_second<ADJ>(i)]);
+  };
+  float sq = qk_dot(x, x);
+  if constexpr (!GRAD) {
+    const float rs = rsqrtf(fmaf(qk_group_sum<G>(sq), inv, eps));
 #pragma unroll
-  for (int i = 0; i < 8; ++i) o[i] = w != nullptr && live ? __ldg(w + 8 * v + i) : 1.f;
+    for (int i = 0; i < 4; ++i) h[i] = weighted(x[i], i);
+    if constexpr (TAB != QK_NO_TABLE) qk_turn<ADJ>(c, s, partner, h);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = fmul2(h[i], pack2(rs, rs));
+    return qk_pack<T, ADJ>(h);
+  } else {
+    uint64_t g[4];
+    qk_unpack<T, ADJ>(gr, g);
+    if constexpr (TAB != QK_NO_TABLE) qk_turn<ADJ>(c, s, partner, g);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = weighted(g[i], i);
+    float dot = qk_dot(h, x);
+#pragma unroll
+    for (int ofs = G / 2; ofs > 0; ofs >>= 1) {
+      sq += __shfl_xor_sync(0xffffffffu, sq, ofs);
+      dot += __shfl_xor_sync(0xffffffffu, dot, ofs);
+    }
+    // dx = r h - x r^3 mean(h x), h = g w;  dw += g x r
+    const float rs = rsqrtf(fmaf(sq, inv, eps)), b = -rs * rs * rs * (dot * inv);
+    const uint64_t r2 = pack2(rs, rs), b2 = pack2(b, b);
+    if (counts) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sums[i] = ffma2(fmul2(g[i], x[i]), r2, sums[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = ffma2(h[i], r2, fmul2(x[i], b2));
+    return qk_pack<T, ADJ>(h);
+  }
 }
 
-// GRAD false: y; true: dx and the sums of dw. Blocks of 256 threads, a stride loop over the items.
-template <typename T, int G, bool ADJ, bool GRAD>
-__global__ void __launch_bounds__(256) qk_norm_rope_kernel(const QkParams p) {
-  constexpr int S = 32 / G, U = QK_ROUNDS;
-  chain_begin();
-  const int lane = threadIdx.x & 31, v = lane & (G - 1), sub = lane / G;
-  const bool live = 8 * v < p.head_dim;
-  const int heads = p.heads[0] + p.heads[1], chunks = (heads + S * U - 1) / (S * U);
-  const float inv = 1.0f / static_cast<float>(p.head_dim);
-  float wq[8], wk[8];
-  qk_weights(p.w[0], v, live, wq);
-  qk_weights(p.w[1], v, live, wk);
-  [[maybe_unused]] float sums[2][8];
-  if constexpr (GRAD) {
+// Weights of this lane's channels. (Read again for every token, from L1: registers that the loop does not have to keep.)
+__device__ __forceinline__ void qk_weights(const float* w, int v, float (&o)[8]) {
+  if (w != nullptr) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(w) + 2 * v), b = __ldg(reinterpret_cast<const float4*>(w) + 2 * v + 1);
+    o[0] = a.x; o[1] = a.y; o[2] = a.z; o[3] = a.w; o[4] = b.x; o[5] = b.y; o[6] = b.z; o[7] = b.w;
+  } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sums[0][i] = sums[1][i] = 0.f;
+    for (int i = 0; i < 8; ++i) o[i] = 1.f;
   }
-  const long long items = p.M * chunks;
-  const long long warps = static_cast<long long>(gridDim.x) * (blockDim.x >> 5);
-  for (long long it = static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5); it < items;
-       it += warps) {
-    const long long m = it / chunks;
-    const int h0 = static_cast<int>(it - m * chunks) * (S * U) + sub;
-    uint4 xr[U], gr[GRAD ? U : 1];
+}
+
+// Bytes a lane asks for ahead, past the registers: into its own 16-byte slots of shared memory (zeros where on is false).
+__device__ __forceinline__ void qk_ask(uint32_t slot, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ uint4 qk_got(uint32_t slot) {
+  uint4 u;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(slot) : "memory");
+  return u;
+}
+
+template <int TAB, bool ADJ, bool GRAD>
+struct QkRing {
+  static constexpr int STAGES = 3;
+  static constexpr int VECTORS = (GRAD ? 2 : 1) * QK_ROUNDS + QkTab<TAB, ADJ>::TV;      // of a lane and stage
+  static constexpr int STAGE = VECTORS * 512 + (TAB == QK_NO_TABLE ? 0 : 128);         // of a warp; + the lanes' rows
+  static constexpr int BYTES = 8 * STAGES * STAGE;
+};
+
+// GRAD false: y; true: dx and the sums of dw. Blocks of 256 threads, a stride loop over the tokens; a step is
+// QK_ROUNDS rounds of a token's q heads or k heads, asked for STAGES - 1 steps ahead.
+template <typename T, int G, int TAB, bool ADJ, bool GRAD>
+__global__ void __launch_bounds__(256, GRAD ? 2 : 4) qk_norm_rope_kernel(const QkParams p) {
+  using Ring = QkRing<TAB, ADJ, GRAD>;
+  constexpr int S = 32 / G, R = QK_ROUNDS, N = QkTab<TAB, ADJ>::N, TV = QkTab<TAB, ADJ>::TV, D = Ring::STAGES;
+  extern __shared__ uint4 ring[];
+  chain_begin();
+  const int lane = threadIdx.x & 31, sub = lane / G, v_raw = lane & (G - 1);
+  const bool lane_on = 8 * v_raw < p.head_dim, turns = 8 * v_raw < p.rot;
+  const int v = lane_on ? v_raw : 0;
+  const int hv = p.rot >> 4;                       // vectors in half the turned channels
+  const int partner = ADJ ? lane : v_raw < hv ? lane + hv : v_raw < 2 * hv ? lane - hv : lane;
+  const float inv = 1.0f / static_cast<float>(p.head_dim);
+  const uint32_t slots = smem_u32(ring) + (threadIdx.x >> 5) * (D * Ring::STAGE) + lane * 16;
+  const uint32_t rows = smem_u32(ring) + (threadIdx.x >> 5) * (D * Ring::STAGE) + Ring::VECTORS * 512 + lane * 4;
+  // heads side by side in the warp, and the tokens that leaves room for
+  int width = 1;
+  while (width < S && (width < p.heads[0] || width < p.heads[1])) width *= 2;
+  const int tokens = S / width, head = sub & (width - 1), tok = sub / width;
+  const uint32_t M = static_cast<uint32_t>(p.M), stride = gridDim.x * (blockDim.x >> 5) * tokens;
+  const uint32_t first = (blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * tokens;
+  auto at = [&](const QkTensor& t, uint32_t m, int h) {
+    return const_cast<uint16_t*>(static_cast<const uint16_t*>(t.p)) + static_cast<long long>(m) * t.token +
+           static_cast<long long>(h) * t.head + 8 * v;
+  };
+  // the step that is asked for next: token m_a (of the warp's first lanes), tensor k_a, heads from h_a; its stage
+  uint32_t m_a = first;
+  int k_a = 0, h_a = 0, stage_a = 0, row_a = 0;
+  if (TAB != QK_NO_TABLE && first + tok < M) row_a = qk_row(p, first + tok);
+  auto ask = [&]() {
+    if (m_a < M) {
+      const uint32_t slot = slots + stage_a * Ring::STAGE, m = m_a + tok;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int h = h0 + u * S;
-      const bool on = live && h < heads;
-      const int k = h >= p.heads[0] ? 1 : 0, hh = h - (k ? p.heads[0] : 0);
-      xr[u] = on ? qk_load(p.x[k], m, hh, v) : make_uint4(0u, 0u, 0u, 0u);
-      if constexpr (GRAD) gr[u] = on ? qk_load(p.dy[k], m, hh, v) : make_uint4(0u, 0u, 0u, 0u);
-    }
-    const int row = qk_row(p, m);
-    float c[8], s[8];
-    qk_table<ADJ>(p, row, v, c, s);
-    if (row == -2 && lane == 0) atomicCAS(&g_status, 0, ST_BAD_POSITION);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int h = h0 + u * S;
-      const int k = h >= p.heads[0] ? 1 : 0, hh = h - (k ? p.heads[0] : 0);
-      float x[8];
-      qk_unpack<T>(xr[u], x);
-      float sq = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) sq = fmaf(x[i], x[i], sq);
-      const float r = rsqrtf(fmaf(qk_group_sum<G>(sq), inv, p.eps));
-      float out[8];
-      if constexpr (!GRAD) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) out[i] = x[i] * r * (k ? wk[i] : wq[i]);
-        if (p.table != nullptr) qk_turn<ADJ>(p, v, c, s, 1.f, out);
-      } else {
-        float g[8];
-        qk_unpack<T>(gr[u], g);
-        if (p.table != nullptr) qk_turn<ADJ>(p, v, c, s, -1.f, g);
-        if (row < 0) {        // padding, whatever x and dy hold there: no part of dw (a bad position: NaN, below)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) g[i] = 0.f;
-        }
-        float dot = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          x[i] = row < 0 ? 0.f : x[i] * r;                    // n
-          if (k) sums[1][i] = fmaf(g[i], x[i], sums[1][i]);
-          else sums[0][i] = fmaf(g[i], x[i], sums[0][i]);
-          g[i] *= k ? wk[i] : wq[i];
-          dot = fmaf(g[i], x[i], dot);
-        }
-        dot = qk_group_sum<G>(dot) * inv;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) out[i] = r * fmaf(-x[i], dot, g[i]);
+      for (int r = 0; r < R; ++r) {
+        const int h = h_a + r * width + head;
+        const bool on = lane_on && m < M && h < p.heads[k_a];
+        qk_ask(slot + r * 512, at(p.x[k_a], on ? m : 0, on ? h : 0), on);
+        if constexpr (GRAD) qk_ask(slot + (R + r) * 512, at(p.dy[k_a], on ? m : 0, on ? h : 0), on);
       }
-      if (live && h < heads) {
-        if (row == -1) {
-          qk_store(p.y[k], m, hh, v, make_uint4(0u, 0u, 0u, 0u));
-        } else {
-          if (row < 0) {
+      if (TAB != QK_NO_TABLE && k_a == 0 && h_a == 0) {
+        if (m >= M) row_a = -1;
+        const bool on = turns && row_a >= 0;
+        const long long e = (on ? static_cast<long long>(row_a) * (p.rot >> 1) : 0) + (turns ? qk_entry<ADJ>(p, v_raw) : 0);
+        const char* src = static_cast<const char*>(p.table) + e * (TAB == QK_F32_TABLE ? 8 : 4);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) out[i] = __int_as_float(0x7FC00000);
-          }
-          qk_store(p.y[k], m, hh, v, qk_pack<T>(out));
+        for (int i = 0; i < TV; ++i) qk_ask(slot + ((GRAD ? 2 : 1) * R + i) * 512, src + i * 16, on);
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(rows + stage_a * Ring::STAGE), "r"(row_a) : "memory");
+        if (m + stride < M) row_a = qk_row(p, m + stride);       // (the next token's, a token ahead)
+      }
+      if ((h_a += R * width) >= p.heads[k_a]) {
+        h_a = 0;
+        if (++k_a == 2) {
+          k_a = 0;
+          m_a += stride;
         }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    stage_a = stage_a + 1 == D ? 0 : stage_a + 1;
+  };
+#pragma unroll
+  for (int i = 0; i < D - 1; ++i) ask();
+  uint64_t sums[2][4];
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sums[k][i] = 0ull;
+  int stage = 0;
+  // (m0: the warp's first token, the same for all lanes)
+  for (uint32_t m0 = first; m0 < M; m0 += stride) {
+    const uint32_t m = m0 + tok;
+    int row = 0;
+    float c[N], s[N];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      for (int h0 = 0; h0 < p.heads[k]; h0 += R * width) {
+        ask();
+        asm volatile("cp.async.wait_group %0;" ::"n"(D - 1) : "memory");
+        const uint32_t slot = slots + stage * Ring::STAGE;
+        if (TAB != QK_NO_TABLE && k == 0 && h0 == 0) {
+          uint4 raw[TV > 0 ? TV : 1];
+#pragma unroll
+          for (int i = 0; i < TV; ++i) raw[i] = qk_got(slot + ((GRAD ? 2 : 1) * R + i) * 512);
+          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(row) : "r"(rows + stage * Ring::STAGE) : "memory");
+          if (row == -2) atomicCAS(&g_status, 0, ST_BAD_POSITION);
+          if constexpr (TAB != QK_NO_TABLE) qk_table<TAB, ADJ>(p, raw, turns && row >= 0, v_raw, GRAD ? 1.f : -1.f, c, s);
+        }
+        float w[8];
+        qk_weights(p.w[k], v, w);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          if (r > 0 && h0 + r * width >= p.heads[k]) continue;       // (the same for the launch)
+          const int h = h0 + r * width + head;
+          const uint4 xr = qk_got(slot + r * 512), gr = GRAD ? qk_got(slot + (R + r) * 512) : xr;
+          uint4 o = qk_vector<T, G, TAB, ADJ, GRAD>(xr, gr, w, c, s, partner, TAB == QK_NO_TABLE || row >= 0, inv, p.eps,
+                                                   sums[k]);
+          if (TAB != QK_NO_TABLE && p.positions != nullptr && row < 0) {     // padding: zero; behind the table: NaN
+            const uint32_t u = row == -1 ? 0u : 0x7FFF7FFFu;
+            o = make_uint4(u, u, u, u);
+          }
+          if (lane_on && m < M && h < p.heads[k]) *reinterpret_cast<uint4*>(at(p.y[k], m, h)) = o;
+        }
+        stage = stage + 1 == D ? 0 : stage + 1;
       }
     }
   }
   if constexpr (GRAD) {
     if (p.partial == nullptr) return;
-    __shared__ float red[8][2][G * 8];
+    // (the ring is empty: steps past the last token were not asked for)
+    float* red = reinterpret_cast<float*>(ring);       // [8][2][G * 8]
+    __syncthreads();
 #pragma unroll
     for (int k = 0; k < 2; ++k)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float t = sums[k][i];
+      for (int i = 0; i < 4; ++i) {
+        float t[2];
+        unpack2(sums[k][i], t[0], t[1]);
 #pragma unroll
-        for (int o = G; o < 32; o <<= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-        if (sub == 0) red[threadIdx.x >> 5][k][8 * v + i] = t;
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int o = G; o < 32; o <<= 1) t[e] += __shfl_xor_sync(0xffffffffu, t[e], o);
+          if (sub == 0)
+            red[((threadIdx.x >> 5) * 2 + k) * (G * 8) + 8 * v_raw + (e ? qk_second<ADJ>(i) : qk_first<ADJ>(i))] = t[e];
+        }
       }
     __syncthreads();
     for (int i = threadIdx.x; i < 2 * p.head_dim; i += 256) {
       const int k = i >= p.head_dim ? 1 : 0, ch = i - k * p.head_dim;
       float t = 0.f;
 #pragma unroll
-      for (int w = 0; w < 8; ++w) t += red[w][k][ch];
+      for (int w = 0; w < 8; ++w) t += red[(w * 2 + k) * (G * 8) + ch];
       p.partial[static_cast<long long>(blockIdx.x) * 2 * p.head_dim + i] = t;
     }
   }
 }
 
-// dw: the blocks' sums in their order. 32 channels a block, eight rows of sums side by side.
+// dw: the blocks' sums in their order. Eight channels a block, 32 rows of sums side by side.
 __global__ void __launch_bounds__(256) qk_weight_grad_kernel(const float* partial, int rows, int head_dim, float* dq,
                                                              float* dk) {
   chain_begin();
-  __shared__ float red[8][33];
-  const int col = blockIdx.x * 32 + (threadIdx.x & 31), r0 = threadIdx.x >> 5;
+  __shared__ float red[32][9];
+  const int col = blockIdx.x * 8 + (threadIdx.x & 7), r0 = threadIdx.x >> 3;
   float a = 0.f;
-  if (col < 2 * head_dim) {
 #pragma unroll 8
-    for (int r = r0; r < rows; r += 8) a += partial[static_cast<long long>(r) * 2 * head_dim + col];
-  }
-  red[r0][threadIdx.x & 31] = a;
+  for (int r = r0; r < rows; r += 32) a += partial[static_cast<long long>(r) * 2 * head_dim + col];
+  red[r0][threadIdx.x & 7] = a;
   __syncthreads();
-  if (r0 != 0 || col >= 2 * head_dim) return;
+  if (r0 != 0) return;
 #pragma unroll
-  for (int i = 1; i < 8; ++i) a += red[i][threadIdx.x & 31];
+  for (int i = 1; i < 32; ++i) a += red[i][threadIdx.x & 7];
   if (col < head_dim) {
     if (dq) dq[col] = a;
   } else if (dk) {
@@ -276,26 +406,39 @@ __global__ void __launch_bounds__(256) qk_weight_grad_kernel(const float* partia
   }
 }
 
-inline int qk_group(int head_dim) {
-  int g = 2;
+inline int qk_group(int head_dim) {      // (16 channels in two lanes are no narrower than 32 in four)
+  int g = 4;
   while (g * 8 < head_dim) g *= 2;
   return g;
 }
-inline long long qk_blocks(long long M, int heads, int head_dim, bool grad, int sms) {
-  const int s = 32 / qk_group(head_dim), chunks = (heads + s * QK_ROUNDS - 1) / (s * QK_ROUNDS);
-  const long long blocks = (M * chunks + 7) / 8, cap = static_cast<long long>(sms) * (grad ? 4 : 16);
-  return blocks < cap ? blocks : cap;
+// A token a warp: no more blocks than that takes, and no more than run at once backward (a row of sums each).
+inline int qk_blocks(long long M, bool grad, int sms) {
+  const long long blocks = (M + 7) / 8, cap = static_cast<long long>(sms) * (grad ? 2 : 16);
+  return static_cast<int>(blocks < cap ? blocks : cap);
 }
 
+template <typename T, int G, int TAB, bool ADJ, bool GRAD>
+inline int launch_qk_k(const QkParams& p, int blocks, cudaStream_t st) {
+  auto kern = qk_norm_rope_kernel<T, G, TAB, ADJ, GRAD>;
+  constexpr int bytes = QkRing<TAB, ADJ, GRAD>::BYTES;
+  static_assert(bytes >= 8 * 2 * G * 8 * 4, "the sums of a block");
+  static std::atomic<uint64_t> smem_set;
+  if (const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), bytes, smem_set); e != cudaSuccess)
+    return -static_cast<int>(e) - 1000;
+  return launch_chained(kern, dim3(static_cast<unsigned>(blocks)), 256, bytes, st, 1, p);
+}
 template <typename T, int G, bool GRAD>
-inline int launch_qk_t(const QkParams& p, bool adjacent, unsigned blocks, cudaStream_t st) {
-  return adjacent ? launch_chained(qk_norm_rope_kernel<T, G, true, GRAD>, dim3(blocks), 256, 0, st, 1, p)
-                  : launch_chained(qk_norm_rope_kernel<T, G, false, GRAD>, dim3(blocks), 256, 0, st, 1, p);
+inline int launch_qk_t(const QkParams& p, bool adjacent, int blocks, cudaStream_t st) {
+  if (p.table == nullptr) return launch_qk_k<T, G, QK_NO_TABLE, true, GRAD>(p, blocks, st);
+  if (p.table_f32)
+    return adjacent ? launch_qk_k<T, G, QK_F32_TABLE, true, GRAD>(p, blocks, st)
+                    : launch_qk_k<T, G, QK_F32_TABLE, false, GRAD>(p, blocks, st);
+  return adjacent ? launch_qk_k<T, G, QK_HALF_TABLE, true, GRAD>(p, blocks, st)
+                  : launch_qk_k<T, G, QK_HALF_TABLE, false, GRAD>(p, blocks, st);
 }
 template <typename T, bool GRAD>
-inline int launch_qk_g(const QkParams& p, bool adjacent, unsigned blocks, cudaStream_t st) {
+inline int launch_qk_g(const QkParams& p, bool adjacent, int blocks, cudaStream_t st) {
   switch (qk_group(p.head_dim)) {
-    case 2: return launch_qk_t<T, 2, GRAD>(p, adjacent, blocks, st);
     case 4: return launch_qk_t<T, 4, GRAD>(p, adjacent, blocks, st);
     case 8: return launch_qk_t<T, 8, GRAD>(p, adjacent, blocks, st);
     case 16: return launch_qk_t<T, 16, GRAD>(p, adjacent, blocks, st);
@@ -303,9 +446,9 @@ inline int launch_qk_g(const QkParams& p, bool adjacent, unsigned blocks, cudaSt
   }
 }
 template <bool GRAD>
-inline int launch_qk(const QkParams& p, bool adjacent, bool fp16, long long blocks, cudaStream_t st) {
-  return fp16 ? launch_qk_g<__half, GRAD>(p, adjacent, static_cast<unsigned>(blocks), st)
-              : launch_qk_g<__nv_bfloat16, GRAD>(p, adjacent, static_cast<unsigned>(blocks), st);
+inline int launch_qk(const QkParams& p, bool adjacent, bool fp16, int blocks, cudaStream_t st) {
+  return fp16 ? launch_qk_g<__half, GRAD>(p, adjacent, blocks, st)
+              : launch_qk_g<__nv_bfloat16, GRAD>(p, adjacent, blocks, st);
 }
 
 }  // namespace strata

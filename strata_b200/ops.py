@@ -716,6 +716,10 @@ def _qk_arguments(q, k, q_weight, k_weight, rope_cs, positions, tokens_per_tile,
         raise ValueError(f"head_dim must be a multiple of 8 up to 256 and both have heads, got {hq} + {hk} heads of {hd}")
     M = qs[0] if len(qs) == 3 else qs[:-2].numel()
     wq, wk = _f32_like(q_weight, "q_weight", hd, q), _f32_like(k_weight, "k_weight", hd, q)
+    if wq is not None and wq.data_ptr() & 15:
+        wq = wq.clone()
+    if wk is not None and wk.data_ptr() & 15:
+        wk = wk.clone()
     if rope_cs is None:
         if positions is not None:
             raise ValueError("positions are rows of rope_cs: give both or neither")
@@ -818,7 +822,7 @@ def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k
     with _lib.on_device(q):
         need, ws = 0, None
         if M and (wq is not None or wk is not None):
-            need = lib.strata_qk_norm_rope_backward_workspace_bytes(M, hq + hk, hd)
+            need = lib.strata_qk_norm_rope_backward_workspace_bytes(M, hd)
             ws = _scratch(need, q)
         code = lib.strata_qk_norm_rope_backward(
             dq3.data_ptr(), dq_token, dq_head, dk3.data_ptr(), dk_token, dk_head, q3.data_ptr(), q_token, q_head,

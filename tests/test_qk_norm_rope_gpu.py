@@ -112,7 +112,8 @@ def test_by_position(ops, M, hq, hk, hd, rot, adjacent, t, f32, weights):
         rot = 0
     d = data(M, hq, hk, hd, t, rot=rot, rows=77, f32=f32, weights=weights, seed=M)
     if not rot:
-        return check(ops, d, adjacent)
+        check(ops, d, adjacent)
+        return
     pos = torch.randint(0, 77, (M,), device="cuda", dtype=torch.int64 if f32 else torch.int32)
     pos[M // 2:M // 2 + 2] = torch.tensor([0, 76], device="cuda", dtype=pos.dtype)[:M - M // 2]
     check(ops, d, adjacent, pos.long(), positions=pos)

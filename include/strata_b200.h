@@ -76,7 +76,8 @@ int strata_linear_bf16(const void* x, int64_t ldx, const void* w, int64_t ldw, c
 /* Dense layer: y[M,N] = residual + act(z), z = x[M,K] W[N,K]^T + bias, any M, N, K and row strides; x, W, residual, y
  * and preact are of one 16-bit type (dtype), bias fp32; sums and the epilogue are fp32, y is rounded once. residual,
  * bias and preact may be NULL; preact receives z, which the backward pass needs for any activation. y may be residual
- * (same stride), nothing else may overlap.
+ * (same stride), nothing else may overlap. padded != 0: the columns behind N up to the next multiple of 8 are the
+ * caller's to write in every row of y and preact (zeros may land there), which lets rows of such strides use TMA.
  * workspace: 256-byte aligned, of strata_linear_act_workspace_bytes(M, N, K, x_aligned, w_aligned) bytes (negative: an
  * error code), where an operand counts as aligned when its address and its row stride are multiples of 16 bytes (others
  * are copied there first). Up to 8 rows are one launch without workspace; M = 0 does nothing. Replaces the nn.Linear
@@ -84,18 +85,18 @@ int strata_linear_bf16(const void* x, int64_t ldx, const void* w, int64_t ldw, c
 int64_t strata_linear_act_workspace_bytes(int M, int N, int K, int x_aligned, int w_aligned);
 int strata_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const float* bias, const void* residual,
                       int64_t ldr, void* y, int64_t ldy, void* preact, int64_t ldz, int M, int N, int K, int activation,
-                      int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+                      int dtype, int padded, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Its gradients, from dy[M,N] and the stored z (preact; unused for STRATA_ACT_NONE):
  *   dz = dy act'(z), dx[M,K] = dz W, dW[N,K] = dz^T x, db[N] = sum over the rows of dz (fp32).
  * Outputs that are NULL are not computed, and x (w) may be NULL without dw (dx). dz is rounded to the 16-bit type in
  * front of the two products (not for db, and not without an activation). No atomics: the same bits every time. M = 0
- * sets dW and db to zero. Workspace as above. */
+ * sets dW and db to zero. Workspace and padded (for dx) as above. */
 int64_t strata_linear_act_backward_workspace_bytes(int M, int N, int K, int activation, int dy_aligned, int z_aligned,
                                                    int x_aligned, int w_aligned, int need_dx, int need_dw, int need_db);
 int strata_linear_act_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, int64_t ldw,
                                const void* preact, int64_t ldz, void* dx, int64_t lddx, void* dw, int64_t lddw,
-                               float* db, int M, int N, int K, int activation, int dtype, void* workspace,
+                               float* db, int M, int N, int K, int activation, int dtype, int padded, void* workspace,
                                int64_t workspace_bytes, void* stream);
 
 /* y[M,C] = aux + [gate *] (W2 gelu(W1 x + b1) + b2): the MLP of a narrow block in one kernel, same bits as

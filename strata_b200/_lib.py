@@ -62,12 +62,12 @@ _SIGNATURES = {
                                    c_void_p]),
     "strata_linear_act_workspace_bytes": (c_int64, [c_int] * 5),
     "strata_linear_act": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64,
-                                  c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int64,
+                                  c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int64,
                                   c_void_p]),
     "strata_linear_act_backward_workspace_bytes": (c_int64, [c_int] * 11),
     "strata_linear_act_backward": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64,
                                            c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_int,
-                                           c_int, c_void_p, c_int64, c_void_p]),
+                                           c_int, c_int, c_void_p, c_int64, c_void_p]),
     "strata_mlp_fused": (c_int, [c_int, c_int, c_int]),
     "strata_mlp_bf16": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
                                 c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int, c_void_p]),

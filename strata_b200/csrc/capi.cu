@@ -155,7 +155,7 @@ int64_t strata_linear_act_workspace_bytes(int M, int N, int K, int x_aligned, in
 
 int strata_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const float* bias, const void* residual,
                       int64_t ldr, void* y, int64_t ldy, void* preact, int64_t ldz, int M, int N, int K, int activation,
-                      int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+                      int dtype, int padded, void* workspace, int64_t workspace_bytes, void* stream) {
   const int sms = current_sm_count();
   if (sms <= 0) return STRATA_ERR_NO_DEVICE;
   if (!dense_sizes(M, N, K, activation, dtype)) return STRATA_ERR_ARG;
@@ -175,8 +175,8 @@ int strata_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, co
   p.bias = bias;
   p.act = activation;
   p.fp16 = dtype == STRATA_F16;
-  p.direct = !dense_whole(y, ldy, N) || (preact && !dense_whole(preact, ldz, N)) ||
-             (residual && !dense_aligned(residual, ldr));
+  p.direct_out = !dense_whole(y, ldy, N, padded != 0) || (preact && !dense_whole(preact, ldz, N, padded != 0));
+  p.direct_aux = residual && !dense_aligned(residual, ldr);
   return launch_dense_forward({x, ldx}, {w, ldw}, p, workspace, sms, as_stream(stream));
 }
 
@@ -193,7 +193,7 @@ int64_t strata_linear_act_backward_workspace_bytes(int M, int N, int K, int acti
 
 int strata_linear_act_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, int64_t ldw,
                                const void* preact, int64_t ldz, void* dx, int64_t lddx, void* dw, int64_t lddw,
-                               float* db, int M, int N, int K, int activation, int dtype, void* workspace,
+                               float* db, int M, int N, int K, int activation, int dtype, int padded, void* workspace,
                                int64_t workspace_bytes, void* stream) {
   const int sms = current_sm_count();
   if (sms <= 0) return STRATA_ERR_NO_DEVICE;
@@ -218,7 +218,7 @@ int strata_linear_act_backward(const void* dy, int64_t lddy, const void* x, int6
   if (g.bytes > 0 && (!workspace || workspace_bytes < g.bytes || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0))
     return STRATA_ERR_ARG;
   DenseGradParams q{};
-  q.M = M; q.N = N; q.K = K; q.act = activation; q.fp16 = dtype == STRATA_F16;
+  q.M = M; q.N = N; q.K = K; q.act = activation; q.fp16 = dtype == STRATA_F16; q.padded = padded != 0;
   q.dy = {dy, lddy}; q.x = {x, ldx}; q.w = {w, ldw}; q.z = {preact, ldz};
   q.dx = dx; q.lddx = lddx; q.dw = dw; q.lddw = lddw; q.db = db;
   return launch_dense_backward(q, g, sms, st);

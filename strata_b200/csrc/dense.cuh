@@ -102,9 +102,11 @@ inline int launch_dense_t(const DenseOperand& A, const DenseOperand& B, const De
   tmOut = tmKeep = tmAux = tmA;
   using S = DenseSmem<BN, PAIR, EPI, AUX && EPI == DENSE_Y>;
   constexpr TmapSwizzle sw = S::BOX_COLS == 64 ? TMAP_SWIZZLE_128B : TMAP_SWIZZLE_64B;
-  if (EPI != DENSE_PART && !p.direct) {
+  if (EPI != DENSE_PART && p.aux && !p.direct_aux &&
+      map(&tmAux, {p.aux, p.ldaux}, p.M, p.N, S::BOX_COLS, 32, sw) != 0)
+    return -23;
+  if (EPI != DENSE_PART && !p.direct_out) {
     if (map(&tmOut, {p.out, p.ldo}, p.M, p.N, S::BOX_COLS, 32, sw) != 0) return -22;
-    if (p.aux && map(&tmAux, {p.aux, p.ldaux}, p.M, p.N, S::BOX_COLS, 32, sw) != 0) return -23;
     if (p.keep && map(&tmKeep, {p.keep, p.ldk}, p.M, p.N, S::BOX_COLS, 32, sw) != 0) return -25;
   }
   auto kern = dense_tcgen05_kernel<BN, PAIR, LAY, EPI, T, ACT, AUX>;
@@ -137,7 +139,7 @@ template <int LAY, int EPI, typename T>
 inline int launch_dense_bn(int bn, const DenseOperand& A, const DenseOperand& B, const DenseParams& p, int units,
                            cudaStream_t st) {
   if constexpr (LAY == DENSE_NT && EPI != DENSE_PART) {
-    if (bn == 256 && !p.direct)
+    if (bn == 256 && !p.direct_out && !p.direct_aux)
       return p.aux ? launch_dense_pair<EPI, T, true>(A, B, p, units, st)
                    : launch_dense_pair<EPI, T, false>(A, B, p, units, st);
   }
@@ -189,30 +191,62 @@ inline int launch_dense(const DenseOperand& A, const DenseOperand& B, DenseParam
   return launch_dense_finish(f, st);
 }
 
-template <typename T>
-inline int launch_few_rows_t(const DenseOperand& x, const DenseOperand& w, const DenseParams& p, bool vec, int sms,
+// Few rows: dot products up to DOT_ROWS, else mma.sync.
+template <typename T, bool ALIGNED>
+inline int launch_few_rows_t(const DenseOperand& x, const DenseOperand& w, const DenseParams& p, int sms,
                              cudaStream_t st) {
-  // warps: a column group of four each; split along the contraction until every SM has eight
-  const int groups = (p.N + FEW_COLS - 1) / FEW_COLS;
-  int kw = 1;
-  while (kw < 8 && groups * kw < 8 * sms && p.K >= 2 * kw * 32 * (vec ? 8 : 1)) kw *= 2;
-  const dim3 grid(static_cast<unsigned>((groups + 8 / kw - 1) / (8 / kw)));
   const T* xp = static_cast<const T*>(x.p);
   const T* wp = static_cast<const T*>(w.p);
-#define STRATA_FEW(R)                                                                                              \
-  (vec ? launch_chained(dense_few_rows_kernel<T, R, 8>, grid, 256, 0, st, 1, xp, x.ld, wp, w.ld, kw, p)            \
-       : launch_chained(dense_few_rows_kernel<T, R, 1>, grid, 256, 0, st, 1, xp, x.ld, wp, w.ld, kw, p))
-  if (p.M == 1) return STRATA_FEW(1);
-  if (p.M == 2) return STRATA_FEW(2);
-  if (p.M <= 4) return STRATA_FEW(4);
-  return STRATA_FEW(8);
-#undef STRATA_FEW
+  if (p.M <= DOT_ROWS) {
+    // warps: four columns each, split along the contraction until every SM has eight
+    const int groups = (p.N + DOT_COLS - 1) / DOT_COLS;
+    int kw = 1;
+    while (kw < 8 && groups * kw < 8 * sms && p.K >= 512 * kw) kw *= 2;
+    const dim3 grid(static_cast<unsigned>((groups + 8 / kw - 1) / (8 / kw)));
+    auto go = [&](auto kern) { return launch_chained(kern, grid, 256, 0, st, 1, xp, x.ld, wp, w.ld, kw, p); };
+    if (p.M == 1) return go(dense_dot_rows_kernel<T, 1, ALIGNED>);
+    if (p.M == 2) return go(dense_dot_rows_kernel<T, 2, ALIGNED>);
+    return go(dense_dot_rows_kernel<T, 4, ALIGNED>);
+  }
+  // a cluster along the contraction where a warp would make more than two steps of it
+  const int blocks = (p.N + FEW_COLS - 1) / FEW_COLS, steps = (p.K + FEW_STEP - 1) / FEW_STEP;
+  int parts = 1;
+  while (parts < 8 && steps > 2 * parts && 2 * parts * blocks <= 8 * sms) parts *= 2;
+  const int k_part = (steps + parts - 1) / parts * FEW_STEP;
+  auto go = [&](auto kern) {
+    return launch_chained(kern, dim3(static_cast<unsigned>(blocks * parts)), 32 * FEW_WARPS, 0, st, parts, xp, x.ld, wp, w.ld,
+                          k_part, parts, p);
+  };
+  if (p.M <= 8) return go(dense_few_rows_kernel<T, 1, ALIGNED>);
+  if (p.M <= 16) return go(dense_few_rows_kernel<T, 2, ALIGNED>);
+  return go(dense_few_rows_kernel<T, 4, ALIGNED>);
+}
+inline int launch_few_rows(const DenseOperand& x, const DenseOperand& w, const DenseParams& p, bool aligned, int sms,
+                           cudaStream_t st) {
+  if (p.fp16)
+    return aligned ? launch_few_rows_t<__half, true>(x, w, p, sms, st) : launch_few_rows_t<__half, false>(x, w, p, sms, st);
+  return aligned ? launch_few_rows_t<__nv_bfloat16, true>(x, w, p, sms, st)
+                 : launch_few_rows_t<__nv_bfloat16, false>(x, w, p, sms, st);
+}
+
+// Whether the forms for a few rows take a product: one launch and no workspace. From nine rows on every block of 16 columns
+// reads more of x than of W, and the tiles of a split product overtake them at large weights. Microseconds of these /
+// of a split, weights out of HBM (half, gelu, residual): 9 x 1024, K = 1024 3.8 / 5.8; 16 x 2048, K = 2048 6.0 / 10.6;
+// 24 x 1024, K = 4096 8.0 / 8.5; 24 x 4096, K = 1024 7.7 / 8.4; 32 x 512, K = 2048 5.2 / 7.8; 32 x 4096, K = 4096 21.9 / 13.6;
+// 48 x 1024, K = 4096 16.2 / 8.7; 8 x 4096, K = 4096 13.3 / 14.0. Dot products / mma.sync: 1 x 4096, K = 1024 4.3 / 5.0; 1 x
+// 1024, K = 4096 4.1 / 7.8; 4 x 4096, K = 1024 4.9 / 5.0; 8 x 4096, K = 1024 12.7 / 5.0.
+inline bool dense_few(int M, int N, int K) {
+  const long long weights = static_cast<long long>(N) * K;
+  return M <= 8 || (M <= FEW_ROWS && (M <= 16 ? 2 : 4) * weights <= (1ll << 25));
 }
 
 inline long long dense_round8(long long n) { return (n + 7) / 8 * 8; }
 inline bool dense_aligned(const void* p, long long ld) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % 8 == 0; }
-// Rows that TMA may store: it writes whole 16-byte pieces, with zeros behind the last column.
-inline bool dense_whole(const void* p, long long ld, int cols) { return dense_aligned(p, ld) && cols % 8 == 0; }
+// Rows that TMA may store: it writes whole 16-byte pieces, with zeros behind the last column. padded: those are the
+// caller's to write.
+inline bool dense_whole(const void* p, long long ld, int cols, bool padded) {
+  return dense_aligned(p, ld) && (cols % 8 == 0 || padded);
+}
 
 // Pieces of a workspace, 256-byte aligned.
 struct DenseArena {
@@ -227,11 +261,8 @@ struct DenseArena {
 
 inline int launch_align_rows(const AlignRows& a, int n, int sms, cudaStream_t st) {
   long long most = 0;
-  for (int j = 0; j < n; ++j) {
-    const long long v = a.rows[j] * (a.ldd[j] / 8);
-    most = v > most ? v : most;
-  }
-  long long blocks = (most + 255) / 256;
+  for (int j = 0; j < n; ++j) most = a.rows[j] > most ? a.rows[j] : most;
+  long long blocks = (most + 31) / 32;
   if (blocks > 8LL * sms) blocks = 8LL * sms;
   return launch_chained(dense_align_rows_kernel, dim3(static_cast<unsigned>(blocks), n), 256, 0, st, 1, a);
 }
@@ -240,7 +271,7 @@ inline int launch_align_rows(const AlignRows& a, int n, int sms, cudaStream_t st
 // Workspace: aligned copies of x and w where they are not aligned themselves, then the slabs of a split. With base
 // nullptr nothing is launched and `used` says how much is needed.
 inline int64_t dense_forward_bytes(int M, int N, int K, bool x_ok, bool w_ok, int sms) {
-  if (M <= FEW_ROWS) return 0;
+  if (dense_few(M, N, K)) return 0;
   DenseArena ws{nullptr, 0};
   if (!x_ok) ws.take(2 * dense_round8(K) * M);
   if (!w_ok) ws.take(2 * dense_round8(K) * N);
@@ -251,10 +282,8 @@ inline int64_t dense_forward_bytes(int M, int N, int K, bool x_ok, bool w_ok, in
 inline int launch_dense_forward(DenseOperand x, DenseOperand w, const DenseParams& p, void* workspace, int sms,
                                 cudaStream_t st) {
   const bool x_ok = dense_aligned(x.p, x.ld), w_ok = dense_aligned(w.p, w.ld);
-  if (p.M <= FEW_ROWS) {
-    const bool vec = x_ok && w_ok && p.K % 8 == 0;
-    return p.fp16 ? launch_few_rows_t<__half>(x, w, p, vec, sms, st)
-                  : launch_few_rows_t<__nv_bfloat16>(x, w, p, vec, sms, st);
+  if (dense_few(p.M, p.N, p.K)) {
+    return launch_few_rows(x, w, p, x_ok && w_ok && p.K % 8 == 0, sms, st);
   }
   DenseArena ws{static_cast<uint8_t*>(workspace), 0};
   AlignRows a{};
@@ -278,6 +307,7 @@ inline int launch_dense_forward(DenseOperand x, DenseOperand w, const DenseParam
 // ---------------------------------------------------------------- backward
 struct DenseGradParams {
   int M, N, K, act, fp16;
+  bool padded;                     // dx may be written up to whole 16-byte pieces of its rows
   DenseOperand dy, x, w, z;        // z.p nullptr: act is none
   void* dx; long long lddx;        // any of the three outputs may be absent
   void* dw; long long lddw;
@@ -286,9 +316,9 @@ struct DenseGradParams {
 
 struct DenseGradSums { int lanes, cols, rows_per_block, blocks; };     // geometry of dense_slope_kernel
 
-inline DenseGradSums dense_grad_sums(int M, int N, int vec, int sms) {
+inline DenseGradSums dense_grad_sums(int M, int N, int sms) {
   DenseGradSums g{};
-  const int units = (N + vec - 1) / vec;
+  const int units = (N + 7) / 8;
   g.lanes = 1;
   while (g.lanes < 32 && g.lanes < units) g.lanes *= 2;
   g.cols = (units + g.lanes - 1) / g.lanes;
@@ -304,7 +334,7 @@ inline DenseGradSums dense_grad_sums(int M, int N, int vec, int sms) {
 
 // dz goes through memory when there is an activation, or when dy is not aligned; then it is [M, round8(N)].
 struct DenseGradPlan {
-  bool copy_x, copy_w, make_dz, vec;
+  bool copy_x, copy_w, make_dz, aligned;
   DenseChoice cx, cw;
   DenseGradSums sums;
   int64_t bytes;
@@ -318,8 +348,8 @@ inline DenseGradPlan dense_grad_plan(int M, int N, int K, bool act, bool dy_ok, 
   g.make_dz = (dx || dw) && (act || !dy_ok);
   g.copy_x = dw && !x_ok;
   g.copy_w = dx && !w_ok;
-  g.vec = dy_ok && (!act || z_ok) && N % 8 == 0;
-  g.sums = dense_grad_sums(M, N, g.vec ? 8 : 1, sms);
+  g.aligned = dy_ok && (!act || z_ok) && N % 8 == 0;
+  g.sums = dense_grad_sums(M, N, sms);
   if (dx) g.cx = dense_choice(M, K, N, sms);
   if (dw) g.cw = dense_choice(N, K, M, sms);
   DenseArena ws{static_cast<uint8_t*>(workspace), 0};
@@ -358,11 +388,9 @@ inline int launch_dense_backward(const DenseGradParams& q, const DenseGradPlan& 
     s.sums = g.col_sums;
     s.M = q.M; s.N = q.N; s.act = q.act; s.lanes = g.sums.lanes; s.rows_per_block = g.sums.rows_per_block;
     const dim3 grid(static_cast<unsigned>(g.sums.cols), static_cast<unsigned>(g.sums.blocks));
-#define STRATA_SLOPE(T) \
-  (g.vec ? launch_chained(dense_slope_kernel<T, 8>, grid, 256, 0, st, 1, s) \
-         : launch_chained(dense_slope_kernel<T, 1>, grid, 256, 0, st, 1, s))
-    r = q.fp16 ? STRATA_SLOPE(__half) : STRATA_SLOPE(__nv_bfloat16);
-#undef STRATA_SLOPE
+    auto go = [&](auto kern) { return launch_chained(kern, grid, 256, 0, st, 1, s); };
+    if (q.fp16) r = g.aligned ? go(dense_slope_kernel<__half, true>) : go(dense_slope_kernel<__half, false>);
+    else r = g.aligned ? go(dense_slope_kernel<__nv_bfloat16, true>) : go(dense_slope_kernel<__nv_bfloat16, false>);
     if (r != 0) return r;
     if (g.make_dz) dz = {g.dz, dense_round8(q.N)};
   }
@@ -370,7 +398,7 @@ inline int launch_dense_backward(const DenseGradParams& q, const DenseGradPlan& 
     DenseParams p{};
     p.M = q.M; p.N = q.K; p.K = q.N;
     p.out = q.dx; p.ldo = q.lddx; p.fp16 = q.fp16;
-    p.direct = !dense_whole(q.dx, q.lddx, q.K);
+    p.direct_out = !dense_whole(q.dx, q.lddx, q.K, q.padded);
     if ((r = launch_dense<DENSE_NN>(dz, w, p, g.cx, g.slabs, nullptr, st)) != 0) return r;
   }
   DenseFinish f{};
@@ -380,7 +408,7 @@ inline int launch_dense_backward(const DenseGradParams& q, const DenseGradPlan& 
     DenseParams p{};
     p.M = q.N; p.N = q.K; p.K = q.M;
     p.out = q.dw; p.ldo = q.lddw; p.fp16 = q.fp16;
-    p.direct = !dense_whole(q.dw, q.lddw, q.K);
+    p.direct_out = !dense_whole(q.dw, q.lddw, q.K, false);
     return launch_dense<DENSE_TN>(dz, x, p, g.cw, g.slabs, q.db ? &f : nullptr, st);
   }
   return q.db ? launch_dense_finish(f, st) : 0;

@@ -5,67 +5,112 @@
 
 namespace strata {
 
-// ---------------------------------------------------------------- y = r + act(x W^T + b) for 1 to 8 rows
-// Bound by the weights' way from HBM (2 N K bytes; at one row an operation per byte), so no tensor cores: a 128-row
-// tile would read the same bytes through N / 64 CTAs. A warp takes four output columns and all rows; its lanes have 16
-// bytes of each of the four weight rows in flight at a time and share the x they multiply them with. kw of the block's
-// eight warps split the contraction where N alone does not give every SM enough warps. Sums are fp32, even and odd k
-// apart, then over the lanes and the kw warps in a fixed order.
-constexpr int FEW_ROWS = 8;
-constexpr int FEW_COLS = 4;
-
-template <typename T, int VEC>
-__device__ __forceinline__ void few_load(const T* p, uint64_t (&v)[VEC == 8 ? 4 : 1]) {
-  if constexpr (VEC == 8) {
-    const uint4 w = __ldg(reinterpret_cast<const uint4*>(p));
-    v[0] = pack2(Pair16<T>::lo(w.x), Pair16<T>::hi(w.x));
-    v[1] = pack2(Pair16<T>::lo(w.y), Pair16<T>::hi(w.y));
-    v[2] = pack2(Pair16<T>::lo(w.z), Pair16<T>::hi(w.z));
-    v[3] = pack2(Pair16<T>::lo(w.w), Pair16<T>::hi(w.w));
-  } else {
-    v[0] = pack2(to_f32<T>(__ldg(p)), 0.f);
+// Eight values of a row from p on, of which n exist (n <= 0: none), the others zero. ALIGNED: p is a multiple of 16 bytes and
+// n >= 8 or n <= 0. Otherwise the two aligned 16-byte pieces that hold them are read and shifted together: a piece is
+// read only if it holds a value that exists, and memory is given out in larger units than 16 bytes.
+template <bool ALIGNED>
+__device__ __forceinline__ uint4 load8(const void* p, int n) {
+  uint4 u = make_uint4(0u, 0u, 0u, 0u);
+  if (n <= 0) return u;
+  if constexpr (ALIGNED) return __ldg(static_cast<const uint4*>(p));
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+  const int off = static_cast<int>(a & 15u) >> 1;
+  const uint4* q = reinterpret_cast<const uint4*>(a & ~static_cast<uintptr_t>(15));
+  const uint4 lo = __ldg(q);
+  uint4 hi = u;
+  if (off + (n < 8 ? n : 8) > 8) hi = __ldg(q + 1);
+  uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+  if (off & 4) {
+#pragma unroll
+    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
   }
+  if (off & 2) {
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+  }
+  const uint32_t bits = (off & 1) * 16;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], bits);
+  if (n < 8) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = 2 * i + 1 < n ? w[i] : (2 * i < n ? w[i] & 0xFFFFu : 0u);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-template <typename T, int ROWS, int VEC>
-__global__ void __launch_bounds__(256) dense_few_rows_kernel(const T* __restrict__ x, long long ldx,
+// The epilogue for one output.
+template <typename T>
+__device__ __forceinline__ void dense_one(const DenseParams& p, int row, int col, float z) {
+  if (row >= p.M || col >= p.N) return;
+  if (p.bias != nullptr) z += __ldg(p.bias + col);
+  if (p.keep != nullptr) static_cast<T*>(p.keep)[row * p.ldk + col] = from_f32<T>(z);
+  uint64_t y[1] = {pack2(z, 0.f)};
+  dense_act<T>(p.act, y);
+  float a, b;
+  unpack2(y[0], a, b);
+  if (p.aux != nullptr) a += to_f32<T>(static_cast<const T*>(p.aux)[row * p.ldaux + col]);
+  static_cast<T*>(p.out)[row * p.ldo + col] = from_f32<T>(a);
+}
+
+// ---------------------------------------------------------------- y = r + act(x W^T + b) for one to four rows
+// Bound by the weights' way from HBM (2 N K bytes; at one row an operation per byte), so no tensor cores. A warp takes four
+// output columns and all rows; its lanes have 16 bytes of each of the four weight rows in flight at a time, whole lines of
+// a row, and share the x they multiply them with. kw of the block's eight warps split the contraction where N alone does
+// not give every SM enough warps. Sums are fp32, even and odd k apart, then over the lanes and the kw warps in a fixed
+// order.
+constexpr int DOT_ROWS = 4;
+constexpr int DOT_COLS = 4;
+
+template <typename T>
+__device__ __forceinline__ void dot_pairs(const uint4& u, uint64_t (&v)[4]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = pack2(Pair16<T>::lo(w[i]), Pair16<T>::hi(w[i]));
+}
+
+template <typename T, int ROWS, bool ALIGNED>
+__global__ void __launch_bounds__(256) dense_dot_rows_kernel(const T* __restrict__ x, long long ldx,
                                                              const T* __restrict__ w, long long ldw, int kw,
                                                              const DenseParams p) {
-  constexpr int NP = VEC == 8 ? 4 : 1, NV = FEW_COLS * ROWS;
+  constexpr int NV = DOT_COLS * ROWS;
   __shared__ float red[8][NV];
   chain_begin();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = warp / kw, part = warp - group * kw;
-  const int col0 = (blockIdx.x * (8 / kw) + group) * FEW_COLS;
-  uint64_t acc[FEW_COLS][ROWS];
+  const int col0 = (blockIdx.x * (8 / kw) + group) * DOT_COLS;
+  uint64_t acc[DOT_COLS][ROWS];
 #pragma unroll
-  for (int c = 0; c < FEW_COLS; ++c)
+  for (int c = 0; c < DOT_COLS; ++c)
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) acc[c][r] = 0ull;
-  const T* wr[FEW_COLS];
+  // (columns and rows that do not exist repeat the last one)
+  const T* wr[DOT_COLS];
 #pragma unroll
-  for (int c = 0; c < FEW_COLS; ++c) wr[c] = w + min(col0 + c, p.N - 1) * ldw;
+  for (int c = 0; c < DOT_COLS; ++c) wr[c] = w + min(col0 + c, p.N - 1) * ldw;
   const T* xr[ROWS];
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) xr[r] = x + min(r, p.M - 1) * ldx;
 #pragma unroll(ROWS <= 2 ? 4 : 2)
-  for (int k = (part * 32 + lane) * VEC; k < p.K; k += kw * 32 * VEC) {
-    uint64_t wv[FEW_COLS][NP];
+  for (int k = (part * 32 + lane) * 8; k < p.K; k += kw * 256) {
+    uint4 raw[DOT_COLS];
 #pragma unroll
-    for (int c = 0; c < FEW_COLS; ++c) few_load<T, VEC>(wr[c] + k, wv[c]);
+    for (int c = 0; c < DOT_COLS; ++c) raw[c] = load8<ALIGNED>(wr[c] + k, p.K - k);
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
-      uint64_t xv[NP];
-      few_load<T, VEC>(xr[r] + k, xv);
+      uint64_t xv[4];
+      dot_pairs<T>(load8<ALIGNED>(xr[r] + k, p.K - k), xv);
 #pragma unroll
-      for (int c = 0; c < FEW_COLS; ++c)
+      for (int c = 0; c < DOT_COLS; ++c) {
+        uint64_t wv[4];
+        dot_pairs<T>(raw[c], wv);
 #pragma unroll
-        for (int q = 0; q < NP; ++q) acc[c][r] = ffma2(wv[c][q], xv[q], acc[c][r]);
+        for (int q = 0; q < 4; ++q) acc[c][r] = ffma2(wv[q], xv[q], acc[c][r]);
+      }
     }
   }
   float v[NV];
 #pragma unroll
-  for (int c = 0; c < FEW_COLS; ++c)
+  for (int c = 0; c < DOT_COLS; ++c)
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
       float lo, hi;
@@ -85,22 +130,107 @@ __global__ void __launch_bounds__(256) dense_few_rows_kernel(const T* __restrict
   }
   for (; off >= 1; off >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], off);
   constexpr int SHARE = 32 / NV;
-  const int idx = lane / SHARE;
-  if (lane % SHARE == 0) red[warp][idx] = v[0];
+  if (lane % SHARE == 0) red[warp][lane / SHARE] = v[0];
   __syncthreads();
   if (part != 0 || lane >= NV) return;
   float z = 0.f;
   for (int i = 0; i < kw; ++i) z += red[warp + i][lane];
-  const int col = col0 + lane / ROWS, row = lane % ROWS;
-  if (col >= p.N || row >= p.M) return;
-  if (p.bias != nullptr) z += __ldg(p.bias + col);
-  if (p.keep != nullptr) static_cast<T*>(p.keep)[row * p.ldk + col] = from_f32<T>(z);
-  uint64_t y[1] = {pack2(z, 0.f)};
-  dense_act<T>(p.act, y);
-  float a, b;
-  unpack2(y[0], a, b);
-  if (p.aux != nullptr) a += to_f32<T>(static_cast<const T*>(p.aux)[row * p.ldaux + col]);
-  static_cast<T*>(p.out)[row * p.ldo + col] = from_f32<T>(a);
+  dense_one<T>(p, lane % ROWS, col0 + lane / ROWS, z);
+}
+
+// ---------------------------------------------------------------- y = r + act(x W^T + b) for a few rows
+// Bound by the weights' way from HBM (2 N K bytes) and by latency: a 128-row tile on tcgen05 would read them through N /
+// 64 CTAs and one pipeline each, or need a second kernel and a workspace to add up a split. Here a block has 16 output
+// columns and all rows; its eight warps, and where K is long the blocks of a cluster, split the contraction so that every
+// warp has all it reads in flight at once. A lane reads 16 bytes of two weight rows and of a row of x straight into the
+// fragments of mma.sync.m16n8k16: the product does not care which k is which as long as both operands agree, so
+// lane t of a quad takes k = 8 t ... 8 t + 7 of 32 and hands them over as two steps of 16. Sums are fp32, over the warps
+// and then over the cluster (through distributed shared memory) in a fixed order.
+constexpr int FEW_ROWS = 32;
+constexpr int FEW_COLS = 16;
+constexpr int FEW_WARPS = 8;
+constexpr int FEW_STEP = 32 * FEW_WARPS;      // contraction values that a block takes at a time
+
+template <typename T>
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
+  if constexpr (Pair16<T>::UMMA_FORMAT == 1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  } else {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+}
+
+// NT: blocks of eight rows. k_part: contraction values of a block of the cluster, a multiple of FEW_STEP.
+template <typename T, int NT, bool ALIGNED>
+__global__ void __launch_bounds__(32 * FEW_WARPS) dense_few_rows_kernel(const T* __restrict__ x, long long ldx,
+                                                                        const T* __restrict__ w, long long ldw, int k_part,
+                                                                        int parts, const DenseParams p) {
+  constexpr int OUTS = 8 * NT * FEW_COLS;
+  __shared__ float red[FEW_WARPS][8 * NT][FEW_COLS + 1];
+  __shared__ float sum[OUTS];
+  chain_begin();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int rank = parts > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int col0 = blockIdx.x / parts * FEW_COLS;
+  const int k0 = rank * k_part, k1 = min(p.K, k0 + k_part);
+  float acc[NT][4];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+  // (columns and rows that do not exist repeat the last one)
+  const T* w0 = w + min(col0 + g, p.N - 1) * ldw + 8 * t;
+  const T* w1 = w + min(col0 + g + 8, p.N - 1) * ldw + 8 * t;
+  const T* xr[NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) xr[i] = x + min(8 * i + g, p.M - 1) * ldx + 8 * t;
+#pragma unroll(NT <= 2 ? 4 : 2)
+  for (int k = k0 + warp * 32; k < k1; k += FEW_STEP) {
+    const int n = p.K - k - 8 * t;
+    const uint4 a = load8<ALIGNED>(w0 + k, n), b = load8<ALIGNED>(w1 + k, n);
+    uint4 v[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) v[i] = load8<ALIGNED>(xr[i] + k, n);
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      mma_16816<T>(acc[i], a.x, b.x, a.y, b.y, v[i].x, v[i].y);
+      mma_16816<T>(acc[i], a.z, b.z, a.w, b.w, v[i].z, v[i].w);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    red[warp][8 * i + 2 * t][g] = acc[i][0];
+    red[warp][8 * i + 2 * t + 1][g] = acc[i][1];
+    red[warp][8 * i + 2 * t][g + 8] = acc[i][2];
+    red[warp][8 * i + 2 * t + 1][g + 8] = acc[i][3];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < OUTS; i += 32 * FEW_WARPS) {
+    const int row = i / FEW_COLS, c = i % FEW_COLS;
+    float z = 0.f;
+#pragma unroll
+    for (int k = 0; k < FEW_WARPS; ++k) z += red[k][row][c];
+    if (parts == 1) dense_one<T>(p, row, col0 + c, z);
+    else sum[i] = z;
+  }
+  if (parts == 1) return;
+  cluster_sync_all();
+  // every block of the cluster finishes its share of the outputs
+  for (int i = rank * 32 * FEW_WARPS + threadIdx.x; i < OUTS; i += parts * 32 * FEW_WARPS) {
+    float z = 0.f;
+    for (int k = 0; k < parts; ++k) {
+      float v;
+      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_cta(smem_u32(&sum[i]), k)) : "memory");
+      z += v;
+    }
+    dense_one<T>(p, i / FEW_COLS, col0 + i % FEW_COLS, z);
+  }
+  cluster_sync_all();       // a block's sums are read until here
 }
 
 // ---------------------------------------------------------------- dz = dy act'(z), and its column sums
@@ -115,95 +245,87 @@ struct SlopeParams {
   int M, N, act, lanes, rows_per_block;   // lanes: threads along a row, a power of two
 };
 
-template <typename T, int VEC>
-__device__ __forceinline__ void slope_load(const T* p, float (&v)[VEC]) {
-  if constexpr (VEC == 8) {
-    const uint4 w = __ldg(reinterpret_cast<const uint4*>(p));
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+template <typename T>
+__device__ __forceinline__ void slope_unpack(const uint4& w, float (&v)[8]) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[2 * i] = Pair16<T>::lo(u[i]);
-      v[2 * i + 1] = Pair16<T>::hi(u[i]);
-    }
-  } else {
-    v[0] = to_f32<T>(__ldg(p));
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = Pair16<T>::lo(u[i]);
+    v[2 * i + 1] = Pair16<T>::hi(u[i]);
   }
 }
 
-template <typename T, int VEC, int ACT>
-__device__ __forceinline__ void slope_rows(const SlopeParams& p, int col, int r0, int step, int r1, float (&sum)[VEC]) {
-  constexpr int U = 4;
+template <typename T, bool ALIGNED, int ACT>
+__device__ __forceinline__ void slope_rows(const SlopeParams& p, int col, int r0, int step, int r1, float (&sum)[8]) {
+  constexpr int U = ALIGNED ? 4 : 2;      // rows in flight; of an unaligned one two pieces
   const T* dy = static_cast<const T*>(p.dy) + col;
   const T* z = static_cast<const T*>(p.z) + (ACT == ACT_NONE ? 0 : col);
   T* dz = static_cast<T*>(p.dz);
   for (int r = r0; r < r1; r += step * U) {
-    float g[U][VEC], s[U][VEC];
+    uint4 g4[U], s4[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const long long row = min(r + u * step, r1 - 1);
-      slope_load<T, VEC>(dy + row * p.ldy, g[u]);
-      if constexpr (ACT != ACT_NONE) slope_load<T, VEC>(z + row * p.ldz, s[u]);
+      g4[u] = load8<ALIGNED>(dy + row * p.ldy, p.N - col);
+      if constexpr (ACT != ACT_NONE) s4[u] = load8<ALIGNED>(z + row * p.ldz, p.N - col);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (r + u * step >= r1) break;
+      float g[8], s[8];
+      slope_unpack<T>(g4[u], g);
+      if constexpr (ACT != ACT_NONE) slope_unpack<T>(s4[u], s);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
+      for (int i = 0; i < 8; ++i) {
         // (not contracted into the sum: db has the same bits whether dz is stored or not)
-        if constexpr (ACT != ACT_NONE) g[u][i] = __fmul_rn(g[u][i], dense_slope<ACT>(s[u][i]));
-        sum[i] += g[u][i];
+        if constexpr (ACT != ACT_NONE) g[i] = __fmul_rn(g[i], dense_slope<ACT>(s[i]));
+        sum[i] += g[i];
       }
-      if (dz != nullptr) {
-        T* to = dz + static_cast<long long>(r + u * step) * p.lddz + col;
-        if constexpr (VEC == 8) {
-          *reinterpret_cast<uint4*>(to) =
-              make_uint4(Pair16<T>::pack(g[u][0], g[u][1]), Pair16<T>::pack(g[u][2], g[u][3]),
-                         Pair16<T>::pack(g[u][4], g[u][5]), Pair16<T>::pack(g[u][6], g[u][7]));
-        } else {
-          *to = from_f32<T>(g[u][0]);
-        }
-      }
+      if (dz != nullptr)      // (rows of whole 16-byte pieces; zeros behind column N)
+        *reinterpret_cast<uint4*>(dz + static_cast<long long>(r + u * step) * p.lddz + col) =
+            make_uint4(Pair16<T>::pack(g[0], g[1]), Pair16<T>::pack(g[2], g[3]), Pair16<T>::pack(g[4], g[5]),
+                       Pair16<T>::pack(g[6], g[7]));
     }
   }
 }
 
-template <typename T, int VEC>
+template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(256) dense_slope_kernel(const SlopeParams p) {
-  __shared__ float red[256][VEC + (VEC > 1 ? 1 : 0)];
+  __shared__ float red[256][9];
   chain_begin();
   const int lane = threadIdx.x & (p.lanes - 1), rr = threadIdx.x / p.lanes, step = 256 / p.lanes;
-  const int col = (blockIdx.x * p.lanes + lane) * VEC;
+  const int col = (blockIdx.x * p.lanes + lane) * 8;
   const long long b0 = static_cast<long long>(blockIdx.y) * p.rows_per_block;
   const int r1 = static_cast<int>(b0 + p.rows_per_block < p.M ? b0 + p.rows_per_block : p.M);
-  float sum[VEC];
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) sum[i] = 0.f;
+  float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   const bool live = col < p.N;
   if (live) {
     const int r0 = static_cast<int>(b0) + rr;
     switch (p.act) {
-      case ACT_GELU: slope_rows<T, VEC, ACT_GELU>(p, col, r0, step, r1, sum); break;
-      case ACT_GELU_TANH: slope_rows<T, VEC, ACT_GELU_TANH>(p, col, r0, step, r1, sum); break;
-      case ACT_SILU: slope_rows<T, VEC, ACT_SILU>(p, col, r0, step, r1, sum); break;
-      case ACT_RELU: slope_rows<T, VEC, ACT_RELU>(p, col, r0, step, r1, sum); break;
-      default: slope_rows<T, VEC, ACT_NONE>(p, col, r0, step, r1, sum); break;
+      case ACT_GELU: slope_rows<T, ALIGNED, ACT_GELU>(p, col, r0, step, r1, sum); break;
+      case ACT_GELU_TANH: slope_rows<T, ALIGNED, ACT_GELU_TANH>(p, col, r0, step, r1, sum); break;
+      case ACT_SILU: slope_rows<T, ALIGNED, ACT_SILU>(p, col, r0, step, r1, sum); break;
+      case ACT_RELU: slope_rows<T, ALIGNED, ACT_RELU>(p, col, r0, step, r1, sum); break;
+      default: slope_rows<T, ALIGNED, ACT_NONE>(p, col, r0, step, r1, sum); break;
     }
   }
   if (p.sums == nullptr) return;
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) red[threadIdx.x][i] = sum[i];
+  for (int i = 0; i < 8; ++i) red[threadIdx.x][i] = sum[i];
   __syncthreads();
   if (rr == 0 && live) {
     for (int k = 1; k < step; ++k)
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) sum[i] += red[k * p.lanes + lane][i];
+      for (int i = 0; i < 8; ++i) sum[i] += red[k * p.lanes + lane][i];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) p.sums[static_cast<long long>(blockIdx.y) * p.N + col + i] = sum[i];
+    for (int i = 0; i < 8; ++i)
+      if (col + i < p.N) p.sums[static_cast<long long>(blockIdx.y) * p.N + col + i] = sum[i];
   }
 }
 
 // ---------------------------------------------------------------- rows with whole 16-byte pieces
-// Copies up to two matrices into rows whose stride is a multiple of 8 (what TMA reads). blockIdx.y: the matrix.
+// Copies up to two matrices into rows whose stride is a multiple of 8 (what TMA reads), with zeros behind their columns. A
+// warp takes four rows at a time, a lane 16 bytes of each. blockIdx.y: the matrix.
 struct AlignRows {
   const uint16_t* src[2];
   uint16_t* dst[2];
@@ -212,20 +334,21 @@ struct AlignRows {
 };
 __global__ void __launch_bounds__(256) dense_align_rows_kernel(const AlignRows a) {
   chain_begin();
-  const int j = blockIdx.y;
+  constexpr int U = 4;
+  const int j = blockIdx.y, lane = threadIdx.x & 31;
   const uint16_t* __restrict__ src = a.src[j];
   uint16_t* __restrict__ dst = a.dst[j];
-  const int cols = a.cols[j], nvec = static_cast<int>(a.ldd[j] >> 3);
-  const long long n = a.rows[j] * nvec, step = static_cast<long long>(gridDim.x) * blockDim.x;
-  for (long long t = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; t < n; t += step) {
-    const long long row = t / nvec;
-    const int c0 = static_cast<int>(t - row * nvec) * 8;
-    const uint16_t* s = src + row * a.lds[j] + c0;
-    uint32_t v[8];
+  const int cols = a.cols[j];
+  const long long rows = a.rows[j], step = static_cast<long long>(gridDim.x) * 8 * U;
+  for (long long r0 = (static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5)) * U; r0 < rows; r0 += step) {
+    for (int c = lane * 8; c < cols; c += 256) {
+      uint4 v[U];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c0 + i < cols ? __ldg(s + i) : 0u;
-    *reinterpret_cast<uint4*>(dst + row * a.ldd[j] + c0) =
-        make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+      for (int u = 0; u < U; ++u) v[u] = load8<false>(src + (r0 + u < rows ? r0 + u : r0) * a.lds[j] + c, cols - c);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (r0 + u < rows) *reinterpret_cast<uint4*>(dst + (r0 + u) * a.ldd[j] + c) = v[u];
+    }
   }
 }
 

@@ -12,8 +12,8 @@
 //   epilogue  DENSE_Y: bias, activation, residual, one rounding; DENSE_Y_KEEP: z = x W^T + b besides;
 //             DENSE_PART: fp32 partial sums of a split contraction (DensePlan), which dense_finish_kernel adds up
 //             with the same epilogue.
-//   widths    Rows of y, z and r that are no whole 16-byte pieces (N not a multiple of 8) go past TMA: each lane stores
-//             its pairs.
+//   widths    Rows of y, z and r that are no whole 16-byte pieces (N not a multiple of 8) go past TMA: the warps copy
+//             between their staging boxes and memory.
 #pragma once
 #include "dense_common.cuh"
 #include "gemm_tcgen05.cuh"
@@ -34,7 +34,7 @@ struct DenseParams {
   const float* bias;            // [N] or nullptr
   int act;
   int fp16;
-  bool direct;                  // out, keep and aux are read and written by the lanes, not by TMA
+  bool direct_out, direct_aux;  // out and keep are written, aux is read, by the warps and not by TMA
   float* part;                  // DENSE_PART: slabs of TILE_M x BN
   DensePlan plan;
 };
@@ -63,8 +63,7 @@ __device__ __forceinline__ uint64_t dense_smem_desc(uint32_t addr, bool mn_major
   return mn_major ? (d & ~(0x3FFFull << 16)) | (static_cast<uint64_t>(8192 >> 4) << 16) : d;
 }
 
-// One pair of values at p (two columns, the second one only if it exists).
-template <typename T>
+// Pairs of values (two columns, the second one only if it exists) of rows with any alignment.
 __device__ __forceinline__ void dense_store_pair(void* base, long long at, uint32_t w, bool two) {
   uint16_t* p = static_cast<uint16_t*>(base) + at;
   if (two && (reinterpret_cast<uintptr_t>(p) & 3u) == 0) {
@@ -79,6 +78,34 @@ __device__ __forceinline__ uint32_t dense_load_pair(const void* base, long long 
   if (two && (reinterpret_cast<uintptr_t>(p) & 3u) == 0) return __ldg(reinterpret_cast<const uint32_t*>(p));
   const uint32_t lo = __ldg(p);
   return two ? lo | (static_cast<uint32_t>(__ldg(p + 1)) << 16) : lo;
+}
+// A warp's copy between a 32 x 32 staging box (64-byte rows and swizzle) and rows of a matrix that TMA does not take: two
+// rows at a time, 16 lanes with neighbouring pairs each.
+template <bool STORE>
+__device__ __forceinline__ void dense_copy_box(uint32_t box, void* base, long long ld, int m0, int n0, int M, int N) {
+  const int lane = threadIdx.x & 31, j = lane & 15, col = n0 + 2 * j;
+  auto at = [&](int r) {
+    return box + r * 64u + ((static_cast<uint32_t>(j >> 2) ^ static_cast<uint32_t>((r >> 1) & 3)) << 4) + (j & 3) * 4;
+  };
+  uint32_t w[16];           // (all of one side's accesses, then all of the other's)
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int r = 2 * i + (lane >> 4), row = m0 + r;
+    if constexpr (STORE) {
+      asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[i]) : "r"(at(r)) : "memory");
+    } else {
+      w[i] = row < M && col < N ? dense_load_pair(base, static_cast<long long>(row) * ld + col, col + 1 < N) : 0u;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int r = 2 * i + (lane >> 4), row = m0 + r;
+    if constexpr (STORE) {
+      if (row < M && col < N) dense_store_pair(base, static_cast<long long>(row) * ld + col, w[i], col + 1 < N);
+    } else {
+      asm volatile("st.shared.b32 [%0], %1;" ::"r"(at(r)), "r"(w[i]) : "memory");
+    }
+  }
 }
 
 // Biases of this lane's column pairs in the 32 columns from n0 (zero behind column N).
@@ -109,7 +136,7 @@ dense_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
   constexpr bool A_MN = LAY == DENSE_TN, B_MN = LAY != DENSE_NT, PART = EPI == DENSE_PART, KEEP = EPI == DENSE_Y_KEEP;
   constexpr int TILE_M = PAIR ? 2 * GEMM_BM : GEMM_BM;
   constexpr bool ANY = ACT == ACT_ANY;
-  const bool has_aux = ANY ? p.aux != nullptr : AUX, direct = ANY && p.direct;
+  const bool has_aux = ANY ? p.aux != nullptr : AUX, direct = ANY && p.direct_out, direct_aux = ANY && p.direct_aux;
   constexpr int BOX = 8192;                                // an MN-major box: 64 contraction rows of 128 bytes
   const uint32_t pair_rank = PAIR ? cluster_ctarank() : 0u;
   const int unit = PAIR ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
@@ -290,7 +317,7 @@ dense_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
       const uint32_t r = ((lane >> 3) & 1) * 8 + (lane & 7), piece = 4 * c + 2 * q + (lane >> 4);
       return b + (16 * hf + r) * (BC * 2u) + ((BC == 64 ? piece ^ (r & 7) : piece ^ ((r >> 1) & 3)) << 4);
     };
-    const bool fetch = !PART && has_aux && !direct;
+    const bool fetch = !PART && has_aux && !direct_aux;
     [[maybe_unused]] uint32_t aux_phase = 0;
     // first row and column of this warp's part of a tile; whether there is anything of it
     auto part_of = [&](int tile, int& m, int& n) -> bool {
@@ -333,6 +360,14 @@ dense_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
       for (int c0 = 0; c0 < WARP_COLS; c0 += BC) {              // a box
         const bool box_live = live && n_warp0 + c0 < p.N;
         if (!AHEAD && fetch && box_live) fetch_aux(m_warp, n_warp0 + c0);
+        if (!PART && has_aux && direct_aux && box_live) {
+          if (!direct) {                     // the box's last store has been read
+            if (elect_one()) tma_store_wait_read0();
+            __syncwarp();
+          }
+          dense_copy_box<false>(box, const_cast<void*>(p.aux), p.ldaux, m_warp, n_warp0 + c0, p.M, p.N);
+          __syncwarp();
+        }
         if (!acc_ready) {
           if (!gemm_wait(accf_bar(buf), (it >> 1) & 1u, abort_flag, ST_TIMEOUT_EPILOGUE)) {
             ok = false;
@@ -385,8 +420,7 @@ dense_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
               uint64_t v[8];
 #pragma unroll
               for (int i = 0; i < 8; ++i) v[i] = fadd2(pack2u(acc[hf][2 * i], acc[hf][2 * i + 1]), bias[i >> 1]);
-              const int row0 = m_warp + 16 * hf + (lane >> 2), col0 = n0 + 2 * (lane & 3);
-              auto put = [&](uint32_t b, void* to, long long ld, bool wait) {
+              auto put = [&](uint32_t b, bool wait) {
                 uint32_t w[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
@@ -394,38 +428,19 @@ dense_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
                   unpack2(v[i], lo, hi);
                   w[i] = P16::pack(lo, hi);
                 }
-                if (!direct) {
-                  if (wait) {      // as late as possible: the box's last store drains meanwhile
-                    if (elect_one()) tma_store_wait_read0();
-                    __syncwarp();
-                  }
-#pragma unroll
-                  for (int q = 0; q < 2; ++q) stmatrix_x4(box_addr(b, hf, c, q), &w[4 * q]);
-                } else {
-#pragma unroll
-                  for (int i = 0; i < 8; ++i) {
-                    const int row = row0 + 8 * (i & 1), col = col0 + 8 * (i >> 1);
-                    if (row < p.M && col < p.N)
-                      dense_store_pair<T>(to, static_cast<long long>(row) * ld + col, w[i], col + 1 < p.N);
-                  }
+                if (wait && !direct) {      // as late as possible: the box's last store drains meanwhile
+                  if (elect_one()) tma_store_wait_read0();
+                  __syncwarp();
                 }
+#pragma unroll
+                for (int q = 0; q < 2; ++q) stmatrix_x4(box_addr(b, hf, c, q), &w[4 * q]);
               };
-              if constexpr (KEEP) put(zbox, p.keep, p.ldk, c == 0 && hf == 0 && !fetch);
+              if constexpr (KEEP) put(zbox, c == 0 && hf == 0 && !has_aux);
               if constexpr (LAY == DENSE_NT) {
                 uint32_t aux[8];
                 if (has_aux) {
-                  if (!direct) {
 #pragma unroll
-                    for (int q = 0; q < 2; ++q) ldmatrix_x4(box_addr(box, hf, c, q), &aux[4 * q]);
-                  } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                      const int row = row0 + 8 * (i & 1), col = col0 + 8 * (i >> 1);
-                      aux[i] = row < p.M && col < p.N
-                                   ? dense_load_pair(p.aux, static_cast<long long>(row) * p.ldaux + col, col + 1 < p.N)
-                                   : 0u;
-                    }
-                  }
+                  for (int q = 0; q < 2; ++q) ldmatrix_x4(box_addr(box, hf, c, q), &aux[4 * q]);
                 }
                 if constexpr (ANY) dense_act<T>(p.act, v); else dense_act_all<T, ACT>(v);
                 if (has_aux) {
@@ -433,9 +448,15 @@ dense_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
                   for (int i = 0; i < 8; ++i) v[i] = fadd2(v[i], pack2(P16::lo(aux[i]), P16::hi(aux[i])));
                 }
               }
-              put(box, p.out, p.ldo, !KEEP && c == 0 && hf == 0 && !fetch);
+              put(box, !KEEP && c == 0 && hf == 0 && !has_aux);
             }
           }
+        }
+        if (!PART && direct && box_live) {
+          __syncwarp();
+          if constexpr (KEEP) dense_copy_box<true>(zbox, p.keep, p.ldk, m_warp, n_warp0 + c0, p.M, p.N);
+          dense_copy_box<true>(box, p.out, p.ldo, m_warp, n_warp0 + c0, p.M, p.N);
+          __syncwarp();
         }
         if (!PART && !direct && box_live) {
           fence_proxy_async_smem();
@@ -551,7 +572,7 @@ __global__ void __launch_bounds__(FINISH_THREADS) dense_finish_kernel(const Dens
     for (int k = 0; k < 2; ++k) {
       float lo, hi;
       unpack2(v[k], lo, hi);
-      if (col + 2 * k < p.N) dense_store_pair<T>(base, at + 2 * k, Pair16<T>::pack(lo, hi), col + 2 * k + 1 < p.N);
+      if (col + 2 * k < p.N) dense_store_pair(base, at + 2 * k, Pair16<T>::pack(lo, hi), col + 2 * k + 1 < p.N);
     }
   };
   if (p.keep != nullptr) put(p.keep, p.ldk);

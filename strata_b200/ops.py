@@ -175,11 +175,22 @@ def _scratch(need: int, x):
     return x.new_empty(need, dtype=torch.uint8) if need else None
 
 
+def _padded_rows(x, shape):
+    """(tensor of this shape and x's type, row stride): rows of whole 16-byte pieces, so that kernels can store them and read
+    them again without a copy; a view of wider rows where the width is no multiple of eight."""
+    n = shape[-1]
+    if n % 8 == 0:
+        return x.new_empty(shape), n
+    wide = (n + 7) // 8 * 8
+    return x.new_empty(shape[:-1] + (wide,))[..., :n], wide
+
+
 def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, activation: str = "none",
                residual: torch.Tensor | None = None, *, save_preact: bool = False, out: torch.Tensor | None = None):
     """y = residual + act(z), z = x @ weight.T + bias, in one pass: x [..., K], weight [N, K], residual and y [..., N] of
     one type (bfloat16 or float16), bias [N] fp32; activation one of "none", "gelu" (erf), "gelu_tanh", "silu", "relu".
-    Any number of rows, any widths and row strides. Sums and the epilogue are fp32, y is rounded once.
+    Any number of rows, any widths and row strides. Sums and the epilogue are fp32, y is rounded once. Where N is no
+    multiple of eight the results are views of rows that are (not contiguous): the next call reads them without a copy.
 
     save_preact: returns (y, z); linear_act_backward needs z for any activation but "none". out: where y goes, [M, N]
     with unit inner stride; it may be the residual, no other operand. The gradients are linear_act_backward's;
@@ -201,24 +212,24 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
             raise ValueError(f"residual must be {tuple(shape)}, got {tuple(residual.shape)}")
         r2, _, ldr = _packed_rows(residual, N, "residual")
     if out is None:
-        y, ldy = x.new_empty(shape), N
+        y, ldy = _padded_rows(x, shape)
     else:
         _like(out, "out", x)
         if out.shape != (M, N) or (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
             raise ValueError(f"out must be [{M}, {N}] with unit inner stride")
         y, ldy = out, out.stride(0) if M > 1 else N
-    z = x.new_empty(shape) if save_preact else None
+    z, ldz = _padded_rows(x, shape) if save_preact else (None, 0)
     if M:
         lib = _lib.load()
         with _lib.on_device(x):
             xp, wp = x2.data_ptr(), w2.data_ptr()
             need, ws = 0, None
-            if M > 8:       # (fewer rows take no workspace)
+            if M > 8:       # (so few rows take no workspace)
                 need = lib.strata_linear_act_workspace_bytes(M, N, K, not (xp & 15 or ldx & 7), not (wp & 15 or ldw & 7))
                 ws = _scratch(need, x)
             code = lib.strata_linear_act(
                 xp, ldx, wp, ldw, None if bias is None else bias.data_ptr(), None if r2 is None else r2.data_ptr(), ldr,
-                y.data_ptr(), ldy, None if z is None else z.data_ptr(), N, M, N, K, act, dtype,
+                y.data_ptr(), ldy, None if z is None else z.data_ptr(), ldz, M, N, K, act, dtype, out is None,
                 None if ws is None else ws.data_ptr(), need, _stream_ptr(x))
             if code:
                 _lib.check(code, "strata_linear_act")
@@ -255,7 +266,7 @@ def linear_act_backward(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tenso
             raise ValueError(f"preact must be {tuple(shape)}, got {tuple(preact.shape)}")
         z2, _, ldz = _packed_rows(preact, N, "preact")
         zp = z2.data_ptr()
-    dx = x.new_empty(x.shape) if need_x else None
+    dx, lddx = _padded_rows(x, x.shape) if need_x else (None, 0)
     dw = x.new_empty((N, K)) if need_weight else None
     db = x.new_empty(N, dtype=torch.float32) if need_bias else None
     if need_x or need_weight or need_bias:
@@ -267,8 +278,8 @@ def linear_act_backward(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tenso
                 not (xp & 15 or ldx & 7), not (wp & 15 or ldw & 7), need_x, need_weight, need_bias)
             ws = _scratch(need, x)
             code = lib.strata_linear_act_backward(
-                gp, ldg, xp, ldx, wp, ldw, zp, ldz, None if dx is None else dx.data_ptr(), K,
-                None if dw is None else dw.data_ptr(), K, None if db is None else db.data_ptr(), M, N, K, act, dtype,
+                gp, ldg, xp, ldx, wp, ldw, zp, ldz, None if dx is None else dx.data_ptr(), lddx,
+                None if dw is None else dw.data_ptr(), K, None if db is None else db.data_ptr(), M, N, K, act, dtype, True,
                 None if ws is None else ws.data_ptr(), need, _stream_ptr(x))
             if code:
                 _lib.check(code, "strata_linear_act_backward")

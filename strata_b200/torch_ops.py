@@ -169,10 +169,17 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     return ops.linear_act(x, weight, bias, activation, residual), x.new_empty(0)
 
 
+def _padded(x, width):
+    """Rows as ops.linear_act lays them out: a view of whole 16-byte pieces."""
+    if width % 8 == 0:
+        return x.new_empty((*x.shape[:-1], width))
+    return x.new_empty((*x.shape[:-1], (width + 7) // 8 * 8))[..., :width]
+
+
 @linear_act.register_fake
 def _linear_act_fake(x, weight, bias=None, activation="none", residual=None, save_preact=False):
-    y = x.new_empty((*x.shape[:-1], weight.shape[0]))
-    return y, torch.empty_like(y) if save_preact else x.new_empty(0)
+    new = lambda: _padded(x, weight.shape[0])
+    return new(), new() if save_preact else x.new_empty(0)
 
 
 @torch.library.custom_op("strata_b200::linear_act_backward", mutates_args=())
@@ -188,7 +195,7 @@ def linear_act_backward(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tenso
 
 @linear_act_backward.register_fake
 def _linear_act_backward_fake(grad, x, weight, activation, preact, need_x, need_weight, need_bias):
-    return (x.new_empty(x.shape if need_x else 0), weight.new_empty(weight.shape if need_weight else 0),
+    return (_padded(x, x.shape[-1]) if need_x else x.new_empty(0), weight.new_empty(weight.shape if need_weight else 0),
             weight.new_empty(weight.shape[0] if need_bias else 0, dtype=torch.float32 if need_bias else x.dtype))
 
 

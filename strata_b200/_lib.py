@@ -60,7 +60,7 @@ _SIGNATURES = {
     "strata_linear_bf16": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
                                    c_int64, c_int, c_int, c_int, c_int, c_void_p, c_int64,
                                    c_void_p]),
-    "strata_linear_act_workspace_bytes": (c_int64, [c_int] * 5),
+    "strata_linear_act_workspace_bytes": (c_int64, [c_int] * 6),
     "strata_linear_act": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64,
                                   c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int64,
                                   c_void_p]),

@@ -146,11 +146,11 @@ static bool dense_rows_ok(const void* p, int64_t ld, int cols) {
   return p != nullptr && ld >= cols && (reinterpret_cast<uintptr_t>(p) & 1u) == 0;
 }
 
-int64_t strata_linear_act_workspace_bytes(int M, int N, int K, int x_aligned, int w_aligned) {
+int64_t strata_linear_act_workspace_bytes(int M, int N, int K, int x_aligned, int w_aligned, int residual_aligned) {
   const int sms = current_sm_count();
   if (sms <= 0) return STRATA_ERR_NO_DEVICE;
   if (!dense_sizes(M, N, K, 0, 0)) return STRATA_ERR_ARG;
-  return dense_forward_bytes(M, N, K, x_aligned != 0, w_aligned != 0, sms);
+  return dense_forward_bytes(M, N, K, x_aligned != 0, w_aligned != 0, residual_aligned != 0, sms);
 }
 
 int strata_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const float* bias, const void* residual,
@@ -164,7 +164,8 @@ int strata_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, co
       (residual && !dense_rows_ok(residual, ldr, N)) || (preact && !dense_rows_ok(preact, ldz, N)) ||
       (reinterpret_cast<uintptr_t>(bias) & 3u) != 0)
     return STRATA_ERR_ARG;
-  const int64_t need = dense_forward_bytes(M, N, K, dense_aligned(x, ldx), dense_aligned(w, ldw), sms);
+  const int64_t need = dense_forward_bytes(M, N, K, dense_aligned(x, ldx), dense_aligned(w, ldw),
+                                           !residual || dense_aligned(residual, ldr), sms);
   if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0))
     return STRATA_ERR_ARG;
   DenseParams p{};
@@ -176,7 +177,6 @@ int strata_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, co
   p.act = activation;
   p.fp16 = dtype == STRATA_F16;
   p.direct_out = !dense_whole(y, ldy, N, padded != 0) || (preact && !dense_whole(preact, ldz, N, padded != 0));
-  p.direct_aux = residual && !dense_aligned(residual, ldr);
   return launch_dense_forward({x, ldx}, {w, ldw}, p, workspace, sms, as_stream(stream));
 }
 

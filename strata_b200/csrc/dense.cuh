@@ -102,7 +102,7 @@ inline int launch_dense_t(const DenseOperand& A, const DenseOperand& B, const De
   tmOut = tmKeep = tmAux = tmA;
   using S = DenseSmem<BN, PAIR, EPI, AUX && EPI == DENSE_Y>;
   constexpr TmapSwizzle sw = S::BOX_COLS == 64 ? TMAP_SWIZZLE_128B : TMAP_SWIZZLE_64B;
-  if (EPI != DENSE_PART && p.aux && !p.direct_aux &&
+  if (EPI != DENSE_PART && p.aux &&
       map(&tmAux, {p.aux, p.ldaux}, p.M, p.N, S::BOX_COLS, 32, sw) != 0)
     return -23;
   if (EPI != DENSE_PART && !p.direct_out) {
@@ -139,7 +139,7 @@ template <int LAY, int EPI, typename T>
 inline int launch_dense_bn(int bn, const DenseOperand& A, const DenseOperand& B, const DenseParams& p, int units,
                            cudaStream_t st) {
   if constexpr (LAY == DENSE_NT && EPI != DENSE_PART) {
-    if (bn == 256 && !p.direct_out && !p.direct_aux)
+    if (bn == 256 && !p.direct_out)
       return p.aux ? launch_dense_pair<EPI, T, true>(A, B, p, units, st)
                    : launch_dense_pair<EPI, T, false>(A, B, p, units, st);
   }
@@ -259,47 +259,55 @@ struct DenseArena {
   }
 };
 
-inline int launch_align_rows(const AlignRows& a, int n, int sms, cudaStream_t st) {
+// Adds a copy of o to a and makes o the copy.
+inline void align_add(AlignRows& a, DenseOperand& o, void* to, long long rows, int cols) {
+  const long long ld = dense_round8(cols);
+  const int n = a.n++;
+  a.src[n] = static_cast<const uint16_t*>(o.p); a.lds[n] = o.ld;
+  a.dst[n] = static_cast<uint16_t*>(to); a.ldd[n] = ld;
+  a.rows[n] = rows; a.cols[n] = cols;
+  o = {to, ld};
+}
+inline int align_blocks(const AlignRows& a, int sms) {       // of one matrix
   long long most = 0;
-  for (int j = 0; j < n; ++j) most = a.rows[j] > most ? a.rows[j] : most;
-  long long blocks = (most + 31) / 32;
-  if (blocks > 8LL * sms) blocks = 8LL * sms;
-  return launch_chained(dense_align_rows_kernel, dim3(static_cast<unsigned>(blocks), n), 256, 0, st, 1, a);
+  for (int j = 0; j < a.n; ++j) {
+    const int per = align_block_rows(a.cols[j]);
+    const long long blocks = (a.rows[j] + per - 1) / per;
+    most = blocks > most ? blocks : most;
+  }
+  return static_cast<int>(most < 8LL * sms ? most : 8LL * sms);
 }
 
 // ---------------------------------------------------------------- forward
-// Workspace: aligned copies of x and w where they are not aligned themselves, then the slabs of a split. With base
-// nullptr nothing is launched and `used` says how much is needed.
-inline int64_t dense_forward_bytes(int M, int N, int K, bool x_ok, bool w_ok, int sms) {
+// Workspace: aligned copies of the operands that are not aligned themselves, then the slabs of a split.
+inline int64_t dense_forward_bytes(int M, int N, int K, bool x_ok, bool w_ok, bool r_ok, int sms) {
   if (dense_few(M, N, K)) return 0;
   DenseArena ws{nullptr, 0};
   if (!x_ok) ws.take(2 * dense_round8(K) * M);
   if (!w_ok) ws.take(2 * dense_round8(K) * N);
+  if (!r_ok) ws.take(2 * dense_round8(N) * M);
   ws.take(dense_choice(M, N, K, sms).slab_bytes());
   return ws.used;
 }
 
-inline int launch_dense_forward(DenseOperand x, DenseOperand w, const DenseParams& p, void* workspace, int sms,
+inline int launch_dense_forward(DenseOperand x, DenseOperand w, DenseParams p, void* workspace, int sms,
                                 cudaStream_t st) {
   const bool x_ok = dense_aligned(x.p, x.ld), w_ok = dense_aligned(w.p, w.ld);
-  if (dense_few(p.M, p.N, p.K)) {
-    return launch_few_rows(x, w, p, x_ok && w_ok && p.K % 8 == 0, sms, st);
-  }
+  if (dense_few(p.M, p.N, p.K)) return launch_few_rows(x, w, p, x_ok && w_ok && p.K % 8 == 0, sms, st);
   DenseArena ws{static_cast<uint8_t*>(workspace), 0};
   AlignRows a{};
-  int n = 0;
-  auto align = [&](DenseOperand& o, long long rows, int cols) {
-    const long long ld = dense_round8(cols);
-    void* to = ws.take(2 * ld * rows);
-    a.src[n] = static_cast<const uint16_t*>(o.p); a.lds[n] = o.ld;
-    a.dst[n] = static_cast<uint16_t*>(to); a.ldd[n] = ld;
-    a.rows[n] = rows; a.cols[n++] = cols;
-    o = {to, ld};
-  };
-  if (!x_ok) align(x, p.M, p.K);
-  if (!w_ok) align(w, p.N, p.K);
-  if (n > 0)
-    if (const int r = launch_align_rows(a, n, sms, st); r != 0) return r;
+  if (!x_ok) align_add(a, x, ws.take(2 * dense_round8(p.K) * p.M), p.M, p.K);
+  if (!w_ok) align_add(a, w, ws.take(2 * dense_round8(p.K) * p.N), p.N, p.K);
+  if (p.aux && !dense_aligned(p.aux, p.ldaux)) {
+    DenseOperand r{p.aux, p.ldaux};
+    align_add(a, r, ws.take(2 * dense_round8(p.N) * p.M), p.M, p.N);
+    p.aux = r.p;
+    p.ldaux = r.ld;
+  }
+  if (a.n > 0) {
+    const dim3 grid(static_cast<unsigned>(align_blocks(a, sms)), static_cast<unsigned>(a.n));
+    if (const int r = launch_chained(dense_align_rows_kernel, grid, 256, 0, st, 1, a); r != 0) return r;
+  }
   const DenseChoice c = dense_choice(p.M, p.N, p.K, sms);
   return launch_dense<DENSE_NT>(x, w, p, c, ws.take(c.slab_bytes()), nullptr, st);
 }
@@ -366,29 +374,21 @@ inline DenseGradPlan dense_grad_plan(int M, int N, int K, bool act, bool dy_ok, 
 inline int launch_dense_backward(const DenseGradParams& q, const DenseGradPlan& g, int sms, cudaStream_t st) {
   DenseOperand x = q.x, w = q.w, dz = q.dy;
   int r;
-  if (g.copy_x || g.copy_w) {
-    AlignRows a{};
-    int n = 0;
-    auto align = [&](DenseOperand& o, void* to, long long rows) {
-      const long long ld = dense_round8(q.K);
-      a.src[n] = static_cast<const uint16_t*>(o.p); a.lds[n] = o.ld;
-      a.dst[n] = static_cast<uint16_t*>(to); a.ldd[n] = ld;
-      a.rows[n] = rows; a.cols[n++] = q.K;
-      o = {to, ld};
-    };
-    if (g.copy_x) align(x, g.xs, q.M);
-    if (g.copy_w) align(w, g.ws, q.N);
-    if ((r = launch_align_rows(a, n, sms, st)) != 0) return r;
-  }
-  if (g.make_dz || q.db) {
+  AlignRows a{};
+  if (g.copy_x) align_add(a, x, g.xs, q.M, q.K);
+  if (g.copy_w) align_add(a, w, g.ws, q.N, q.K);
+  if (g.make_dz || q.db || a.n > 0) {
     SlopeParams s{};
     s.dy = q.dy.p; s.ldy = q.dy.ld;
     s.z = q.z.p; s.ldz = q.z.ld;
     s.dz = g.make_dz ? g.dz : nullptr; s.lddz = dense_round8(q.N);
     s.sums = g.col_sums;
     s.M = q.M; s.N = q.N; s.act = q.act; s.lanes = g.sums.lanes; s.rows_per_block = g.sums.rows_per_block;
-    const dim3 grid(static_cast<unsigned>(g.sums.cols), static_cast<unsigned>(g.sums.blocks));
-    auto go = [&](auto kern) { return launch_chained(kern, grid, 256, 0, st, 1, s); };
+    s.cols = g.sums.cols;
+    s.blocks = g.make_dz || q.db ? g.sums.cols * g.sums.blocks : 0;
+    s.align_blocks = align_blocks(a, sms);
+    const dim3 grid(static_cast<unsigned>(s.blocks + s.align_blocks * a.n));
+    auto go = [&](auto kern) { return launch_chained(kern, grid, 256, 0, st, 1, s, a); };
     if (q.fp16) r = g.aligned ? go(dense_slope_kernel<__half, true>) : go(dense_slope_kernel<__half, false>);
     else r = g.aligned ? go(dense_slope_kernel<__nv_bfloat16, true>) : go(dense_slope_kernel<__nv_bfloat16, false>);
     if (r != 0) return r;

@@ -233,6 +233,55 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) dense_few_rows_kernel(const T*
   cluster_sync_all();       // a block's sums are read until here
 }
 
+// ---------------------------------------------------------------- rows with whole 16-byte pieces
+// Copies up to three matrices into rows whose stride is a multiple of 8 (what TMA reads), with zeros behind their columns. A
+// block takes whole rows, about ALIGN_VECTORS 16-byte pieces of them; a thread walks every 256th piece, four in flight.
+struct AlignRows {
+  const uint16_t* src[3];
+  uint16_t* dst[3];
+  long long lds[3], ldd[3], rows[3];
+  int cols[3];
+  int n;
+};
+constexpr int ALIGN_VECTORS = 2048;
+__host__ __device__ inline int align_block_rows(int cols) {
+  const int n = ALIGN_VECTORS / ((cols + 7) / 8);
+  return n > 0 ? n : 1;
+}
+__device__ __forceinline__ void align_rows(const AlignRows& a, int j, int block, int blocks) {
+  constexpr int U = 4;
+  const int cols = a.cols[j], nvec = (cols + 7) / 8, per = align_block_rows(cols);
+  const int dr = 256 / nvec, dc = 256 - dr * nvec, r_first = threadIdx.x / nvec, c_first = threadIdx.x - r_first * nvec;
+  for (long long r0 = static_cast<long long>(block) * per; r0 < a.rows[j]; r0 += static_cast<long long>(blocks) * per) {
+    const int rows = static_cast<int>(a.rows[j] - r0 < per ? a.rows[j] - r0 : per);
+    const uint16_t* __restrict__ src = a.src[j] + r0 * a.lds[j];
+    uint16_t* __restrict__ dst = a.dst[j] + r0 * a.ldd[j];
+    int r = r_first, c = c_first;
+    while (r < rows) {
+      uint4 v[U];
+      long long to[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        to[u] = r < rows ? r * a.ldd[j] + c * 8 : -1;
+        if (r < rows) v[u] = load8<false>(src + r * a.lds[j] + c * 8, cols - c * 8);
+        r += dr;
+        c += dc;
+        if (c >= nvec) {
+          c -= nvec;
+          ++r;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (to[u] >= 0) *reinterpret_cast<uint4*>(dst + to[u]) = v[u];
+    }
+  }
+}
+__global__ void __launch_bounds__(256) dense_align_rows_kernel(const AlignRows a) {
+  chain_begin();
+  align_rows(a, blockIdx.y, blockIdx.x, gridDim.x);
+}
+
 // ---------------------------------------------------------------- dz = dy act'(z), and its column sums
 // HBM-bound: reads dy and z, writes dz (act = none: reads dy, and writes it only where the products need aligned
 // rows). A thread keeps its eight columns over all rows of the block, so the sums cost no extra read; the blocks' sums
@@ -241,8 +290,9 @@ struct SlopeParams {
   const void* dy;  long long ldy;
   const void* z;   long long ldz;       // nullptr: act is none
   void* dz;        long long lddz;      // nullptr: sums only
-  float* sums;                          // [gridDim.y, N] or nullptr
+  float* sums;                          // [blocks / cols, N] or nullptr
   int M, N, act, lanes, rows_per_block;   // lanes: threads along a row, a power of two
+  int cols, blocks, align_blocks;         // blocks along a row; of dz and the sums; of each matrix that is copied besides
 };
 
 template <typename T>
@@ -290,12 +340,18 @@ __device__ __forceinline__ void slope_rows(const SlopeParams& p, int col, int r0
 }
 
 template <typename T, bool ALIGNED>
-__global__ void __launch_bounds__(256) dense_slope_kernel(const SlopeParams p) {
+__global__ void __launch_bounds__(256) dense_slope_kernel(const SlopeParams p, const AlignRows a) {
   __shared__ float red[256][9];
   chain_begin();
+  if (static_cast<int>(blockIdx.x) >= p.blocks) {
+    const int b = blockIdx.x - p.blocks, j = b / p.align_blocks;
+    align_rows(a, j, b - j * p.align_blocks, p.align_blocks);
+    return;
+  }
+  const int block_y = blockIdx.x / p.cols, block_x = blockIdx.x - block_y * p.cols;
   const int lane = threadIdx.x & (p.lanes - 1), rr = threadIdx.x / p.lanes, step = 256 / p.lanes;
-  const int col = (blockIdx.x * p.lanes + lane) * 8;
-  const long long b0 = static_cast<long long>(blockIdx.y) * p.rows_per_block;
+  const int col = (block_x * p.lanes + lane) * 8;
+  const long long b0 = static_cast<long long>(block_y) * p.rows_per_block;
   const int r1 = static_cast<int>(b0 + p.rows_per_block < p.M ? b0 + p.rows_per_block : p.M);
   float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   const bool live = col < p.N;
@@ -319,36 +375,7 @@ __global__ void __launch_bounds__(256) dense_slope_kernel(const SlopeParams p) {
       for (int i = 0; i < 8; ++i) sum[i] += red[k * p.lanes + lane][i];
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (col + i < p.N) p.sums[static_cast<long long>(blockIdx.y) * p.N + col + i] = sum[i];
-  }
-}
-
-// ---------------------------------------------------------------- rows with whole 16-byte pieces
-// Copies up to two matrices into rows whose stride is a multiple of 8 (what TMA reads), with zeros behind their columns. A
-// warp takes four rows at a time, a lane 16 bytes of each. blockIdx.y: the matrix.
-struct AlignRows {
-  const uint16_t* src[2];
-  uint16_t* dst[2];
-  long long lds[2], ldd[2], rows[2];
-  int cols[2];
-};
-__global__ void __launch_bounds__(256) dense_align_rows_kernel(const AlignRows a) {
-  chain_begin();
-  constexpr int U = 4;
-  const int j = blockIdx.y, lane = threadIdx.x & 31;
-  const uint16_t* __restrict__ src = a.src[j];
-  uint16_t* __restrict__ dst = a.dst[j];
-  const int cols = a.cols[j];
-  const long long rows = a.rows[j], step = static_cast<long long>(gridDim.x) * 8 * U;
-  for (long long r0 = (static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5)) * U; r0 < rows; r0 += step) {
-    for (int c = lane * 8; c < cols; c += 256) {
-      uint4 v[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) v[u] = load8<false>(src + (r0 + u < rows ? r0 + u : r0) * a.lds[j] + c, cols - c);
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (r0 + u < rows) *reinterpret_cast<uint4*>(dst + (r0 + u) * a.ldd[j] + c) = v[u];
-    }
+      if (col + i < p.N) p.sums[static_cast<long long>(block_y) * p.N + col + i] = sum[i];
   }
 }
 

@@ -12,8 +12,8 @@
 //   epilogue  DENSE_Y: bias, activation, residual, one rounding; DENSE_Y_KEEP: z = x W^T + b besides;
 //             DENSE_PART: fp32 partial sums of a split contraction (DensePlan), which dense_finish_kernel adds up
 //             with the same epilogue.
-//   widths    Rows of y, z and r that are no whole 16-byte pieces (N not a multiple of 8) go past TMA: the warps copy
-//             between their staging boxes and memory.
+//   widths    Rows of y and z that TMA cannot store (it writes whole 16-byte pieces) are copied from the staging boxes by
+//             the warps.
 #pragma once
 #include "dense_common.cuh"
 #include "gemm_tcgen05.cuh"
@@ -34,7 +34,7 @@ struct DenseParams {
   const float* bias;            // [N] or nullptr
   int act;
   int fp16;
-  bool direct_out, direct_aux;  // out and keep are written, aux is read, by the warps and not by TMA
+  bool direct_out;              // out and keep are written by the warps, not by TMA
   float* part;                  // DENSE_PART: slabs of TILE_M x BN
   DensePlan plan;
 };
@@ -79,32 +79,22 @@ __device__ __forceinline__ uint32_t dense_load_pair(const void* base, long long 
   const uint32_t lo = __ldg(p);
   return two ? lo | (static_cast<uint32_t>(__ldg(p + 1)) << 16) : lo;
 }
-// A warp's copy between a 32 x 32 staging box (64-byte rows and swizzle) and rows of a matrix that TMA does not take: two
-// rows at a time, 16 lanes with neighbouring pairs each.
-template <bool STORE>
+// A warp's copy of a 32 x 32 staging box (64-byte rows and swizzle) to rows that TMA does not store: two rows at a time, 16
+// lanes with neighbouring pairs each.
 __device__ __forceinline__ void dense_copy_box(uint32_t box, void* base, long long ld, int m0, int n0, int M, int N) {
   const int lane = threadIdx.x & 31, j = lane & 15, col = n0 + 2 * j;
-  auto at = [&](int r) {
-    return box + r * 64u + ((static_cast<uint32_t>(j >> 2) ^ static_cast<uint32_t>((r >> 1) & 3)) << 4) + (j & 3) * 4;
-  };
-  uint32_t w[16];           // (all of one side's accesses, then all of the other's)
+  uint32_t w[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    const int r = 2 * i + (lane >> 4), row = m0 + r;
-    if constexpr (STORE) {
-      asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[i]) : "r"(at(r)) : "memory");
-    } else {
-      w[i] = row < M && col < N ? dense_load_pair(base, static_cast<long long>(row) * ld + col, col + 1 < N) : 0u;
-    }
+    const int r = 2 * i + (lane >> 4);
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[i])
+                 : "r"(box + r * 64u + ((static_cast<uint32_t>(j >> 2) ^ static_cast<uint32_t>((r >> 1) & 3)) << 4) + (j & 3) * 4)
+                 : "memory");
   }
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    const int r = 2 * i + (lane >> 4), row = m0 + r;
-    if constexpr (STORE) {
-      if (row < M && col < N) dense_store_pair(base, static_cast<long long>(row) * ld + col, w[i], col + 1 < N);
-    } else {
-      asm volatile("st.shared.b32 [%0], %1;" ::"r"(at(r)), "r"(w[i]) : "memory");
-    }
+    const int row = m0 + 2 * i + (lane >> 4);
+    if (row < M && col < N) dense_store_pair(base, static_cast<long long>(row) * ld + col, w[i], col + 1 < N);
   }
 }
 
@@ -136,7 +126,7 @@ dense_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
   constexpr bool A_MN = LAY == DENSE_TN, B_MN = LAY != DENSE_NT, PART = EPI == DENSE_PART, KEEP = EPI == DENSE_Y_KEEP;
   constexpr int TILE_M = PAIR ? 2 * GEMM_BM : GEMM_BM;
   constexpr bool ANY = ACT == ACT_ANY;
-  const bool has_aux = ANY ? p.aux != nullptr : AUX, direct = ANY && p.direct_out, direct_aux = ANY && p.direct_aux;
+  const bool has_aux = ANY ? p.aux != nullptr : AUX, direct = ANY && p.direct_out;
   constexpr int BOX = 8192;                                // an MN-major box: 64 contraction rows of 128 bytes
   const uint32_t pair_rank = PAIR ? cluster_ctarank() : 0u;
   const int unit = PAIR ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
@@ -317,7 +307,7 @@ dense_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
       const uint32_t r = ((lane >> 3) & 1) * 8 + (lane & 7), piece = 4 * c + 2 * q + (lane >> 4);
       return b + (16 * hf + r) * (BC * 2u) + ((BC == 64 ? piece ^ (r & 7) : piece ^ ((r >> 1) & 3)) << 4);
     };
-    const bool fetch = !PART && has_aux && !direct_aux;
+    const bool fetch = !PART && has_aux;
     [[maybe_unused]] uint32_t aux_phase = 0;
     // first row and column of this warp's part of a tile; whether there is anything of it
     auto part_of = [&](int tile, int& m, int& n) -> bool {
@@ -360,14 +350,6 @@ dense_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
       for (int c0 = 0; c0 < WARP_COLS; c0 += BC) {              // a box
         const bool box_live = live && n_warp0 + c0 < p.N;
         if (!AHEAD && fetch && box_live) fetch_aux(m_warp, n_warp0 + c0);
-        if (!PART && has_aux && direct_aux && box_live) {
-          if (!direct) {                     // the box's last store has been read
-            if (elect_one()) tma_store_wait_read0();
-            __syncwarp();
-          }
-          dense_copy_box<false>(box, const_cast<void*>(p.aux), p.ldaux, m_warp, n_warp0 + c0, p.M, p.N);
-          __syncwarp();
-        }
         if (!acc_ready) {
           if (!gemm_wait(accf_bar(buf), (it >> 1) & 1u, abort_flag, ST_TIMEOUT_EPILOGUE)) {
             ok = false;
@@ -454,8 +436,8 @@ dense_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         }
         if (!PART && direct && box_live) {
           __syncwarp();
-          if constexpr (KEEP) dense_copy_box<true>(zbox, p.keep, p.ldk, m_warp, n_warp0 + c0, p.M, p.N);
-          dense_copy_box<true>(box, p.out, p.ldo, m_warp, n_warp0 + c0, p.M, p.N);
+          if constexpr (KEEP) dense_copy_box(zbox, p.keep, p.ldk, m_warp, n_warp0 + c0, p.M, p.N);
+          dense_copy_box(box, p.out, p.ldo, m_warp, n_warp0 + c0, p.M, p.N);
           __syncwarp();
         }
         if (!PART && !direct && box_live) {

@@ -225,7 +225,8 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
             xp, wp = x2.data_ptr(), w2.data_ptr()
             need, ws = 0, None
             if M > 8:       # (so few rows take no workspace)
-                need = lib.strata_linear_act_workspace_bytes(M, N, K, not (xp & 15 or ldx & 7), not (wp & 15 or ldw & 7))
+                need = lib.strata_linear_act_workspace_bytes(M, N, K, not (xp & 15 or ldx & 7), not (wp & 15 or ldw & 7),
+                                                             r2 is None or not (r2.data_ptr() & 15 or ldr & 7))
                 ws = _scratch(need, x)
             code = lib.strata_linear_act(
                 xp, ldx, wp, ldw, None if bias is None else bias.data_ptr(), None if r2 is None else r2.data_ptr(), ldr,

@@ -149,45 +149,34 @@ inline int launch_dense_bn(int bn, const DenseOperand& A, const DenseOperand& B,
 }
 
 inline int launch_dense_finish(const DenseFinish& f, cudaStream_t st) {
-  const DensePlan& s = f.p.plan;
-  const int blocks = (f.p.part ? s.tiles * f.blocks_per_tile : 0) + (f.db ? (f.sum_cols + 7) / 8 : 0);
-  if (blocks == 0) return 0;
+  const int blocks = f.p.part ? f.p.plan.tiles * f.blocks_per_tile : (f.p.sum_cols + 7) / 8;
   if (f.p.fp16)
     return launch_chained(dense_finish_kernel<__half>, dim3(blocks), FINISH_THREADS, 0, st, 1, f);
   return launch_chained(dense_finish_kernel<__nv_bfloat16>, dim3(blocks), FINISH_THREADS, 0, st, 1, f);
 }
 
-// One product of a choice, with the second kernel where it is split. `fin`: the column sums that kernel adds up besides
-// (their fields only), or nullptr.
+// One product of a choice, with the second kernel where it is split.
 template <int LAY>
 inline int launch_dense(const DenseOperand& A, const DenseOperand& B, DenseParams p, const DenseChoice& c, void* slabs,
-                        const DenseFinish* sums, cudaStream_t st) {
-  DenseFinish f{};
-  if (sums) f = *sums;
-  int r;
-  if (c.split) {
-    p.part = static_cast<float*>(slabs);
-    p.plan = c.plan;
-    // (the slabs are fp32 and the type is a bit of the instruction descriptor: one kernel for both)
-    r = launch_dense_bn<LAY, DENSE_PART, __nv_bfloat16>(c.bn, A, B, p, c.plan.units, st);
-    f.p = p;
-    f.tile_m = c.tile_m();
-    f.bn = c.bn;
-    f.tiles_n = (p.N + c.bn - 1) / c.bn;
-    const int rows = p.M < f.tile_m ? p.M : f.tile_m;        // of a slab that exist
-    f.blocks_per_tile = (rows * c.bn + 4 * FINISH_THREADS - 1) / (4 * FINISH_THREADS);
-  } else {
-    p.part = nullptr;
-    if (LAY == DENSE_NT && p.keep != nullptr) {
-      r = p.fp16 ? launch_dense_bn<DENSE_NT, DENSE_Y_KEEP, __half>(c.bn, A, B, p, c.plan.units, st)
-                 : launch_dense_bn<DENSE_NT, DENSE_Y_KEEP, __nv_bfloat16>(c.bn, A, B, p, c.plan.units, st);
-    } else {
-      r = p.fp16 ? launch_dense_bn<LAY, DENSE_Y, __half>(c.bn, A, B, p, c.plan.units, st)
-                 : launch_dense_bn<LAY, DENSE_Y, __nv_bfloat16>(c.bn, A, B, p, c.plan.units, st);
-    }
-    f.p = p;
+                        cudaStream_t st) {
+  if (!c.split) {
+    if (LAY == DENSE_NT && p.keep != nullptr)
+      return p.fp16 ? launch_dense_bn<DENSE_NT, DENSE_Y_KEEP, __half>(c.bn, A, B, p, c.plan.units, st)
+                    : launch_dense_bn<DENSE_NT, DENSE_Y_KEEP, __nv_bfloat16>(c.bn, A, B, p, c.plan.units, st);
+    return p.fp16 ? launch_dense_bn<LAY, DENSE_Y, __half>(c.bn, A, B, p, c.plan.units, st)
+                  : launch_dense_bn<LAY, DENSE_Y, __nv_bfloat16>(c.bn, A, B, p, c.plan.units, st);
   }
-  if (r != 0 || (!c.split && !sums)) return r;
+  p.part = static_cast<float*>(slabs);
+  p.plan = c.plan;
+  // (the slabs are fp32 and the type is a bit of the instruction descriptor: one kernel for both)
+  if (const int r = launch_dense_bn<LAY, DENSE_PART, __nv_bfloat16>(c.bn, A, B, p, c.plan.units, st); r != 0) return r;
+  DenseFinish f{};
+  f.p = p;
+  f.tile_m = c.tile_m();
+  f.bn = c.bn;
+  f.tiles_n = (p.N + c.bn - 1) / c.bn;
+  const int rows = p.M < f.tile_m ? p.M : f.tile_m;        // of a slab that exist
+  f.blocks_per_tile = (rows * c.bn + 4 * FINISH_THREADS - 1) / (4 * FINISH_THREADS);
   return launch_dense_finish(f, st);
 }
 
@@ -309,7 +298,7 @@ inline int launch_dense_forward(DenseOperand x, DenseOperand w, DenseParams p, v
     if (const int r = launch_chained(dense_align_rows_kernel, grid, 256, 0, st, 1, a); r != 0) return r;
   }
   const DenseChoice c = dense_choice(p.M, p.N, p.K, sms);
-  return launch_dense<DENSE_NT>(x, w, p, c, ws.take(c.slab_bytes()), nullptr, st);
+  return launch_dense<DENSE_NT>(x, w, p, c, ws.take(c.slab_bytes()), st);
 }
 
 // ---------------------------------------------------------------- backward
@@ -394,24 +383,32 @@ inline int launch_dense_backward(const DenseGradParams& q, const DenseGradPlan& 
     if (r != 0) return r;
     if (g.make_dz) dz = {g.dz, dense_round8(q.N)};
   }
+  // db is added up by the first product's kernel
+  auto sums = [&](DenseParams& p) {
+    p.sums = g.col_sums; p.sum_rows = g.sums.blocks; p.sum_cols = q.N; p.db = q.db;
+  };
   if (q.dx) {
     DenseParams p{};
     p.M = q.M; p.N = q.K; p.K = q.N;
     p.out = q.dx; p.ldo = q.lddx; p.fp16 = q.fp16;
     p.direct_out = !dense_whole(q.dx, q.lddx, q.K, q.padded);
-    if ((r = launch_dense<DENSE_NN>(dz, w, p, g.cx, g.slabs, nullptr, st)) != 0) return r;
+    if (q.db) sums(p);
+    if ((r = launch_dense<DENSE_NN>(dz, w, p, g.cx, g.slabs, st)) != 0) return r;
   }
-  DenseFinish f{};
-  f.sums = g.col_sums;
-  f.sum_rows = g.sums.blocks; f.sum_cols = q.N; f.db = q.db;
   if (q.dw) {
     DenseParams p{};
     p.M = q.N; p.N = q.K; p.K = q.M;
     p.out = q.dw; p.ldo = q.lddw; p.fp16 = q.fp16;
     p.direct_out = !dense_whole(q.dw, q.lddw, q.K, false);
-    return launch_dense<DENSE_TN>(dz, x, p, g.cw, g.slabs, q.db ? &f : nullptr, st);
+    if (q.db && !q.dx) sums(p);
+    return launch_dense<DENSE_TN>(dz, x, p, g.cw, g.slabs, st);
   }
-  return q.db ? launch_dense_finish(f, st) : 0;
+  if (q.db && !q.dx) {
+    DenseFinish f{};
+    sums(f.p);
+    return launch_dense_finish(f, st);
+  }
+  return 0;
 }
 
 }  // namespace strata

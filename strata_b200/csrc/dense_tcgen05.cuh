@@ -36,8 +36,29 @@ struct DenseParams {
   int fp16;
   bool direct_out;              // out and keep are written by the warps, not by TMA
   float* part;                  // DENSE_PART: slabs of TILE_M x BN
+  const float* sums;            // column sums that dense_slope_kernel left, [sum_rows, sum_cols], or nullptr; added up into
+  int sum_rows, sum_cols;       //   db by epilogue warps that wait for their first tile
+  float* db;
   DensePlan plan;
 };
+
+// db of eight columns: 256 threads, 32 rows of sums side by side, in a fixed order. `sync` is a barrier of those threads.
+template <typename Sync>
+__device__ __forceinline__ void dense_column_sums(const DenseParams& p, int group, int tid, float (*red)[9], Sync sync) {
+  const int col = group * 8 + (tid & 7), r0 = tid >> 3;
+  float a = 0.f;
+  if (col < p.sum_cols) {
+#pragma unroll 8
+    for (int r = r0; r < p.sum_rows; r += 32) a += p.sums[static_cast<long long>(r) * p.sum_cols + col];
+  }
+  red[r0][tid & 7] = a;
+  sync();
+  if (r0 == 0 && col < p.sum_cols) {
+#pragma unroll
+    for (int i = 1; i < 32; ++i) a += red[i][tid & 7];
+    p.db[col] = a;
+  }
+}
 
 // AHEAD: the residual of the next tile is loaded while this one is computed.
 template <int BN, bool PAIR, int EPI, bool AHEAD>
@@ -51,7 +72,8 @@ struct DenseSmem {
   static constexpr int BOXES = EPI == DENSE_PART ? 0 : EPI == DENSE_Y_KEEP ? 2 : 1;
   static constexpr int STAGES = BN > 64 && BOXES * BOX_BYTES > 2048 ? 5 : 6;
   static constexpr int STAGING_OFF = STAGES * STAGE_BYTES;
-  static constexpr int BAR_OFF = STAGING_OFF + GEMM_EPI_WARPS * BOXES * BOX_BYTES;
+  static constexpr int SUMS_BYTES = 32 * 9 * 4;                  // of dense_column_sums, in the boxes' place
+  static constexpr int BAR_OFF = STAGING_OFF + (BOXES > 0 ? GEMM_EPI_WARPS * BOXES * BOX_BYTES : SUMS_BYTES);
   static constexpr int TOTAL = BAR_OFF + 512 + 1024;            // + alignment slack
   static_assert(TOTAL <= 232448, "shared memory of an SM");
 };
@@ -324,6 +346,17 @@ dense_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         tma_load_2d(box, &tmAux, n, m, aux_bar(e));
       }
     };
+    if constexpr (LAY != DENSE_NT) {
+      // the first eight warps, while the operands of the first tile are on their way
+      if (p.sums != nullptr && e < 8) {
+        float(*red)[9] = reinterpret_cast<float(*)[9]>(smem_gen + S::STAGING_OFF);
+        auto sync = []() { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+        for (int group = blockIdx.x; group * 8 < p.sum_cols; group += gridDim.x) {
+          dense_column_sums(p, group, static_cast<int>(threadIdx.x) - 64, red, sync);
+          sync();
+        }
+      }
+    }
     int it = 0;
     bool ok = true;
     DenseWalk walk(unit);
@@ -469,14 +502,11 @@ dense_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
 }
 
 // ---------------------------------------------------------------- the second half of a split product
-// Adds up a tile's slabs in the order of their slots and applies the epilogue; blocks behind the tiles' add up the
-// column sums that dense_slope_kernel left (db). A thread has four columns of a row.
+// Adds up a tile's slabs in the order of their slots and applies the epilogue. A thread has four columns of a row. Without
+// slabs: the column sums alone (db where no product is asked for).
 struct DenseFinish {
   DenseParams p;
   int tile_m, bn, tiles_n, blocks_per_tile;
-  const float* sums;       // [sum_rows, N] or nullptr
-  int sum_rows, sum_cols;
-  float* db;
 };
 
 constexpr int FINISH_THREADS = 256;
@@ -487,23 +517,9 @@ __global__ void __launch_bounds__(FINISH_THREADS) dense_finish_kernel(const Dens
   chain_begin();
   const DenseParams& p = f.p;
   const DensePlan& s = p.plan;
-  const int tile_blocks = p.part != nullptr ? s.tiles * f.blocks_per_tile : 0;
-  if (static_cast<int>(blockIdx.x) >= tile_blocks) {
-    // eight columns a block, 32 rows of sums side by side
+  if (p.part == nullptr) {
     __shared__ float red[32][9];
-    const int col = (blockIdx.x - tile_blocks) * 8 + (threadIdx.x & 7), r0 = threadIdx.x >> 3;
-    float a = 0.f;
-    if (col < f.sum_cols) {
-#pragma unroll 8
-      for (int r = r0; r < f.sum_rows; r += 32) a += f.sums[static_cast<long long>(r) * f.sum_cols + col];
-    }
-    red[r0][threadIdx.x & 7] = a;
-    __syncthreads();
-    if (r0 == 0 && col < f.sum_cols) {
-#pragma unroll
-      for (int i = 1; i < 32; ++i) a += red[i][threadIdx.x & 7];
-      f.db[col] = a;
-    }
+    dense_column_sums(p, blockIdx.x, threadIdx.x, red, []() { __syncthreads(); });
     return;
   }
   __shared__ int slots[FINISH_SLOTS];

@@ -62,7 +62,8 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
   return y;
 }
-// x / (1 + 2^v) of a pair with one reciprocal for both: 1 / a = b / (a b). 2^v must stay below 2^63.
+// x / (1 + 2^v) of a pair with one reciprocal for both: 1 / a = b / (a b). 2^v must stay below 2^63, and v may not be NaN:
+// it would reach the other value.
 __device__ __forceinline__ uint64_t dense_sigmoid_pair(uint64_t x, uint64_t v) {
   float v0, v1, d0, d1;
   unpack2(v, v0, v1);
@@ -107,15 +108,16 @@ __device__ __forceinline__ uint64_t dense_act_pair(uint64_t x) {
     return ffma2(hx, pack2(fast_tanh(u0), fast_tanh(u1)), hx);
   } else if constexpr (ACT == ACT_GELU) {
     x = pack2(max_nan(a, -6.f), max_nan(b, -6.f));
+    const uint64_t e = pack2(fmaxf(a, -6.f), fmaxf(b, -6.f));       // (no NaN)
     using F = GeluFit<T>;
-    const uint64_t t = fmul2(x, x);
+    const uint64_t t = fmul2(e, e);
     uint64_t p = pack2(F::c(F::N - 1), F::c(F::N - 1));
 #pragma unroll
     for (int i = F::N - 2; i >= 0; --i) p = ffma2(p, t, pack2(F::c(i), F::c(i)));
-    return dense_sigmoid_pair(x, fmul2(x, p));
+    return dense_sigmoid_pair(x, fmul2(e, p));
   } else if constexpr (ACT == ACT_SILU) {
     x = pack2(max_nan(a, -40.f), max_nan(b, -40.f));
-    return dense_sigmoid_pair(x, fmul2(x, pack2(-LOG2E, -LOG2E)));
+    return dense_sigmoid_pair(x, fmul2(pack2(fmaxf(a, -40.f), fmaxf(b, -40.f)), pack2(-LOG2E, -LOG2E)));
   } else if constexpr (ACT == ACT_RELU) {
     return pack2(max_nan(a, 0.f), max_nan(b, 0.f));
   } else {

@@ -169,6 +169,14 @@ def _packed_rows(t: torch.Tensor, cols: int, name: str):
     return t, rows, row if rows > 1 else cols
 
 
+_MOST = 0x7FFF0000      # rows, columns and tokens that the kernels count with 32 bits
+
+
+def _countable(*sizes) -> None:
+    if max(sizes) > _MOST:
+        raise ValueError(f"sizes up to {_MOST} are supported, got {sizes}")
+
+
 def _scratch(need: int, x):
     if need < 0:
         _lib.check(need, "workspace size")
@@ -203,6 +211,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     N, K = weight.shape
     x2, M, ldx = _packed_rows(x, K, "x")
     w2, _, ldw = _packed_rows(weight, K, "weight")
+    _countable(M, N, K)
     bias = _f32_like(bias, "bias", N, x)
     shape = x.shape[:-1] + (N,)
     r2, ldr = None, 0
@@ -254,6 +263,7 @@ def linear_act_backward(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tenso
     N, K = weight.shape
     x2, M, ldx = _packed_rows(x, K, "x")
     w2, _, ldw = _packed_rows(weight, K, "weight")
+    _countable(M, N, K)
     shape = x.shape[:-1] + (N,)
     if grad.shape != shape:
         raise ValueError(f"grad must be {tuple(shape)}, got {tuple(grad.shape)}")
@@ -727,6 +737,7 @@ def _qk_arguments(q, k, q_weight, k_weight, rope_cs, positions, tokens_per_tile,
     if hd % 8 or not 8 <= hd <= 256 or not hq or not hk:
         raise ValueError(f"head_dim must be a multiple of 8 up to 256 and both have heads, got {hq} + {hk} heads of {hd}")
     M = qs[0] if len(qs) == 3 else qs[:-2].numel()
+    _countable(M)
     wq, wk = _f32_like(q_weight, "q_weight", hd, q), _f32_like(k_weight, "k_weight", hd, q)
     if wq is not None and wq.data_ptr() & 15:
         wq = wq.clone()
@@ -749,8 +760,8 @@ def _qk_arguments(q, k, q_weight, k_weight, rope_cs, positions, tokens_per_tile,
     if cs.data_ptr() & 15:
         cs = cs.clone()
     rows = cs.numel() // rot
-    if not rows:
-        raise ValueError("rope_cs has no rows")
+    if not 0 < rows <= _MOST:
+        raise ValueError(f"rope_cs must have 1 to {_MOST} rows, got {rows}")
     pos, wide = None, 0
     if positions is not None:
         if positions.dtype not in (torch.int32, torch.int64) or positions.device != q.device:
@@ -768,6 +779,7 @@ def _qk_arguments(q, k, q_weight, k_weight, rope_cs, positions, tokens_per_tile,
             raise ValueError("tokens_per_tile and hw must be positive")
         if M and (M - 1) // per * hw + min(M, hw) > rows:
             raise ValueError(f"{M} tokens, {per} a tile with {hw} rows each, need more than the {rows} rows of rope_cs")
+        per, hw = min(per, _MOST), min(hw, _MOST)      # (more tokens than there are: the same rule)
     return hq, hk, hd, M, (wq, wk, cs, pos), (
         rot, interleaved, cs.data_ptr(), cs.dtype == torch.float32, rows, None if pos is None else pos.data_ptr(), wide,
         per, hw)

@@ -83,6 +83,16 @@ def test_qk_norm_rope_refuses(cuda, change, error):
         ops.qk_norm_rope_backward(t["q"], t["k"], t["q"], t["k"], t["qw"], t["kw"], **table)
 
 
+def test_sizes_that_32_bits_do_not_count_are_refused(cuda):
+    big = 2 ** 32 + 8
+    with pytest.raises(ValueError, match="supported"):
+        ops.linear_act(cuda(1, 16).expand(big, 16), cuda(8, 16))
+    with pytest.raises(ValueError, match="supported"):
+        ops.linear_act_backward(cuda(4, 8), cuda(4, big), cuda(8, big))
+    with pytest.raises(ValueError, match="supported"):
+        ops.qk_norm_rope(cuda(big, 1, 8), cuda(big, 1, 8))
+
+
 def test_empty_batches_come_back_empty(cuda):
     y, z = ops.linear_act(cuda(2, 0, 16), cuda(8, 16), activation="silu", save_preact=True)
     assert y.shape == z.shape == (2, 0, 8)

@@ -258,6 +258,23 @@ def test_infinite_and_nan_preactivations(ops, act):
     assert y[2].isnan().all() and int(y.isnan().sum()) == 16
 
 
+@pytest.mark.parametrize("act", ["none", "gelu", "gelu_tanh", "silu", "relu"])
+@pytest.mark.parametrize("M,N,K", [(3, 40, 64), (20, 40, 512), (64, 72, 4096), (200, 72, 64), (2048, 1024, 64)])
+def test_nan_stays_in_its_column(ops, act, M, N, K):
+    """A NaN or an infinity in one output's weights or bias reaches no other output, in any form of the product."""
+    d = data(M, N, K, BF)
+    want = ops.linear_act(d["x"], d["w"], d["b"], act, d["r"])
+    w, b = d["w"].clone(), d["b"].clone()
+    w[5], b[10], b[17], b[22] = float("nan"), float("nan"), float("inf"), float("-inf")
+    y, z = ops.linear_act(d["x"], w, b, act, d["r"], save_preact=True)
+    clean = torch.ones(N, dtype=torch.bool, device="cuda")
+    clean[[5, 10, 17, 22]] = False
+    # (two neighbours share a reciprocal, so a neighbour may move within the formula's rounding, 2^-20 |z|, and then by a step)
+    step = torch.finfo(BF).eps * want[:, clean].float().abs() + 2.0 ** -19 * z[:, clean].float().abs()
+    assert bool(((y[:, clean].float() - want[:, clean].float()).abs() <= step).all())
+    assert y[:, [5, 10]].isnan().all() and (y[:, 17] == float("inf")).all() and not z[:, clean].isnan().any()
+
+
 def test_offsets_beyond_32_bits(ops):
     """4.3e9 outputs and inputs: the rows behind 2^32 elements are their own."""
     M, N = 1_048_800, 4104
@@ -335,6 +352,22 @@ def test_autograd_is_the_backward_call(ops):
     w = d["w"].clone().requires_grad_()
     op(d["x"], w, d["b"], "silu")[0].sum().backward()
     assert w.grad is not None
+
+
+@pytest.mark.parametrize("N", [24, 27])
+def test_operator_registration(ops, N):
+    """Schema, shape-only implementation (strides of odd widths included) and gradients as torch checks them."""
+    from strata_b200 import torch_ops  # noqa: F401
+    d = data(40, N, 32, BF)
+    x, w, b, r = (d[k].clone().requires_grad_() for k in "xwbr")
+    torch.library.opcheck(torch.ops.strata_b200.linear_act, (x, w, b, "silu", r, True),
+                          test_utils=("test_schema", "test_faketensor", "test_autograd_registration"))
+    f = torch.compile(lambda x, w, b, r: torch.ops.strata_b200.linear_act(x, w, b, "silu", r, True)[0] * 2, fullgraph=True)
+    y = f(x, w, b, r)
+    assert torch.equal(y, 2 * ops.linear_act(d["x"], d["w"], d["b"], "silu", d["r"]))
+    y.backward(d["dy"])
+    want = ops.linear_act_backward(2 * d["dy"], d["x"], d["w"], "silu", ops.linear_act(d["x"], d["w"], d["b"]))
+    assert all(torch.equal(t.grad, v) for t, v in zip((x, w, b, r), (*want, 2 * d["dy"])))
 
 
 def test_captured_training_step(ops):

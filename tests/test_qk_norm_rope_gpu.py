@@ -291,6 +291,19 @@ def test_projection_norm_attention_projection(ops):
     assert float((got.float() - want.float()).abs().max() / want.float().abs().max()) < 2e-2
 
 
+def test_operator_registration(ops):
+    from strata_b200 import torch_ops  # noqa: F401
+    d = data(30, 4, 2, 64, BF, rot=64, rows=30)
+    q, k, qw, kw = (d[n].clone().requires_grad_() for n in ("q", "k", "qw", "kw"))
+    pos = torch.arange(30, device="cuda").flip(0)
+    torch.library.opcheck(torch.ops.strata_b200.qk_norm_rope, (q, k, qw, kw, d["cs"], pos),
+                          test_utils=("test_schema", "test_faketensor", "test_autograd_registration"))
+    f = torch.compile(lambda q, k, qw, kw: torch.ops.strata_b200.qk_norm_rope(q, k, qw, kw, d["cs"], pos), fullgraph=True)
+    torch.autograd.backward(f(q, k, qw, kw), (d["dq"], d["dk"]))
+    want = ops.qk_norm_rope_backward(d["dq"], d["dk"], d["q"], d["k"], d["qw"], d["kw"], rope_cs=d["cs"], positions=pos)
+    assert all(torch.equal(t.grad, v) for t, v in zip((q, k, qw, kw), want))
+
+
 def test_gradients_through_projection_norm_and_mlp(ops):
     """A training step over the differentiable operators against autograd in 64 bits on the same bf16 weights: bf16 keeps 8
     bits of every intermediate value and gradient, four roundings in a row of 2^-9 rms each at most."""

@@ -49,7 +49,15 @@ inline int dense_pairs(int sms) {
 }
 
 // The cheapest form by a model of each one's time, in microseconds: a k-block of 64 on one unit, the part of a tile's
-// epilogue that nothing hides, a launch, and a slab's way to memory and back.
+// epilogue that nothing hides, a launch, and a slab's way to memory and back. Some of the shapes it was checked on,
+// tiles of 64 / 128 / 256 unsplit, then split (the one taken in brackets):
+//   y   64 x 1024, K = 4096    12.0 / 13.5 / 23.3   [7.4] / 10.6 / 12.3
+//   y   2500 x 650, K = 207    6.6 / [5.9] / 7.2    (no split: enough tiles, four k-blocks)
+//   y   98304 x 512, K = 2048  255 / 187 / [153]    371 / 296 / 249
+//   dW  512 x 128 of 65536 rows    161 / 176 / 182    [21.5] / 24.4 / 24.5
+//   dW  1536 x 384 of 20000 rows   54 / 59 / 93       53 / [26.2] / 29.2
+//   dW  2048 x 512 of 98304 rows   265 / 289 / 438    271 / 194 / [158]
+//   dW  4096 x 4096 of 3000 rows   115 / 77 / [68]    156 / 77 / 97
 inline DenseChoice dense_choice(int M, int N, int K, int sms) {
   const int num_kb = (K + GEMM_BK - 1) / GEMM_BK;
   DenseChoice best{};
@@ -86,7 +94,8 @@ inline DenseChoice dense_choice(int M, int N, int K, int sms) {
 struct DenseOperand { const void* p; long long ld; };
 
 template <int BN, bool PAIR, int LAY, int EPI, typename T, int ACT = ACT_ANY, bool AUX = false>
-inline int launch_dense_t(const DenseOperand& A, const DenseOperand& B, const DenseParams& p, int units, cudaStream_t st) {
+inline int launch_dense_t(const DenseOperand& A, const DenseOperand& B, const DenseParams& p, int units,
+                          cudaStream_t st) {
   const bool a_mn = LAY == DENSE_TN, b_mn = LAY != DENSE_NT;
   constexpr int TILE_M = PAIR ? 2 * GEMM_BM : GEMM_BM;
   CUtensorMap tmA, tmB, tmOut, tmKeep, tmAux;
@@ -122,7 +131,10 @@ inline int launch_dense_t(const DenseOperand& A, const DenseOperand& B, const De
 }
 
 // Forward pass on pairs of CTAs: a kernel for each activation, with and without a residual. One kernel that reads both
-// from its parameters keeps the registers of all of them (TODO figures).
+// from its parameters keeps the registers and the code of all of them in its loop; 262144 x 2048, K = 512, microseconds
+// that way / this: no activation 431 / 415, silu 539 / 435, gelu 673 / 481 (473 with the shorter fit), with a residual
+// 658 / 590. The residual a tile ahead, in boxes of 64 columns: 590 -> 537; such boxes without a residual: silu 435 ->
+// 497.
 template <int EPI, typename T, bool AUX>
 inline int launch_dense_pair(const DenseOperand& A, const DenseOperand& B, const DenseParams& p, int units,
                              cudaStream_t st) {
@@ -203,8 +215,8 @@ inline int launch_few_rows_t(const DenseOperand& x, const DenseOperand& w, const
   while (parts < 8 && steps > 2 * parts && 2 * parts * blocks <= 8 * sms) parts *= 2;
   const int k_part = (steps + parts - 1) / parts * FEW_STEP;
   auto go = [&](auto kern) {
-    return launch_chained(kern, dim3(static_cast<unsigned>(blocks * parts)), 32 * FEW_WARPS, 0, st, parts, xp, x.ld, wp, w.ld,
-                          k_part, parts, p);
+    return launch_chained(kern, dim3(static_cast<unsigned>(blocks * parts)), 32 * FEW_WARPS, 0, st, parts, xp, x.ld, wp,
+                          w.ld, k_part, parts, p);
   };
   if (p.M <= 8) return go(dense_few_rows_kernel<T, 1, ALIGNED>);
   if (p.M <= 16) return go(dense_few_rows_kernel<T, 2, ALIGNED>);
@@ -213,24 +225,27 @@ inline int launch_few_rows_t(const DenseOperand& x, const DenseOperand& w, const
 inline int launch_few_rows(const DenseOperand& x, const DenseOperand& w, const DenseParams& p, bool aligned, int sms,
                            cudaStream_t st) {
   if (p.fp16)
-    return aligned ? launch_few_rows_t<__half, true>(x, w, p, sms, st) : launch_few_rows_t<__half, false>(x, w, p, sms, st);
+    return aligned ? launch_few_rows_t<__half, true>(x, w, p, sms, st)
+                   : launch_few_rows_t<__half, false>(x, w, p, sms, st);
   return aligned ? launch_few_rows_t<__nv_bfloat16, true>(x, w, p, sms, st)
                  : launch_few_rows_t<__nv_bfloat16, false>(x, w, p, sms, st);
 }
 
-// Whether the forms for a few rows take a product: one launch and no workspace. From nine rows on every block of 16 columns
-// reads more of x than of W, and the tiles of a split product overtake them at large weights. Microseconds of these /
-// of a split, weights out of HBM (half, gelu, residual): 9 x 1024, K = 1024 3.8 / 5.8; 16 x 2048, K = 2048 6.0 / 10.6;
-// 24 x 1024, K = 4096 8.0 / 8.5; 24 x 4096, K = 1024 7.7 / 8.4; 32 x 512, K = 2048 5.2 / 7.8; 32 x 4096, K = 4096 21.9 / 13.6;
-// 48 x 1024, K = 4096 16.2 / 8.7; 8 x 4096, K = 4096 13.3 / 14.0. Dot products / mma.sync: 1 x 4096, K = 1024 4.3 / 5.0; 1 x
-// 1024, K = 4096 4.1 / 7.8; 4 x 4096, K = 1024 4.9 / 5.0; 8 x 4096, K = 1024 12.7 / 5.0.
+// Whether the forms for a few rows take a product: one launch and no workspace. From nine rows on every block of 16
+// columns reads more of x than of W, and the tiles of a split product overtake them at large weights. Microseconds of
+// these / of a split, weights out of HBM (half, gelu, residual): 9 x 1024, K = 1024 3.8 / 5.8; 16 x 2048, K = 2048 6.0
+// / 10.6; 24 x 1024, K = 4096 8.0 / 8.5; 24 x 4096, K = 1024 7.7 / 8.4; 32 x 512, K = 2048 5.2 / 7.8; 32 x 4096, K =
+// 4096 21.9 / 13.6; 48 x 1024, K = 4096 16.2 / 8.7; 8 x 4096, K = 4096 13.3 / 14.0. Dot products / mma.sync: 1 x 4096,
+// K = 1024 4.3 / 5.0; 1 x 1024, K = 4096 4.1 / 7.8; 4 x 4096, K = 1024 4.9 / 5.0; 8 x 4096, K = 1024 12.7 / 5.0.
 inline bool dense_few(int M, int N, int K) {
   const long long weights = static_cast<long long>(N) * K;
   return M <= 8 || (M <= FEW_ROWS && (M <= 16 ? 2 : 4) * weights <= (1ll << 25));
 }
 
 inline long long dense_round8(long long n) { return (n + 7) / 8 * 8; }
-inline bool dense_aligned(const void* p, long long ld) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % 8 == 0; }
+inline bool dense_aligned(const void* p, long long ld) {
+  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % 8 == 0;
+}
 // Rows that TMA may store: it writes whole 16-byte pieces, with zeros behind the last column. padded: those are the
 // caller's to write.
 inline bool dense_whole(const void* p, long long ld, int cols, bool padded) {
@@ -339,8 +354,8 @@ struct DenseGradPlan {
   float* col_sums;
 };
 
-inline DenseGradPlan dense_grad_plan(int M, int N, int K, bool act, bool dy_ok, bool z_ok, bool x_ok, bool w_ok, bool dx,
-                                     bool dw, bool db, void* workspace, int sms) {
+inline DenseGradPlan dense_grad_plan(int M, int N, int K, bool act, bool dy_ok, bool z_ok, bool x_ok, bool w_ok,
+                                     bool dx, bool dw, bool db, void* workspace, int sms) {
   DenseGradPlan g{};
   g.make_dz = (dx || dw) && (act || !dy_ok);
   g.copy_x = dw && !x_ok;

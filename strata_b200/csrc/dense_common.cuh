@@ -48,8 +48,8 @@ __device__ __forceinline__ float fast_rcp(float x) {
   return y;
 }
 
-// The slope's Phi: the normal distribution's upper tail Q(a) = 1 - Phi(a), a >= 0, by formula 7.1.26 of Abramowitz and Stegun (erf to
-// 1.5e-7) with x = a / sqrt(2); e = exp(-a^2 / 2).
+// The slope's Phi: the normal distribution's upper tail Q(a) = 1 - Phi(a), a >= 0, by formula 7.1.26 of Abramowitz and
+// Stegun (erf to 1.5e-7) with x = a / sqrt(2); e = exp(-a^2 / 2).
 constexpr float GELU_P = 0.3275911f * 0.70710678118654752f;
 constexpr float GELU_C1 = 0.5f * 0.254829592f, GELU_C2 = 0.5f * -0.284496736f, GELU_C3 = 0.5f * 1.421413741f,
                 GELU_C4 = 0.5f * -1.453152027f, GELU_C5 = 0.5f * 1.061405429f;
@@ -62,8 +62,8 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
   return y;
 }
-// x / (1 + 2^v) of a pair with one reciprocal for both: 1 / a = b / (a b). 2^v must stay below 2^63, and v may not be NaN:
-// it would reach the other value.
+// x / (1 + 2^v) of a pair with one reciprocal for both: 1 / a = b / (a b). 2^v must stay below 2^63, and v may not be
+// NaN: it would reach the other value.
 __device__ __forceinline__ uint64_t dense_sigmoid_pair(uint64_t x, uint64_t v) {
   float v0, v1, d0, d1;
   unpack2(v, v0, v1);
@@ -142,8 +142,8 @@ __device__ __forceinline__ void dense_act(int act, uint64_t (&v)[N]) {
   }
 }
 
-// act'(z). A stored z may be infinite (fp16): the slope is then that of a far z, 0 or 1 to 1e-11; NaN stays NaN. 1 - s of
-// s = 1 / (1 + e) is taken as e s: the difference would lose the digits that z s (1 - s) multiplies up.
+// act'(z). A stored z may be infinite (fp16): the slope is then that of a far z, 0 or 1 to 1e-11; NaN stays NaN. 1 - s
+// of s = 1 / (1 + e) is taken as e s: the difference would lose the digits that z s (1 - s) multiplies up.
 template <int ACT>
 __device__ __forceinline__ float dense_slope(float z) {
   if constexpr (ACT == ACT_NONE) return 1.f;
@@ -172,8 +172,8 @@ __device__ __forceinline__ float dense_slope(float z) {
 // tiles = whole + rest. The first `whole` (a multiple of the units) are walked as they are. Of the others every tile's
 // k-blocks are cut into `chunks` of `len`, and each of the rest * chunks pieces has a unit that does its first `head`
 // blocks; the units left over share the tails, in order, so that all finish together. Units beside one another work on
-// the same k-blocks of different tiles at the same time and share their operands in L2 (cut into one contiguous range of
-// (tile, k-block) per unit instead, no two read the same and each tile's operands come from HBM).
+// the same k-blocks of different tiles at the same time and share their operands in L2 (cut into one contiguous range
+// of (tile, k-block) per unit instead, no two read the same and each tile's operands come from HBM).
 struct DensePlan {
   int tiles, units, num_kb;
   int whole, rest, chunks, len, head, tail;   // tail = len - head

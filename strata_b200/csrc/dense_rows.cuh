@@ -5,9 +5,9 @@
 
 namespace strata {
 
-// Eight values of a row from p on, of which n exist (n <= 0: none), the others zero. ALIGNED: p is a multiple of 16 bytes and
-// n >= 8 or n <= 0. Otherwise the two aligned 16-byte pieces that hold them are read and shifted together: a piece is
-// read only if it holds a value that exists, and memory is given out in larger units than 16 bytes.
+// Eight values of a row from p on, of which n exist (n <= 0: none), the others zero. ALIGNED: p is a multiple of 16
+// bytes and n >= 8 or n <= 0. Otherwise the two aligned 16-byte pieces that hold them are read and shifted together: a
+// piece is read only if it holds a value that exists, and memory is given out in larger units than 16 bytes.
 template <bool ALIGNED>
 __device__ __forceinline__ uint4 load8(const void* p, int n) {
   uint4 u = make_uint4(0u, 0u, 0u, 0u);
@@ -53,11 +53,11 @@ __device__ __forceinline__ void dense_one(const DenseParams& p, int row, int col
 }
 
 // ---------------------------------------------------------------- y = r + act(x W^T + b) for one to four rows
-// Bound by the weights' way from HBM (2 N K bytes; at one row an operation per byte), so no tensor cores. A warp takes four
-// output columns and all rows; its lanes have 16 bytes of each of the four weight rows in flight at a time, whole lines of
-// a row, and share the x they multiply them with. kw of the block's eight warps split the contraction where N alone does
-// not give every SM enough warps. Sums are fp32, even and odd k apart, then over the lanes and the kw warps in a fixed
-// order.
+// Bound by the weights' way from HBM (2 N K bytes; at one row an operation per byte), so no tensor cores. A warp takes
+// four output columns and all rows; its lanes have 16 bytes of each of the four weight rows in flight at a time, whole
+// lines of a row, and share the x they multiply them with. kw of the block's eight warps split the contraction where N
+// alone does not give every SM enough warps. Sums are fp32, even and odd k apart, then over the lanes and the kw warps
+// in a fixed order.
 constexpr int DOT_ROWS = 4;
 constexpr int DOT_COLS = 4;
 
@@ -117,7 +117,8 @@ __global__ void __launch_bounds__(256) dense_dot_rows_kernel(const T* __restrict
       unpack2(acc[c][r], lo, hi);
       v[c * ROWS + r] = lo + hi;
     }
-  // over the lanes, halving what a lane keeps while there is something to halve: lane l ends up with value l / (32 / NV)
+  // over the lanes, halving what a lane keeps while there is something to halve: lane l ends up with value l / (32 /
+  // NV)
   int off = 16;
 #pragma unroll
   for (int n = NV / 2; n >= 1; n >>= 1, off >>= 1) {
@@ -139,21 +140,21 @@ __global__ void __launch_bounds__(256) dense_dot_rows_kernel(const T* __restrict
 }
 
 // ---------------------------------------------------------------- y = r + act(x W^T + b) for a few rows
-// Bound by the weights' way from HBM (2 N K bytes) and by latency: a 128-row tile on tcgen05 would read them through N /
-// 64 CTAs and one pipeline each, or need a second kernel and a workspace to add up a split. Here a block has 16 output
-// columns and all rows; its eight warps, and where K is long the blocks of a cluster, split the contraction so that every
-// warp has all it reads in flight at once. A lane reads 16 bytes of two weight rows and of a row of x straight into the
-// fragments of mma.sync.m16n8k16: the product does not care which k is which as long as both operands agree, so
-// lane t of a quad takes k = 8 t ... 8 t + 7 of 32 and hands them over as two steps of 16. Sums are fp32, over the warps
-// and then over the cluster (through distributed shared memory) in a fixed order.
+// Bound by the weights' way from HBM (2 N K bytes) and by latency: a 128-row tile on tcgen05 would read them through N
+// / 64 CTAs and one pipeline each, or need a second kernel and a workspace to add up a split. Here a block has 16
+// output columns and all rows; its eight warps, and where K is long the blocks of a cluster, split the contraction so
+// that every warp has all it reads in flight at once. A lane reads 16 bytes of two weight rows and of a row of x
+// straight into the fragments of mma.sync.m16n8k16: the product does not care which k is which as long as both
+// operands agree, so lane t of a quad takes k = 8 t ... 8 t + 7 of 32 and hands them over as two steps of 16. Sums are
+// fp32, over the warps and then over the cluster (through distributed shared memory) in a fixed order.
 constexpr int FEW_ROWS = 32;
 constexpr int FEW_COLS = 16;
 constexpr int FEW_WARPS = 8;
 constexpr int FEW_STEP = 32 * FEW_WARPS;      // contraction values that a block takes at a time
 
 template <typename T>
-__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                          uint32_t b1) {
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                          uint32_t b0, uint32_t b1) {
   if constexpr (Pair16<T>::UMMA_FORMAT == 1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
                  "{%0, %1, %2, %3};"
@@ -170,8 +171,8 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
 // NT: blocks of eight rows. k_part: contraction values of a block of the cluster, a multiple of FEW_STEP.
 template <typename T, int NT, bool ALIGNED>
 __global__ void __launch_bounds__(32 * FEW_WARPS) dense_few_rows_kernel(const T* __restrict__ x, long long ldx,
-                                                                        const T* __restrict__ w, long long ldw, int k_part,
-                                                                        int parts, const DenseParams p) {
+                                                                        const T* __restrict__ w, long long ldw,
+                                                                        int k_part, int parts, const DenseParams p) {
   constexpr int OUTS = 8 * NT * FEW_COLS;
   __shared__ float red[FEW_WARPS][8 * NT][FEW_COLS + 1];
   __shared__ float sum[OUTS];
@@ -234,8 +235,9 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) dense_few_rows_kernel(const T*
 }
 
 // ---------------------------------------------------------------- rows with whole 16-byte pieces
-// Copies up to three matrices into rows whose stride is a multiple of 8 (what TMA reads), with zeros behind their columns. A
-// block takes whole rows, about ALIGN_VECTORS 16-byte pieces of them; a thread walks every 256th piece, four in flight.
+// Copies up to three matrices into rows whose stride is a multiple of 8 (what TMA reads), with zeros behind their
+// columns. A block takes whole rows, about ALIGN_VECTORS 16-byte pieces of them; a thread walks every 256th piece,
+// four in flight.
 struct AlignRows {
   const uint16_t* src[3];
   uint16_t* dst[3];
@@ -292,7 +294,7 @@ struct SlopeParams {
   void* dz;        long long lddz;      // nullptr: sums only
   float* sums;                          // [blocks / cols, N] or nullptr
   int M, N, act, lanes, rows_per_block;   // lanes: threads along a row, a power of two
-  int cols, blocks, align_blocks;         // blocks along a row; of dz and the sums; of each matrix that is copied besides
+  int cols, blocks, align_blocks;         // blocks along a row; of dz and the sums; of each matrix copied
 };
 
 template <typename T>

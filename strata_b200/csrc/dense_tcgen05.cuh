@@ -12,7 +12,8 @@
 //   epilogue  DENSE_Y: bias, activation, residual, one rounding; DENSE_Y_KEEP: z = x W^T + b besides;
 //             DENSE_PART: fp32 partial sums of a split contraction (DensePlan), which dense_finish_kernel adds up
 //             with the same epilogue.
-//   widths    Rows of y and z that TMA cannot store (it writes whole 16-byte pieces) are copied from the staging boxes by
+//   widths    Rows of y and z that TMA cannot store (it writes whole 16-byte pieces) are copied from the staging boxes
+// by
 //             the warps.
 #pragma once
 #include "dense_common.cuh"
@@ -36,15 +37,17 @@ struct DenseParams {
   int fp16;
   bool direct_out;              // out and keep are written by the warps, not by TMA
   float* part;                  // DENSE_PART: slabs of TILE_M x BN
-  const float* sums;            // column sums that dense_slope_kernel left, [sum_rows, sum_cols], or nullptr; added up into
+  const float* sums;            // column sums of dense_slope_kernel, [sum_rows, sum_cols], or nullptr; added up into
   int sum_rows, sum_cols;       //   db by epilogue warps that wait for their first tile
   float* db;
   DensePlan plan;
 };
 
-// db of eight columns: 256 threads, 32 rows of sums side by side, in a fixed order. `sync` is a barrier of those threads.
+// db of eight columns: 256 threads, 32 rows of sums side by side, in a fixed order. `sync` is a barrier of those
+// threads.
 template <typename Sync>
-__device__ __forceinline__ void dense_column_sums(const DenseParams& p, int group, int tid, float (*red)[9], Sync sync) {
+__device__ __forceinline__ void dense_column_sums(const DenseParams& p, int group, int tid, float (*red)[9],
+                                                  Sync sync) {
   const int col = group * 8 + (tid & 7), r0 = tid >> 3;
   float a = 0.f;
   if (col < p.sum_cols) {
@@ -101,17 +104,15 @@ __device__ __forceinline__ uint32_t dense_load_pair(const void* base, long long 
   const uint32_t lo = __ldg(p);
   return two ? lo | (static_cast<uint32_t>(__ldg(p + 1)) << 16) : lo;
 }
-// A warp's copy of a 32 x 32 staging box (64-byte rows and swizzle) to rows that TMA does not store: two rows at a time, 16
-// lanes with neighbouring pairs each.
+// A warp's copy of a 32 x 32 staging box (64-byte rows and swizzle) to rows that TMA does not store: two rows at a
+// time, 16 lanes with neighbouring pairs each.
 __device__ __forceinline__ void dense_copy_box(uint32_t box, void* base, long long ld, int m0, int n0, int M, int N) {
   const int lane = threadIdx.x & 31, j = lane & 15, col = n0 + 2 * j;
   uint32_t w[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    const int r = 2 * i + (lane >> 4);
-    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[i])
-                 : "r"(box + r * 64u + ((static_cast<uint32_t>(j >> 2) ^ static_cast<uint32_t>((r >> 1) & 3)) << 4) + (j & 3) * 4)
-                 : "memory");
+    const uint32_t r = 2 * i + (lane >> 4), piece = static_cast<uint32_t>(j >> 2) ^ ((r >> 1) & 3u);
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[i]) : "r"(box + r * 64u + (piece << 4) + (j & 3) * 4) : "memory");
   }
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
@@ -502,8 +503,8 @@ dense_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
 }
 
 // ---------------------------------------------------------------- the second half of a split product
-// Adds up a tile's slabs in the order of their slots and applies the epilogue. A thread has four columns of a row. Without
-// slabs: the column sums alone (db where no product is asked for).
+// Adds up a tile's slabs in the order of their slots and applies the epilogue. A thread has four columns of a row.
+// Without slabs: the column sums alone (db where no product is asked for).
 struct DenseFinish {
   DenseParams p;
   int tile_m, bn, tiles_n, blocks_per_tile;

@@ -8,11 +8,11 @@
 // and dy) and written once, in 16 bits; all arithmetic is fp32.
 //
 // A group of G lanes (a power of two, 8 channels each) has a head; a warp has a token, S = 32 / G heads of it at a time
-// (several tokens where both q and k have fewer heads than that), in steps of two rounds of q heads or of k heads. So the
-// token's table row is read and unpacked once for all its heads. A head whose width is no power of two leaves the group's
-// last lanes idle. What a step reads is asked for two steps ahead with cp.async into slots of shared memory that only the
-// asking lane reads: bytes in flight that cost no registers, and no barrier. Divisions by launch constants are
-// multiplications; arithmetic runs on fp32 pairs.
+// (several tokens where both q and k have fewer heads than that), in steps of two rounds of q heads or of k heads. So
+// the token's table row is read and unpacked once for all its heads. A head whose width is no power of two leaves the
+// group's last lanes idle. What a step reads is asked for two steps ahead with cp.async into slots of shared memory
+// that only the asking lane reads: bytes in flight that cost no registers, and no barrier. Divisions by launch
+// constants are multiplications; arithmetic runs on fp32 pairs.
 // Measured (8 + 8 heads of 64, 262144 tokens, bf16, half table; the bytes alone take 166 us forward, 250 backward):
 // forward 198 us, backward 292 (178 and 263 without rotation). With the loads straight into registers, two rounds of q
 // and two of k at a time: 190 and 355 (16 + 4 heads of 128: 303 against 248, 370 against 323); more blocks per SM at
@@ -72,8 +72,8 @@ __device__ __forceinline__ int qk_row(const QkParams& p, long long m) {
   return r < 0 ? -1 : static_cast<int>(r);
 }
 
-// (cos, sin) for this lane's channels 8 v .. 8 v + 7: four pairs where neighbours turn, else one for each channel; (1, 0)
-// where nothing turns. sin has the sign with which a pair's second channel enters its first: -1 forward, +1 for the
+// (cos, sin) for this lane's channels 8 v .. 8 v + 7: four pairs where neighbours turn, else one for each channel; (1,
+// 0) where nothing turns. sin has the sign with which a pair's second channel enters its first: -1 forward, +1 for the
 // inverse turn; for channels of the second half the other sign.
 // raw: the lane's part of the table row, TV 16-byte vectors.
 template <int TAB, bool ADJ>
@@ -111,8 +111,8 @@ __device__ __forceinline__ void qk_table(const QkParams& p, const uint4 (&raw)[T
   }
 }
 
-// A lane's eight channels as four fp32 pairs. Where neighbours turn the pairs are (0, 2), (4, 6), (1, 3), (5, 7), so that the
-// rotation multiplies whole pairs: even' = even c + odd s, odd' = odd c - even s; else (0, 1), (2, 3), ...
+// A lane's eight channels as four fp32 pairs. Where neighbours turn the pairs are (0, 2), (4, 6), (1, 3), (5, 7), so
+// that the rotation multiplies whole pairs: even' = even c + odd s, odd' = odd c - even s; else (0, 1), (2, 3), ...
 template <bool ADJ>
 __device__ constexpr int qk_first(int i) { return ADJ ? (i & 1) * 4 + (i >> 1) : 2 * i; }
 template <bool ADJ>
@@ -219,10 +219,12 @@ __device__ __forceinline__ uint4 qk_vector(const uint4& xr, const uint4& gr, con
   }
 }
 
-// Weights of this lane's channels. (Read again for every token, from L1: registers that the loop does not have to keep.)
+// Weights of this lane's channels. (Read again for every token, from L1: registers that the loop does not have to
+// keep.)
 __device__ __forceinline__ void qk_weights(const float* w, int v, float (&o)[8]) {
   if (w != nullptr) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(w) + 2 * v), b = __ldg(reinterpret_cast<const float4*>(w) + 2 * v + 1);
+    const float4* f = reinterpret_cast<const float4*>(w) + 2 * v;
+    const float4 a = __ldg(f), b = __ldg(f + 1);
     o[0] = a.x; o[1] = a.y; o[2] = a.z; o[3] = a.w; o[4] = b.x; o[5] = b.y; o[6] = b.z; o[7] = b.w;
   } else {
 #pragma unroll
@@ -230,13 +232,15 @@ __device__ __forceinline__ void qk_weights(const float* w, int v, float (&o)[8])
   }
 }
 
-// Bytes a lane asks for ahead, past the registers: into its own 16-byte slots of shared memory (zeros where on is false).
+// Bytes a lane asks for ahead, past the registers: into its own 16-byte slots of shared memory (zeros where on is
+// false).
 __device__ __forceinline__ void qk_ask(uint32_t slot, const void* src, bool on) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot), "l"(src), "r"(on ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ uint4 qk_got(uint32_t slot) {
   uint4 u;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(slot) : "memory");
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(slot) : "memory");
   return u;
 }
 
@@ -291,7 +295,8 @@ __global__ void __launch_bounds__(256, GRAD ? 2 : 4) qk_norm_rope_kernel(const Q
       if (TAB != QK_NO_TABLE && k_a == 0 && h_a == 0) {
         if (m >= M) row_a = -1;
         const bool on = turns && row_a >= 0;
-        const long long e = (on ? static_cast<long long>(row_a) * (p.rot >> 1) : 0) + (turns ? qk_entry<ADJ>(p, v_raw) : 0);
+        const long long e =
+            (on ? static_cast<long long>(row_a) * (p.rot >> 1) : 0) + (turns ? qk_entry<ADJ>(p, v_raw) : 0);
         const char* src = static_cast<const char*>(p.table) + e * (TAB == QK_F32_TABLE ? 8 : 4);
 #pragma unroll
         for (int i = 0; i < TV; ++i) qk_ask(slot + ((GRAD ? 2 : 1) * R + i) * 512, src + i * 16, on);
@@ -334,7 +339,8 @@ __global__ void __launch_bounds__(256, GRAD ? 2 : 4) qk_norm_rope_kernel(const Q
           for (int i = 0; i < TV; ++i) raw[i] = qk_got(slot + ((GRAD ? 2 : 1) * R + i) * 512);
           asm volatile("ld.shared.b32 %0, [%1];" : "=r"(row) : "r"(rows + stage * Ring::STAGE) : "memory");
           if (row == -2) atomicCAS(&g_status, 0, ST_BAD_POSITION);
-          if constexpr (TAB != QK_NO_TABLE) qk_table<TAB, ADJ>(p, raw, turns && row >= 0, v_raw, GRAD ? 1.f : -1.f, c, s);
+          if constexpr (TAB != QK_NO_TABLE)
+            qk_table<TAB, ADJ>(p, raw, turns && row >= 0, v_raw, GRAD ? 1.f : -1.f, c, s);
         }
         float w[8];
         qk_weights(p.w[k], v, w);
@@ -343,8 +349,8 @@ __global__ void __launch_bounds__(256, GRAD ? 2 : 4) qk_norm_rope_kernel(const Q
           if (r > 0 && h0 + r * width >= p.heads[k]) continue;       // (the same for the launch)
           const int h = h0 + r * width + head;
           const uint4 xr = qk_got(slot + r * 512), gr = GRAD ? qk_got(slot + (R + r) * 512) : xr;
-          uint4 o = qk_vector<T, G, TAB, ADJ, GRAD>(xr, gr, w, c, s, partner, TAB == QK_NO_TABLE || row >= 0, inv, p.eps,
-                                                   sums[k]);
+          uint4 o = qk_vector<T, G, TAB, ADJ, GRAD>(xr, gr, w, c, s, partner, TAB == QK_NO_TABLE || row >= 0, inv,
+                                                   p.eps, sums[k]);
           if (TAB != QK_NO_TABLE && p.positions != nullptr && row < 0) {     // padding: zero; behind the table: NaN
             const uint32_t u = row == -1 ? 0u : 0x7FFF7FFFu;
             o = make_uint4(u, u, u, u);

@@ -275,7 +275,7 @@ def test_projection_norm_attention_projection(ops):
     x, wqkv, bqkv = n(M, C).to(BF), (n(3 * C, C) * C ** -0.5).to(BF), n(3 * C) * 0.1
     wp, bp = (n(C, C) * C ** -0.5).to(BF), n(C) * 0.1
     cs = d["cs"].view(tiles, H * W, 32, 2)
-    grid = lambda t: t.view(tiles, D, H, W, heads, 64)
+    grid = lambda t: t.reshape(tiles, D, H, W, heads, 64)
 
     def half(q, k, v):
         a = ops.na3d(grid(q), grid(k), grid(v), (3, 3, 3))
@@ -284,7 +284,7 @@ def test_projection_norm_attention_projection(ops):
     qkv = ops.linear_act(x, wqkv, bqkv)
     q, k = ops.qk_norm_rope(*(t.view(M, heads, 64) for t in (qkv[:, :C], qkv[:, C:2 * C])), rope_cs=cs, tokens_per_tile=T,
                             hw=H * W)
-    got = half(q, k, qkv[:, 2 * C:].contiguous())
+    got = half(q, k, qkv[:, 2 * C:])
     fused = ops.qkv_rope(x, wqkv, bqkv, 64, None, None, T, H * W, qk_norm=True, rope_cs=cs)
     want = half(*(fused[:, i * C:(i + 1) * C].contiguous() for i in range(3)))
     # q and k carry one more rounding (2^-8 at most); their scores, and so the result, move by a few times that

@@ -189,6 +189,8 @@ class DistributedTileCopyHaloPadding(torch.nn.Module):
         failed barrier is NaN, so a missed poll cannot let a rollout continue on stale halos."""
         st = _lib.device_status()
         if st != 0:
+            if st == 107:      # not of an exchange, but the first thing that went wrong
+                raise RuntimeError("a position given to ops.qk_norm_rope lies behind its table (device status 107)")
             raise RuntimeError(f"halo exchange failed on the device (status {st}: "
                                f"{'peer flag wait timed out' if st == 105 else 'kernel wait timed out'})")
 

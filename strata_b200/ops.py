@@ -226,6 +226,8 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
         _like(out, "out", x)
         if out.shape != (M, N) or (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
             raise ValueError(f"out must be [{M}, {N}] with unit inner stride")
+        if out.data_ptr() in (x2.data_ptr(), w2.data_ptr()) and M:
+            raise ValueError("out may be the residual, but not x or weight")
         y, ldy = out, out.stride(0) if M > 1 else N
     z, ldz = _padded_rows(x, shape) if save_preact else (None, 0)
     if M:

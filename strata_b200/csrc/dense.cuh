@@ -93,6 +93,12 @@ inline DenseChoice dense_choice(int M, int N, int K, int sms) {
 // ---------------------------------------------------------------- launches
 struct DenseOperand { const void* p; long long ld; };
 
+// Units that a product's kernel runs on, and its blocks.
+inline int dense_grid(int tiles, int units, bool split) { return split || tiles >= units ? units : tiles; }
+inline int dense_blocks(const DenseChoice& c) {
+  return dense_grid(c.plan.tiles, c.plan.units, c.split) * (c.bn == 256 ? 2 : 1);
+}
+
 template <int BN, bool PAIR, int LAY, int EPI, typename T, int ACT = ACT_ANY, bool AUX = false>
 inline int launch_dense_t(const DenseOperand& A, const DenseOperand& B, const DenseParams& p, int units,
                           cudaStream_t st) {
@@ -125,7 +131,7 @@ inline int launch_dense_t(const DenseOperand& A, const DenseOperand& B, const De
   const int tiles = ((p.M + TILE_M - 1) / TILE_M) * ((p.N + BN - 1) / BN);
   // a split's units are its plan's: blocks that are not resident at once run one after the other, none waits
   // for another
-  int grid = EPI == DENSE_PART || tiles >= units ? units : tiles;
+  const int grid = dense_grid(tiles, units, EPI == DENSE_PART);
   return launch_chained(kern, dim3(static_cast<unsigned>(PAIR ? 2 * grid : grid)), GEMM_THREADS, S::TOTAL, st,
                         PAIR ? 2 : 1, tmA, tmB, tmOut, tmKeep, tmAux, p);
 }
@@ -368,7 +374,7 @@ inline DenseGradPlan dense_grad_plan(int M, int N, int K, bool act, bool dy_ok, 
   if (g.make_dz) g.dz = ws.take(2 * dense_round8(N) * M);
   if (g.copy_x) g.xs = ws.take(2 * dense_round8(K) * M);
   if (g.copy_w) g.ws = ws.take(2 * dense_round8(K) * N);
-  if (db) g.col_sums = static_cast<float*>(ws.take(4LL * g.sums.blocks * N));
+  if (db && g.sums.blocks > 1) g.col_sums = static_cast<float*>(ws.take(4LL * g.sums.blocks * N));
   const int64_t sx = g.cx.slab_bytes(), sw = g.cw.slab_bytes();
   g.slabs = ws.take(sx > sw ? sx : sw);        // one after the other on the stream
   g.bytes = ws.used;
@@ -386,7 +392,7 @@ inline int launch_dense_backward(const DenseGradParams& q, const DenseGradPlan& 
     s.dy = q.dy.p; s.ldy = q.dy.ld;
     s.z = q.z.p; s.ldz = q.z.ld;
     s.dz = g.make_dz ? g.dz : nullptr; s.lddz = dense_round8(q.N);
-    s.sums = g.col_sums;
+    s.sums = g.sums.blocks == 1 ? q.db : g.col_sums;
     s.M = q.M; s.N = q.N; s.act = q.act; s.lanes = g.sums.lanes; s.rows_per_block = g.sums.rows_per_block;
     s.cols = g.sums.cols;
     s.blocks = g.make_dz || q.db ? g.sums.cols * g.sums.blocks : 0;
@@ -398,16 +404,26 @@ inline int launch_dense_backward(const DenseGradParams& q, const DenseGradPlan& 
     if (r != 0) return r;
     if (g.make_dz) dz = {g.dz, dense_round8(q.N)};
   }
-  // db is added up by the first product's kernel
+  // db is added up by the first product's kernel, unless the product has too few blocks for it (2 x 16 x 472: 31 us in
+  // the one block of dx, 4 in a kernel of its own). The sums of a single block of rows are db.
   auto sums = [&](DenseParams& p) {
     p.sums = g.col_sums; p.sum_rows = g.sums.blocks; p.sum_cols = q.N; p.db = q.db;
   };
+  const int groups = q.db && g.sums.blocks > 1 ? (q.N + 7) / 8 : 0;
+  const bool in_dx = q.dx && groups > 0 && groups <= 4 * dense_blocks(g.cx);
+  const bool in_dw = !q.dx && q.dw && groups > 0 && groups <= 4 * dense_blocks(g.cw);
+  if (groups > 0 && !in_dx && !in_dw) {
+    DenseFinish f{};
+    sums(f.p);
+    f.p.fp16 = q.fp16;
+    if ((r = launch_dense_finish(f, st)) != 0) return r;
+  }
   if (q.dx) {
     DenseParams p{};
     p.M = q.M; p.N = q.K; p.K = q.N;
     p.out = q.dx; p.ldo = q.lddx; p.fp16 = q.fp16;
     p.direct_out = !dense_whole(q.dx, q.lddx, q.K, q.padded);
-    if (q.db) sums(p);
+    if (in_dx) sums(p);
     if ((r = launch_dense<DENSE_NN>(dz, w, p, g.cx, g.slabs, st)) != 0) return r;
   }
   if (q.dw) {
@@ -415,13 +431,8 @@ inline int launch_dense_backward(const DenseGradParams& q, const DenseGradPlan& 
     p.M = q.N; p.N = q.K; p.K = q.M;
     p.out = q.dw; p.ldo = q.lddw; p.fp16 = q.fp16;
     p.direct_out = !dense_whole(q.dw, q.lddw, q.K, false);
-    if (q.db && !q.dx) sums(p);
+    if (in_dw) sums(p);
     return launch_dense<DENSE_TN>(dz, x, p, g.cw, g.slabs, st);
-  }
-  if (q.db && !q.dx) {
-    DenseFinish f{};
-    sums(f.p);
-    return launch_dense_finish(f, st);
   }
   return 0;
 }

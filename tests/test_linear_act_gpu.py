@@ -142,6 +142,26 @@ def test_backward(ops, M, N, K, t):
     assert _lib.device_status() == 0
 
 
+# db where one block of rows has it whole, in the blocks of a product, and where the product has too few of them
+@pytest.mark.parametrize("M,N,K", [(2, 472, 16), (64, 4000, 8), (600, 472, 16), (3000, 4001, 8), (3000, 40, 8)])
+def test_bias_gradient_with_few_blocks(ops, M, N, K):
+    d = data(M, N, K, BF, seed=M)
+    for act in ("none", "silu"):
+        z = ops.linear_act(d["x"], d["w"], d["b"], "none")
+        got = ops.linear_act_backward(d["dy"], d["x"], d["w"], act, z)
+        check_backward(got, d, z, act)
+        for nx, nw in ((False, False), (True, False), (False, True)):
+            part = ops.linear_act_backward(d["dy"], d["x"], d["w"], act, z, need_x=nx, need_weight=nw)
+            assert torch.equal(part[2], got[2])
+
+
+def test_out_may_not_be_an_operand(ops):
+    d = data(64, 64, 64, BF)
+    for out in (d["x"], d["w"]):
+        with pytest.raises(ValueError, match="not x or weight"):
+            ops.linear_act(d["x"], d["w"], d["b"], "gelu", out=out)
+
+
 def test_gradients_are_the_forward_pass_differences():
     """The 64-bit gradients that the kernels are held to, against central differences of the 64-bit forward formula."""
     g = torch.Generator("cuda").manual_seed(0)

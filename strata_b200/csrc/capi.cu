@@ -1035,15 +1035,15 @@ int strata_qk_norm_rope(const void* q, int64_t q_st, int64_t q_sh, const void* k
   const int r = qk_params(p, heads_q, heads_k, head_dim, rot, adjacent, table, table_f32, table_rows, positions,
                           positions_64, tokens_per_tile, hw, M, eps, dtype);
   if (r != STRATA_OK) return r;
-  return launch_qk<false>(p, adjacent != 0, dtype == STRATA_F16, qk_blocks(M, false, sms),
-                          as_stream(stream));
+  const dim3 grid = qk_grid(p, false, sms);
+  return launch_qk<false>(p, adjacent != 0, dtype == STRATA_F16, grid, as_stream(stream));
 }
 
 int64_t strata_qk_norm_rope_backward_workspace_bytes(int64_t M, int head_dim) {
   const int sms = current_sm_count();
   if (sms <= 0) return STRATA_ERR_NO_DEVICE;
   if (M < 0 || M > 0x7FFF0000 || head_dim <= 0 || head_dim > 256) return STRATA_ERR_ARG;
-  return static_cast<int64_t>(qk_blocks(M, true, sms)) * 2 * head_dim * 4;
+  return M == 0 ? 0 : qk_most_blocks(true, sms) * 2 * head_dim * 4;
 }
 
 int strata_qk_norm_rope_backward(const void* dyq, int64_t dyq_st, int64_t dyq_sh, const void* dyk, int64_t dyk_st,
@@ -1073,13 +1073,14 @@ int strata_qk_norm_rope_backward(const void* dyq, int64_t dyq_st, int64_t dyq_sh
                     tokens_per_tile, hw, M, eps, dtype);
   if (r != STRATA_OK) return r;
   if (!qk_heads_ok(p.dy[0]) || !qk_heads_ok(p.dy[1])) return STRATA_ERR_ARG;
-  const int blocks = qk_blocks(M, true, sms);
+  const dim3 grid = qk_grid(p, true, sms);
+  const int blocks = static_cast<int>(grid.x * grid.y);
   if (dw_q || dw_k) {
     if (!workspace || !aligned16(workspace) || workspace_bytes < static_cast<int64_t>(blocks) * 2 * head_dim * 4)
        return STRATA_ERR_ARG;
     p.partial = static_cast<float*>(workspace);
   }
-  r = launch_qk<true>(p, adjacent != 0, dtype == STRATA_F16, blocks, st);
+  r = launch_qk<true>(p, adjacent != 0, dtype == STRATA_F16, grid, st);
   if (r != 0 || !p.partial) return r;
   return launch_chained(qk_weight_grad_kernel, dim3(2 * head_dim / 8), 256, 0, st, 1,
                         static_cast<const float*>(p.partial), blocks, head_dim, dw_q, dw_k);

@@ -47,6 +47,7 @@ struct QkParams {
   QkTensor dy[2];                     // backward
   const float* w[2];                  // [head_dim] or nullptr
   int heads[2];
+  int part[2];                        // heads of a block: block (x, y) has those from y part on
   int head_dim, rot;
   const void* table;                  // [rows, rot / 2] (cos, sin) pairs, half or float; nullptr: no rotation
   int table_f32, table_rows;
@@ -252,9 +253,10 @@ struct QkRing {
   static constexpr int BYTES = 8 * STAGES * STAGE;
 };
 
-// GRAD false: y; true: dx and the sums of dw. Blocks of 256 threads, a stride loop over the tokens; a step is
+// SPLIT: a token's heads go to the blocks of a grid column (a kernel of its own: with its limits in registers the loop
+// over many tokens is 5 to 11 % slower). GRAD false: y; true: dx and the sums of dw. Blocks of 256 threads, a stride loop over the tokens; a step is
 // QK_ROUNDS rounds of a token's q heads or k heads, asked for STAGES - 1 steps ahead.
-template <typename T, int G, int TAB, bool ADJ, bool GRAD>
+template <typename T, int G, int TAB, bool ADJ, bool GRAD, bool SPLIT>
 __global__ void __launch_bounds__(256, GRAD ? 2 : 4) qk_norm_rope_kernel(const QkParams p) {
   using Ring = QkRing<TAB, ADJ, GRAD>;
   constexpr int S = 32 / G, R = QK_ROUNDS, N = QkTab<TAB, ADJ>::N, TV = QkTab<TAB, ADJ>::TV, D = Ring::STAGES;
@@ -270,8 +272,14 @@ __global__ void __launch_bounds__(256, GRAD ? 2 : 4) qk_norm_rope_kernel(const Q
   const uint32_t rows = smem_u32(ring) + (threadIdx.x >> 5) * (D * Ring::STAGE) + Ring::VECTORS * 512 + lane * 4;
   // heads side by side in the warp, and the tokens that leaves room for
   int width = 1;
-  while (width < S && (width < p.heads[0] || width < p.heads[1])) width *= 2;
+  while (width < S && (width < p.part[0] || width < p.part[1])) width *= 2;
   const int tokens = S / width, head = sub & (width - 1), tok = sub / width;
+  // the block's heads: lim of them from base on (none: lim <= 0)
+  const int part = SPLIT ? blockIdx.y : 0;
+  const int lim_q = SPLIT ? min(p.heads[0] - part * p.part[0], p.part[0]) : 0;
+  const int lim_k = SPLIT ? min(p.heads[1] - part * p.part[1], p.part[1]) : 0;
+  auto base = [&](int k) { return SPLIT ? part * p.part[k] : 0; };
+  auto lim = [&](int k) { return !SPLIT ? p.heads[k] : k == 0 ? lim_q : lim_k; };
   const uint32_t M = static_cast<uint32_t>(p.M), stride = gridDim.x * (blockDim.x >> 5) * tokens;
   const uint32_t first = (blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * tokens;
   auto at = [&](const QkTensor& t, uint32_t m, int h) {
@@ -288,9 +296,9 @@ __global__ void __launch_bounds__(256, GRAD ? 2 : 4) qk_norm_rope_kernel(const Q
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         const int h = h_a + r * width + head;
-        const bool on = lane_on && m < M && h < p.heads[k_a];
-        qk_ask(slot + r * 512, at(p.x[k_a], on ? m : 0, on ? h : 0), on);
-        if constexpr (GRAD) qk_ask(slot + (R + r) * 512, at(p.dy[k_a], on ? m : 0, on ? h : 0), on);
+        const bool on = lane_on && m < M && h < lim(k_a);
+        qk_ask(slot + r * 512, at(p.x[k_a], on ? m : 0, on ? base(k_a) + h : 0), on);
+        if constexpr (GRAD) qk_ask(slot + (R + r) * 512, at(p.dy[k_a], on ? m : 0, on ? base(k_a) + h : 0), on);
       }
       if (TAB != QK_NO_TABLE && k_a == 0 && h_a == 0) {
         if (m >= M) row_a = -1;
@@ -303,7 +311,7 @@ __global__ void __launch_bounds__(256, GRAD ? 2 : 4) qk_norm_rope_kernel(const Q
         asm volatile("st.shared.b32 [%0], %1;" ::"r"(rows + stage_a * Ring::STAGE), "r"(row_a) : "memory");
         if (m + stride < M) row_a = qk_row(p, m + stride);       // (the next token's, a token ahead)
       }
-      if ((h_a += R * width) >= p.heads[k_a]) {
+      if ((h_a += R * width) >= lim(k_a)) {
         h_a = 0;
         if (++k_a == 2) {
           k_a = 0;
@@ -329,7 +337,7 @@ __global__ void __launch_bounds__(256, GRAD ? 2 : 4) qk_norm_rope_kernel(const Q
     float c[N], s[N];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      for (int h0 = 0; h0 < p.heads[k]; h0 += R * width) {
+      for (int h0 = 0; (SPLIT && h0 == 0) || h0 < lim(k); h0 += R * width) {     // (a part without k heads: an empty step)
         ask();
         asm volatile("cp.async.wait_group %0;" ::"n"(D - 1) : "memory");
         const uint32_t slot = slots + stage * Ring::STAGE;
@@ -346,7 +354,7 @@ __global__ void __launch_bounds__(256, GRAD ? 2 : 4) qk_norm_rope_kernel(const Q
         qk_weights(p.w[k], v, w);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          if (r > 0 && h0 + r * width >= p.heads[k]) continue;       // (the same for the launch)
+          if (r > 0 && h0 + r * width >= lim(k)) continue;       // (the same for the block)
           const int h = h0 + r * width + head;
           const uint4 xr = qk_got(slot + r * 512), gr = GRAD ? qk_got(slot + (R + r) * 512) : xr;
           uint4 o = qk_vector<T, G, TAB, ADJ, GRAD>(xr, gr, w, c, s, partner, TAB == QK_NO_TABLE || row >= 0, inv,
@@ -355,7 +363,7 @@ __global__ void __launch_bounds__(256, GRAD ? 2 : 4) qk_norm_rope_kernel(const Q
             const uint32_t u = row == -1 ? 0u : 0x7FFF7FFFu;
             o = make_uint4(u, u, u, u);
           }
-          if (lane_on && m < M && h < p.heads[k]) *reinterpret_cast<uint4*>(at(p.y[k], m, h)) = o;
+          if (lane_on && m < M && h < lim(k)) *reinterpret_cast<uint4*>(at(p.y[k], m, base(k) + h)) = o;
         }
         stage = stage + 1 == D ? 0 : stage + 1;
       }
@@ -386,7 +394,7 @@ __global__ void __launch_bounds__(256, GRAD ? 2 : 4) qk_norm_rope_kernel(const Q
       float t = 0.f;
 #pragma unroll
       for (int w = 0; w < 8; ++w) t += red[(w * 2 + k) * (G * 8) + ch];
-      p.partial[static_cast<long long>(blockIdx.x) * 2 * p.head_dim + i] = t;
+      p.partial[(static_cast<long long>(part) * gridDim.x + blockIdx.x) * 2 * p.head_dim + i] = t;
     }
   }
 }
@@ -418,43 +426,64 @@ inline int qk_group(int head_dim) {      // (16 channels in two lanes are no nar
   return g;
 }
 // A token a warp: no more blocks than that takes, and no more than run at once backward (a row of sums each).
-inline int qk_blocks(long long M, bool grad, int sms) {
-  const long long blocks = (M + 7) / 8, cap = static_cast<long long>(sms) * (grad ? 2 : 16);
-  return static_cast<int>(blocks < cap ? blocks : cap);
+inline long long qk_most_blocks(bool grad, int sms) { return static_cast<long long>(sms) * (grad ? 2 : 16); }
+// Grid for p's tokens and heads; sets p.part. Where the tokens leave room for that, a token's heads go to several
+// blocks, down to one round of q heads each (44 tokens, 48 + 12 heads of 256, in a row of calls: forward 29.3 us -> 13.0,
+// backward 38.7 -> 16.7; from 300 tokens of 12 + 12 heads of 64 on no difference).
+inline dim3 qk_grid(QkParams& p, bool grad, int sms) {
+  const long long blocks = (p.M + 7) / 8, cap = qk_most_blocks(grad, sms);
+  p.part[0] = p.heads[0];
+  p.part[1] = p.heads[1];
+  const int side = 32 / qk_group(p.head_dim);
+  long long parts = 2LL * sms / blocks;
+  if (parts > (p.heads[0] + side - 1) / side) parts = (p.heads[0] + side - 1) / side;
+  if (parts > 1) {
+    p.part[0] = static_cast<int>((p.heads[0] + parts - 1) / parts);
+    parts = (p.heads[0] + p.part[0] - 1) / p.part[0];
+    p.part[1] = static_cast<int>((p.heads[1] + parts - 1) / parts);
+  } else {
+    parts = 1;
+  }
+  return dim3(static_cast<unsigned>(blocks < cap ? blocks : cap), static_cast<unsigned>(parts));
 }
 
-template <typename T, int G, int TAB, bool ADJ, bool GRAD>
-inline int launch_qk_k(const QkParams& p, int blocks, cudaStream_t st) {
-  auto kern = qk_norm_rope_kernel<T, G, TAB, ADJ, GRAD>;
+template <typename T, int G, int TAB, bool ADJ, bool GRAD, bool SPLIT>
+inline int launch_qk_s(const QkParams& p, dim3 grid, cudaStream_t st) {
+  auto kern = qk_norm_rope_kernel<T, G, TAB, ADJ, GRAD, SPLIT>;
   constexpr int bytes = QkRing<TAB, ADJ, GRAD>::BYTES;
   static_assert(bytes >= 8 * 2 * G * 8 * 4, "the sums of a block");
   static std::atomic<uint64_t> smem_set;
   if (const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), bytes, smem_set); e != cudaSuccess)
     return -static_cast<int>(e) - 1000;
-  return launch_chained(kern, dim3(static_cast<unsigned>(blocks)), 256, bytes, st, 1, p);
+  return launch_chained(kern, grid, 256, bytes, st, 1, p);
+}
+template <typename T, int G, int TAB, bool ADJ, bool GRAD>
+inline int launch_qk_k(const QkParams& p, dim3 grid, cudaStream_t st) {
+  return grid.y > 1 ? launch_qk_s<T, G, TAB, ADJ, GRAD, true>(p, grid, st)
+                    : launch_qk_s<T, G, TAB, ADJ, GRAD, false>(p, grid, st);
 }
 template <typename T, int G, bool GRAD>
-inline int launch_qk_t(const QkParams& p, bool adjacent, int blocks, cudaStream_t st) {
-  if (p.table == nullptr) return launch_qk_k<T, G, QK_NO_TABLE, true, GRAD>(p, blocks, st);
+inline int launch_qk_t(const QkParams& p, bool adjacent, dim3 grid, cudaStream_t st) {
+  if (p.table == nullptr) return launch_qk_k<T, G, QK_NO_TABLE, true, GRAD>(p, grid, st);
   if (p.table_f32)
-    return adjacent ? launch_qk_k<T, G, QK_F32_TABLE, true, GRAD>(p, blocks, st)
-                    : launch_qk_k<T, G, QK_F32_TABLE, false, GRAD>(p, blocks, st);
-  return adjacent ? launch_qk_k<T, G, QK_HALF_TABLE, true, GRAD>(p, blocks, st)
-                  : launch_qk_k<T, G, QK_HALF_TABLE, false, GRAD>(p, blocks, st);
+    return adjacent ? launch_qk_k<T, G, QK_F32_TABLE, true, GRAD>(p, grid, st)
+                    : launch_qk_k<T, G, QK_F32_TABLE, false, GRAD>(p, grid, st);
+  return adjacent ? launch_qk_k<T, G, QK_HALF_TABLE, true, GRAD>(p, grid, st)
+                  : launch_qk_k<T, G, QK_HALF_TABLE, false, GRAD>(p, grid, st);
 }
 template <typename T, bool GRAD>
-inline int launch_qk_g(const QkParams& p, bool adjacent, int blocks, cudaStream_t st) {
+inline int launch_qk_g(const QkParams& p, bool adjacent, dim3 grid, cudaStream_t st) {
   switch (qk_group(p.head_dim)) {
-    case 4: return launch_qk_t<T, 4, GRAD>(p, adjacent, blocks, st);
-    case 8: return launch_qk_t<T, 8, GRAD>(p, adjacent, blocks, st);
-    case 16: return launch_qk_t<T, 16, GRAD>(p, adjacent, blocks, st);
-    default: return launch_qk_t<T, 32, GRAD>(p, adjacent, blocks, st);
+    case 4: return launch_qk_t<T, 4, GRAD>(p, adjacent, grid, st);
+    case 8: return launch_qk_t<T, 8, GRAD>(p, adjacent, grid, st);
+    case 16: return launch_qk_t<T, 16, GRAD>(p, adjacent, grid, st);
+    default: return launch_qk_t<T, 32, GRAD>(p, adjacent, grid, st);
   }
 }
 template <bool GRAD>
-inline int launch_qk(const QkParams& p, bool adjacent, bool fp16, int blocks, cudaStream_t st) {
-  return fp16 ? launch_qk_g<__half, GRAD>(p, adjacent, blocks, st)
-              : launch_qk_g<__nv_bfloat16, GRAD>(p, adjacent, blocks, st);
+inline int launch_qk(const QkParams& p, bool adjacent, bool fp16, dim3 grid, cudaStream_t st) {
+  return fp16 ? launch_qk_g<__half, GRAD>(p, adjacent, grid, st)
+              : launch_qk_g<__nv_bfloat16, GRAD>(p, adjacent, grid, st);
 }
 
 }  // namespace strata

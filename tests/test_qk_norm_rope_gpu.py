@@ -120,6 +120,20 @@ def test_by_position(ops, M, hq, hk, hd, rot, adjacent, t, f32, weights):
     assert _lib.device_status() == 0
 
 
+# few tokens: a token's heads over several blocks, also where the last ones have no k heads, or no whole share
+@pytest.mark.parametrize("M,hq,hk,hd", [(1, 48, 12, 256), (44, 48, 12, 256), (5, 48, 1, 128), (9, 3, 40, 64), (300, 13, 7, 64),
+                                        (1100, 17, 3, 200), (2, 1000, 999, 8)])
+@pytest.mark.parametrize("adjacent", [True, False])
+def test_heads_over_several_blocks(ops, M, hq, hk, hd, adjacent):
+    d = data(M, hq, hk, hd, BF, rot=hd if adjacent else hd // 16 * 16 or None, rows=M, f32=True, seed=M + hq)
+    at = torch.arange(M - 1, -1, -1, device="cuda")
+    live = at != M // 2 if M > 2 else torch.ones_like(at, dtype=torch.bool)
+    if d["cs"] is None:
+        check(ops, d, adjacent)
+    else:
+        check(ops, d, adjacent, at, live, positions=torch.where(live, at, -1))
+
+
 @pytest.mark.parametrize("tiles,depth,hw", [(1, 1, 1), (3, 4, 50), (2, 16, 33)])
 def test_by_tile_and_cell(ops, tiles, depth, hw):
     M = tiles * depth * hw

@@ -49,8 +49,9 @@ inline int dense_pairs(int sms) {
 }
 
 // The cheapest form by a model of each one's time, in microseconds: a k-block of 64 on one unit, the part of a tile's
-// epilogue that nothing hides, a launch, and a slab's way to memory and back. Some of the shapes it was checked on,
-// tiles of 64 / 128 / 256 unsplit, then split (the one taken in brackets):
+// epilogue that nothing hides, a launch, and a slab's way to memory and back. On 210 random products (40 to 100000 rows,
+// widths from 32 to 4000) the form it takes was within 1 % of the fastest on average, within 30 % in all. Some of the
+// shapes it was checked on, tiles of 64 / 128 / 256 unsplit, then split (the one taken in brackets):
 //   y   64 x 1024, K = 4096    12.0 / 13.5 / 23.3   [7.4] / 10.6 / 12.3
 //   y   2500 x 650, K = 207    6.6 / [5.9] / 7.2    (no split: enough tiles, four k-blocks)
 //   y   98304 x 512, K = 2048  255 / 187 / [153]    371 / 296 / 249
@@ -64,7 +65,7 @@ inline DenseChoice dense_choice(int M, int N, int K, int sms) {
   double best_us = 0.0;
   for (int bn = 64; bn <= 256; bn *= 2) {
     const int units = bn == 256 ? dense_pairs(sms) : sms, tiles = dense_tiles(M, N, bn);
-    const double kb_us = bn == 256 ? 0.27 : bn == 128 ? 0.19 : 0.15;
+    const double kb_us = bn == 256 ? 0.25 : bn == 128 ? 0.20 : 0.15;
     const double tile_us = bn == 256 ? 1.6 : bn == 128 ? 1.0 : 0.8;     // epilogue that nothing hides
     const int turns = (tiles + units - 1) / units;
     const double us = turns * (num_kb * kb_us > tile_us ? num_kb * kb_us : tile_us) + tile_us + 2.0;
@@ -81,7 +82,7 @@ inline DenseChoice dense_choice(int M, int N, int K, int sms) {
     const double rows = static_cast<double>(M < tm ? M : tm) / tm;       // of a slab that exist
     const double slab_mb = s.slots() * rows * tm * bn * 4e-6;
     const int kbs = s.whole / units * num_kb + s.head;
-    const double split_us = kbs * kb_us + 2 * tile_us + 2.0 + 3.0 + slab_mb * 2 / 5.0;
+    const double split_us = kbs * kb_us + tile_us + 2.0 + 1.7 + slab_mb * 2 / 6.0;
     if (split_us < 0.95 * best_us) {
       best = DenseChoice{bn, true, s};
       best_us = split_us;
@@ -91,7 +92,11 @@ inline DenseChoice dense_choice(int M, int N, int K, int sms) {
 }
 
 // ---------------------------------------------------------------- launches
-struct DenseOperand { const void* p; long long ld; };
+struct DenseOperand {
+  const void* p;
+  long long ld;
+  int readable = 0;      // columns that exist in memory, where they are more than the operand's (0: no more)
+};
 
 // Units that a product's kernel runs on, and its blocks.
 inline int dense_grid(int tiles, int units, bool split) { return split || tiles >= units ? units : tiles; }
@@ -105,14 +110,18 @@ inline int launch_dense_t(const DenseOperand& A, const DenseOperand& B, const De
   const bool a_mn = LAY == DENSE_TN, b_mn = LAY != DENSE_NT;
   constexpr int TILE_M = PAIR ? 2 * GEMM_BM : GEMM_BM;
   CUtensorMap tmA, tmB, tmOut, tmKeep, tmAux;
+  // (a box that a row ends in costs up to twice a whole one where the columns are the tile's rows or columns: there the
+  // map has all that exist, and what they hold stays in outputs that nobody stores)
+  auto mn_cols = [](const DenseOperand& o, int cols) { return o.readable > cols ? o.readable : cols; };
   auto map = [](CUtensorMap* tm, const DenseOperand& o, int rows, int cols, uint32_t bx, uint32_t by, TmapSwizzle sw) {
     const uint64_t dims[2] = {static_cast<uint64_t>(cols), static_cast<uint64_t>(rows)};
     const uint64_t str[1] = {static_cast<uint64_t>(o.ld) * 2};
     const uint32_t box[2] = {bx, by};
     return make_tmap_bf16(tm, o.p, 2, dims, str, box, sw);      // (either 16-bit type: nothing is converted)
   };
-  if (map(&tmA, A, a_mn ? p.K : p.M, a_mn ? p.M : p.K, 64, a_mn ? 64 : GEMM_BM, TMAP_SWIZZLE_128B) != 0) return -20;
-  if (map(&tmB, B, b_mn ? p.K : p.N, b_mn ? p.N : p.K, 64, b_mn ? 64 : (PAIR ? BN / 2 : BN), TMAP_SWIZZLE_128B) != 0)
+  if (map(&tmA, A, a_mn ? p.K : p.M, a_mn ? mn_cols(A, p.M) : p.K, 64, a_mn ? 64 : GEMM_BM, TMAP_SWIZZLE_128B) != 0) return -20;
+  if (map(&tmB, B, b_mn ? p.K : p.N, b_mn ? mn_cols(B, p.N) : p.K, 64, b_mn ? 64 : (PAIR ? BN / 2 : BN),
+          TMAP_SWIZZLE_128B) != 0)
     return -21;
   tmOut = tmKeep = tmAux = tmA;
   using S = DenseSmem<BN, PAIR, EPI, AUX && EPI == DENSE_Y>;
@@ -194,7 +203,8 @@ inline int launch_dense(const DenseOperand& A, const DenseOperand& B, DenseParam
   f.bn = c.bn;
   f.tiles_n = (p.N + c.bn - 1) / c.bn;
   const int rows = p.M < f.tile_m ? p.M : f.tile_m;        // of a slab that exist
-  f.blocks_per_tile = (rows * c.bn + 4 * FINISH_THREADS - 1) / (4 * FINISH_THREADS);
+  f.ways = c.plan.slots() >= 16 * c.plan.tiles ? 8 : 1;
+  f.blocks_per_tile = (rows * c.bn * f.ways + 4 * FINISH_THREADS - 1) / (4 * FINISH_THREADS);
   return launch_dense_finish(f, st);
 }
 
@@ -248,7 +258,11 @@ inline bool dense_few(int M, int N, int K) {
   return M <= 8 || (M <= FEW_ROWS && (M <= 16 ? 2 : 4) * weights <= (1ll << 25));
 }
 
-inline long long dense_round8(long long n) { return (n + 7) / 8 * 8; }
+// Row stride of what the layer lays out for itself: whole 128-byte lines (or a part of one that holds the row). TMA's
+// boxes are 128 bytes wide, and each of their rows that straddles two lines is two requests: dW 1080 x 632 of 18159 rows
+// 48 us with both operands' rows on any 16 bytes, 42 with dz's on lines, 38 with both; dx 18159 x 632 of 1080 columns 31,
+// 26, 25; y 20000 x 2040 of 520 columns 55, 48 (x on lines), 41.
+inline int dense_pitch(int n) { return n <= 16 ? 16 : n <= 32 ? 32 : (n + 63) / 64 * 64; }
 inline bool dense_aligned(const void* p, long long ld) {
   return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % 8 == 0;
 }
@@ -271,12 +285,12 @@ struct DenseArena {
 
 // Adds a copy of o to a and makes o the copy.
 inline void align_add(AlignRows& a, DenseOperand& o, void* to, long long rows, int cols) {
-  const long long ld = dense_round8(cols);
+  const int ld = dense_pitch(cols);
   const int n = a.n++;
   a.src[n] = static_cast<const uint16_t*>(o.p); a.lds[n] = o.ld;
   a.dst[n] = static_cast<uint16_t*>(to); a.ldd[n] = ld;
   a.rows[n] = rows; a.cols[n] = cols;
-  o = {to, ld};
+  o = {to, ld, ld};
 }
 inline int align_blocks(const AlignRows& a, int sms) {       // of one matrix
   long long most = 0;
@@ -293,9 +307,9 @@ inline int align_blocks(const AlignRows& a, int sms) {       // of one matrix
 inline int64_t dense_forward_bytes(int M, int N, int K, bool x_ok, bool w_ok, bool r_ok, int sms) {
   if (dense_few(M, N, K)) return 0;
   DenseArena ws{nullptr, 0};
-  if (!x_ok) ws.take(2 * dense_round8(K) * M);
-  if (!w_ok) ws.take(2 * dense_round8(K) * N);
-  if (!r_ok) ws.take(2 * dense_round8(N) * M);
+  if (!x_ok) ws.take(2LL * dense_pitch(K) * M);
+  if (!w_ok) ws.take(2LL * dense_pitch(K) * N);
+  if (!r_ok) ws.take(2LL * dense_pitch(N) * M);
   ws.take(dense_choice(M, N, K, sms).slab_bytes());
   return ws.used;
 }
@@ -306,11 +320,11 @@ inline int launch_dense_forward(DenseOperand x, DenseOperand w, DenseParams p, v
   if (dense_few(p.M, p.N, p.K)) return launch_few_rows(x, w, p, x_ok && w_ok && p.K % 8 == 0, sms, st);
   DenseArena ws{static_cast<uint8_t*>(workspace), 0};
   AlignRows a{};
-  if (!x_ok) align_add(a, x, ws.take(2 * dense_round8(p.K) * p.M), p.M, p.K);
-  if (!w_ok) align_add(a, w, ws.take(2 * dense_round8(p.K) * p.N), p.N, p.K);
+  if (!x_ok) align_add(a, x, ws.take(2LL * dense_pitch(p.K) * p.M), p.M, p.K);
+  if (!w_ok) align_add(a, w, ws.take(2LL * dense_pitch(p.K) * p.N), p.N, p.K);
   if (p.aux && !dense_aligned(p.aux, p.ldaux)) {
     DenseOperand r{p.aux, p.ldaux};
-    align_add(a, r, ws.take(2 * dense_round8(p.N) * p.M), p.M, p.N);
+    align_add(a, r, ws.take(2LL * dense_pitch(p.N) * p.M), p.M, p.N);
     p.aux = r.p;
     p.ldaux = r.ld;
   }
@@ -350,7 +364,7 @@ inline DenseGradSums dense_grad_sums(int M, int N, int sms) {
   return g;
 }
 
-// dz goes through memory when there is an activation, or when dy is not aligned; then it is [M, round8(N)].
+// dz goes through memory when there is an activation, or when dy is not aligned; then its rows are dense_pitch(N) apart.
 struct DenseGradPlan {
   bool copy_x, copy_w, make_dz, aligned;
   DenseChoice cx, cw;
@@ -371,9 +385,9 @@ inline DenseGradPlan dense_grad_plan(int M, int N, int K, bool act, bool dy_ok, 
   if (dx) g.cx = dense_choice(M, K, N, sms);
   if (dw) g.cw = dense_choice(N, K, M, sms);
   DenseArena ws{static_cast<uint8_t*>(workspace), 0};
-  if (g.make_dz) g.dz = ws.take(2 * dense_round8(N) * M);
-  if (g.copy_x) g.xs = ws.take(2 * dense_round8(K) * M);
-  if (g.copy_w) g.ws = ws.take(2 * dense_round8(K) * N);
+  if (g.make_dz) g.dz = ws.take(2LL * dense_pitch(N) * M);
+  if (g.copy_x) g.xs = ws.take(2LL * dense_pitch(K) * M);
+  if (g.copy_w) g.ws = ws.take(2LL * dense_pitch(K) * N);
   if (db && g.sums.blocks > 1) g.col_sums = static_cast<float*>(ws.take(4LL * g.sums.blocks * N));
   const int64_t sx = g.cx.slab_bytes(), sw = g.cw.slab_bytes();
   g.slabs = ws.take(sx > sw ? sx : sw);        // one after the other on the stream
@@ -391,7 +405,7 @@ inline int launch_dense_backward(const DenseGradParams& q, const DenseGradPlan& 
     SlopeParams s{};
     s.dy = q.dy.p; s.ldy = q.dy.ld;
     s.z = q.z.p; s.ldz = q.z.ld;
-    s.dz = g.make_dz ? g.dz : nullptr; s.lddz = dense_round8(q.N);
+    s.dz = g.make_dz ? g.dz : nullptr; s.lddz = dense_pitch(q.N);
     s.sums = g.sums.blocks == 1 ? q.db : g.col_sums;
     s.M = q.M; s.N = q.N; s.act = q.act; s.lanes = g.sums.lanes; s.rows_per_block = g.sums.rows_per_block;
     s.cols = g.sums.cols;
@@ -402,7 +416,7 @@ inline int launch_dense_backward(const DenseGradParams& q, const DenseGradPlan& 
     if (q.fp16) r = g.aligned ? go(dense_slope_kernel<__half, true>) : go(dense_slope_kernel<__half, false>);
     else r = g.aligned ? go(dense_slope_kernel<__nv_bfloat16, true>) : go(dense_slope_kernel<__nv_bfloat16, false>);
     if (r != 0) return r;
-    if (g.make_dz) dz = {g.dz, dense_round8(q.N)};
+    if (g.make_dz) dz = {g.dz, dense_pitch(q.N), dense_pitch(q.N)};
   }
   // db is added up by the first product's kernel, unless the product has too few blocks for it (2 x 16 x 472: 31 us in
   // the one block of dx, 4 in a kernel of its own). The sums of a single block of rows are db.

@@ -503,11 +503,12 @@ dense_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
 }
 
 // ---------------------------------------------------------------- the second half of a split product
-// Adds up a tile's slabs in the order of their slots and applies the epilogue. A thread has four columns of a row.
+// Adds up a tile's slabs in a fixed order and applies the epilogue. A thread has four columns of a row; where a tile has
+// many slabs, eight threads share them (64 x 64 of 64678 rows, 148 slabs: dW 30.7 us -> 15.8).
 // Without slabs: the column sums alone (db where no product is asked for).
 struct DenseFinish {
   DenseParams p;
-  int tile_m, bn, tiles_n, blocks_per_tile;
+  int tile_m, bn, tiles_n, blocks_per_tile, ways;
 };
 
 constexpr int FINISH_THREADS = 256;
@@ -547,17 +548,31 @@ __global__ void __launch_bounds__(FINISH_THREADS) dense_finish_kernel(const Dens
   }
   __syncthreads();
   const int mt = tile / f.tiles_n, jt = tile - mt * f.tiles_n;
-  const int i = ((blockIdx.x - tile * f.blocks_per_tile) * FINISH_THREADS + threadIdx.x) * 4;
+  const int per = FINISH_THREADS / f.ways, way = threadIdx.x / per;
+  const int i = ((blockIdx.x - tile * f.blocks_per_tile) * per + threadIdx.x - way * per) * 4;
   const int r = i / f.bn, c = i - r * f.bn;
   const int row = mt * f.tile_m + r, col = jt * f.bn + c;
-  if (r >= f.tile_m || row >= p.M || col >= p.N) return;
+  const bool live = r < f.tile_m && row < p.M && col < p.N;
+  if (f.ways == 1 && !live) return;
   const long long slab = static_cast<long long>(f.tile_m) * f.bn;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  const int n = n_slots;
+  const int n = n_slots, share = (n + f.ways - 1) / f.ways, k1 = min(n, (way + 1) * share);
+  if (live) {
 #pragma unroll 4
-  for (int k = 0; k < n; ++k) {
-    const float4 b = *reinterpret_cast<const float4*>(p.part + slots[k] * slab + i);
-    a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+    for (int k = way * share; k < k1; ++k) {
+      const float4 b = *reinterpret_cast<const float4*>(p.part + slots[k] * slab + i);
+      a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+    }
+  }
+  if (f.ways > 1) {
+    __shared__ float4 sums[FINISH_THREADS];
+    sums[threadIdx.x] = a;
+    __syncthreads();
+    if (way > 0 || !live) return;
+    for (int k = 1; k < f.ways; ++k) {
+      const float4 b = sums[k * per + threadIdx.x];
+      a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+    }
   }
   float z[4] = {a.x, a.y, a.z, a.w};
   if (p.bias != nullptr) {

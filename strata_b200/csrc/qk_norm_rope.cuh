@@ -253,9 +253,9 @@ struct QkRing {
   static constexpr int BYTES = 8 * STAGES * STAGE;
 };
 
-// SPLIT: a token's heads go to the blocks of a grid column (a kernel of its own: with its limits in registers the loop
-// over many tokens is 5 to 11 % slower). GRAD false: y; true: dx and the sums of dw. Blocks of 256 threads, a stride loop over the tokens; a step is
-// QK_ROUNDS rounds of a token's q heads or k heads, asked for STAGES - 1 steps ahead.
+// GRAD false: y; true: dx and the sums of dw. SPLIT: a token's heads go to the blocks of a grid column (a kernel of its
+// own: with its limits in registers the loop over many tokens is 5 to 11 % slower). Blocks of 256 threads, a stride loop
+// over the tokens; a step is QK_ROUNDS rounds of a token's q heads or k heads, asked for STAGES - 1 steps ahead.
 template <typename T, int G, int TAB, bool ADJ, bool GRAD, bool SPLIT>
 __global__ void __launch_bounds__(256, GRAD ? 2 : 4) qk_norm_rope_kernel(const QkParams p) {
   using Ring = QkRing<TAB, ADJ, GRAD>;
@@ -336,8 +336,8 @@ __global__ void __launch_bounds__(256, GRAD ? 2 : 4) qk_norm_rope_kernel(const Q
     int row = 0;
     float c[N], s[N];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      for (int h0 = 0; (SPLIT && h0 == 0) || h0 < lim(k); h0 += R * width) {     // (a part without k heads: an empty step)
+    for (int k = 0; k < 2; ++k) {      // (a part without k heads: an empty step)
+      for (int h0 = 0; (SPLIT && h0 == 0) || h0 < lim(k); h0 += R * width) {
         ask();
         asm volatile("cp.async.wait_group %0;" ::"n"(D - 1) : "memory");
         const uint32_t slot = slots + stage * Ring::STAGE;
@@ -428,8 +428,8 @@ inline int qk_group(int head_dim) {      // (16 channels in two lanes are no nar
 // A token a warp: no more blocks than that takes, and no more than run at once backward (a row of sums each).
 inline long long qk_most_blocks(bool grad, int sms) { return static_cast<long long>(sms) * (grad ? 2 : 16); }
 // Grid for p's tokens and heads; sets p.part. Where the tokens leave room for that, a token's heads go to several
-// blocks, down to one round of q heads each (44 tokens, 48 + 12 heads of 256, in a row of calls: forward 29.3 us -> 13.0,
-// backward 38.7 -> 16.7; from 300 tokens of 12 + 12 heads of 64 on no difference).
+// blocks, down to one round of q heads each (44 tokens, 48 + 12 heads of 256, in a row of calls: forward 29.3 us ->
+// 13.0, backward 38.7 -> 16.7; from 300 tokens of 12 + 12 heads of 64 on no difference).
 inline dim3 qk_grid(QkParams& p, bool grad, int sms) {
   const long long blocks = (p.M + 7) / 8, cap = qk_most_blocks(grad, sms);
   p.part[0] = p.heads[0];

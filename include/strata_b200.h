@@ -79,7 +79,7 @@ int strata_linear_bf16(const void* x, int64_t ldx, const void* w, int64_t ldw, c
  * (same stride), nothing else may overlap. padded != 0: the columns behind N up to the next multiple of 8 are the
  * caller's to write in every row of y and preact (zeros may land there), which lets rows of such strides use TMA.
  * workspace: 256-byte aligned, of strata_linear_act_workspace_bytes bytes (negative: an error code), where an operand
- * counts as aligned when its address and its row stride are multiples of 16 bytes, or it is not there (others are
+ * counts as aligned when its address and its row stride are multiples of 16 bytes, or it is not there (others may be
  * copied there first). Up to 8 rows are one launch without workspace; M = 0 does nothing. Replaces the nn.Linear
  * calls of a block together with the operators around them (attn.proj, mlp.layers.*) in fine-tuning. */
 int64_t strata_linear_act_workspace_bytes(int M, int N, int K, int x_aligned, int w_aligned, int residual_aligned);

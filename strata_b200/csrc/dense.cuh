@@ -49,9 +49,9 @@ inline int dense_pairs(int sms) {
 }
 
 // The cheapest form by a model of each one's time, in microseconds: a k-block of 64 on one unit, the part of a tile's
-// epilogue that nothing hides, a launch, and a slab's way to memory and back. On 210 random products (40 to 100000 rows,
-// widths from 32 to 4000) the form it takes was within 1 % of the fastest on average, within 30 % in all. Some of the
-// shapes it was checked on, tiles of 64 / 128 / 256 unsplit, then split (the one taken in brackets):
+// epilogue that nothing hides, a launch, and a slab's way to memory and back. On 210 random products (40 to 100000
+// rows, widths from 32 to 4000) the form it takes was within 1 % of the fastest on average, within 30 % in all. Some of
+// the shapes it was checked on, tiles of 64 / 128 / 256 unsplit, then split (the one taken in brackets):
 //   y   64 x 1024, K = 4096    12.0 / 13.5 / 23.3   [7.4] / 10.6 / 12.3
 //   y   2500 x 650, K = 207    6.6 / [5.9] / 7.2    (no split: enough tiles, four k-blocks)
 //   y   98304 x 512, K = 2048  255 / 187 / [153]    371 / 296 / 249
@@ -119,14 +119,15 @@ inline int launch_dense_t(const DenseOperand& A, const DenseOperand& B, const De
     const uint32_t box[2] = {bx, by};
     return make_tmap_bf16(tm, o.p, 2, dims, str, box, sw);      // (either 16-bit type: nothing is converted)
   };
-  if (map(&tmA, A, a_mn ? p.K : p.M, a_mn ? mn_cols(A, p.M) : p.K, 64, a_mn ? 64 : GEMM_BM, TMAP_SWIZZLE_128B) != 0) return -20;
+  if (map(&tmA, A, a_mn ? p.K : p.M, a_mn ? mn_cols(A, p.M) : p.K, 64, a_mn ? 64 : GEMM_BM, TMAP_SWIZZLE_128B) != 0)
+    return -20;
   if (map(&tmB, B, b_mn ? p.K : p.N, b_mn ? mn_cols(B, p.N) : p.K, 64, b_mn ? 64 : (PAIR ? BN / 2 : BN),
           TMAP_SWIZZLE_128B) != 0)
     return -21;
   tmOut = tmKeep = tmAux = tmA;
   using S = DenseSmem<BN, PAIR, EPI, AUX && EPI == DENSE_Y>;
   constexpr TmapSwizzle sw = S::BOX_COLS == 64 ? TMAP_SWIZZLE_128B : TMAP_SWIZZLE_64B;
-  if (EPI != DENSE_PART && p.aux &&
+  if (EPI != DENSE_PART && p.aux && !p.direct_aux &&
       map(&tmAux, {p.aux, p.ldaux}, p.M, p.N, S::BOX_COLS, 32, sw) != 0)
     return -23;
   if (EPI != DENSE_PART && !p.direct_out) {
@@ -166,7 +167,7 @@ template <int LAY, int EPI, typename T>
 inline int launch_dense_bn(int bn, const DenseOperand& A, const DenseOperand& B, const DenseParams& p, int units,
                            cudaStream_t st) {
   if constexpr (LAY == DENSE_NT && EPI != DENSE_PART) {
-    if (bn == 256 && !p.direct_out)
+    if (bn == 256 && !p.direct_out && !p.direct_aux)
       return p.aux ? launch_dense_pair<EPI, T, true>(A, B, p, units, st)
                    : launch_dense_pair<EPI, T, false>(A, B, p, units, st);
   }
@@ -259,9 +260,9 @@ inline bool dense_few(int M, int N, int K) {
 }
 
 // Row stride of what the layer lays out for itself: whole 128-byte lines (or a part of one that holds the row). TMA's
-// boxes are 128 bytes wide, and each of their rows that straddles two lines is two requests: dW 1080 x 632 of 18159 rows
-// 48 us with both operands' rows on any 16 bytes, 42 with dz's on lines, 38 with both; dx 18159 x 632 of 1080 columns 31,
-// 26, 25; y 20000 x 2040 of 520 columns 55, 48 (x on lines), 41.
+// boxes are 128 bytes wide, and each of their rows that straddles two lines is two requests: dW 1080 x 632 of 18159
+// rows 48 us with both operands' rows on any 16 bytes, 42 with dz's on lines, 38 with both; dx 18159 x 632 of 1080
+// columns 31, 26, 25; y 20000 x 2040 of 520 columns 55, 48 (x on lines), 41.
 inline int dense_pitch(int n) { return n <= 16 ? 16 : n <= 32 ? 32 : (n + 63) / 64 * 64; }
 inline bool dense_aligned(const void* p, long long ld) {
   return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % 8 == 0;
@@ -303,14 +304,23 @@ inline int align_blocks(const AlignRows& a, int sms) {       // of one matrix
 }
 
 // ---------------------------------------------------------------- forward
+// A residual that TMA cannot read is read by the epilogue's warps, or copied where a kernel for copies runs anyway and
+// units have several tiles (which hide a TMA load better). Read / copied, microseconds (x aligned but for the first
+// two): 10473 x 650, K = 207 27 / 24; 2500 x 650, K = 207 11.4 / 14.1; 10473 x 650, K = 208 18 / 22; 24000 x 105, K =
+// 40 15 / 30; 61552 x 97, K = 552 29 / 41; 16899 x 913, K = 3448 105 / 116; 20000 x 2047, K = 512 92 / 91; 120828 x
+// 1428, K = 40 308 / 294.
+inline bool dense_copies_residual(const DenseChoice& c, bool x_ok, bool w_ok, bool r_ok) {
+  return !r_ok && !(x_ok && w_ok) && c.plan.tiles > c.plan.units;
+}
 // Workspace: aligned copies of the operands that are not aligned themselves, then the slabs of a split.
 inline int64_t dense_forward_bytes(int M, int N, int K, bool x_ok, bool w_ok, bool r_ok, int sms) {
   if (dense_few(M, N, K)) return 0;
   DenseArena ws{nullptr, 0};
+  const DenseChoice c = dense_choice(M, N, K, sms);
   if (!x_ok) ws.take(2LL * dense_pitch(K) * M);
   if (!w_ok) ws.take(2LL * dense_pitch(K) * N);
-  if (!r_ok) ws.take(2LL * dense_pitch(N) * M);
-  ws.take(dense_choice(M, N, K, sms).slab_bytes());
+  if (dense_copies_residual(c, x_ok, w_ok, r_ok)) ws.take(2LL * dense_pitch(N) * M);
+  ws.take(c.slab_bytes());
   return ws.used;
 }
 
@@ -322,17 +332,19 @@ inline int launch_dense_forward(DenseOperand x, DenseOperand w, DenseParams p, v
   AlignRows a{};
   if (!x_ok) align_add(a, x, ws.take(2LL * dense_pitch(p.K) * p.M), p.M, p.K);
   if (!w_ok) align_add(a, w, ws.take(2LL * dense_pitch(p.K) * p.N), p.N, p.K);
-  if (p.aux && !dense_aligned(p.aux, p.ldaux)) {
+  const DenseChoice c = dense_choice(p.M, p.N, p.K, sms);
+  p.direct_aux = p.aux && !dense_aligned(p.aux, p.ldaux);
+  if (dense_copies_residual(c, x_ok, w_ok, !p.direct_aux)) {
     DenseOperand r{p.aux, p.ldaux};
     align_add(a, r, ws.take(2LL * dense_pitch(p.N) * p.M), p.M, p.N);
     p.aux = r.p;
     p.ldaux = r.ld;
+    p.direct_aux = false;
   }
   if (a.n > 0) {
     const dim3 grid(static_cast<unsigned>(align_blocks(a, sms)), static_cast<unsigned>(a.n));
     if (const int r = launch_chained(dense_align_rows_kernel, grid, 256, 0, st, 1, a); r != 0) return r;
   }
-  const DenseChoice c = dense_choice(p.M, p.N, p.K, sms);
   return launch_dense<DENSE_NT>(x, w, p, c, ws.take(c.slab_bytes()), st);
 }
 
@@ -364,7 +376,8 @@ inline DenseGradSums dense_grad_sums(int M, int N, int sms) {
   return g;
 }
 
-// dz goes through memory when there is an activation, or when dy is not aligned; then its rows are dense_pitch(N) apart.
+// dz goes through memory when there is an activation, or when dy is not aligned; then its rows are dense_pitch(N)
+// apart.
 struct DenseGradPlan {
   bool copy_x, copy_w, make_dz, aligned;
   DenseChoice cx, cw;

@@ -5,39 +5,6 @@
 
 namespace strata {
 
-// Eight values of a row from p on, of which n exist (n <= 0: none), the others zero. ALIGNED: p is a multiple of 16
-// bytes and n >= 8 or n <= 0. Otherwise the two aligned 16-byte pieces that hold them are read and shifted together: a
-// piece is read only if it holds a value that exists, and memory is given out in larger units than 16 bytes.
-template <bool ALIGNED>
-__device__ __forceinline__ uint4 load8(const void* p, int n) {
-  uint4 u = make_uint4(0u, 0u, 0u, 0u);
-  if (n <= 0) return u;
-  if constexpr (ALIGNED) return __ldg(static_cast<const uint4*>(p));
-  const uintptr_t a = reinterpret_cast<uintptr_t>(p);
-  const int off = static_cast<int>(a & 15u) >> 1;
-  const uint4* q = reinterpret_cast<const uint4*>(a & ~static_cast<uintptr_t>(15));
-  const uint4 lo = __ldg(q);
-  uint4 hi = u;
-  if (off + (n < 8 ? n : 8) > 8) hi = __ldg(q + 1);
-  uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-  if (off & 4) {
-#pragma unroll
-    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
-  }
-  if (off & 2) {
-#pragma unroll
-    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
-  }
-  const uint32_t bits = (off & 1) * 16;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], bits);
-  if (n < 8) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = 2 * i + 1 < n ? w[i] : (2 * i < n ? w[i] & 0xFFFFu : 0u);
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
 // The epilogue for one output.
 template <typename T>
 __device__ __forceinline__ void dense_one(const DenseParams& p, int row, int col, float z) {

@@ -36,6 +36,7 @@ struct DenseParams {
   int act;
   int fp16;
   bool direct_out;              // out and keep are written by the warps, not by TMA
+  bool direct_aux;              // the residual is read by the warps
   float* part;                  // DENSE_PART: slabs of TILE_M x BN
   const float* sums;            // column sums of dense_slope_kernel, [sum_rows, sum_cols], or nullptr; added up into
   int sum_rows, sum_cols;       //   db by epilogue warps that wait for their first tile
@@ -100,9 +101,9 @@ __device__ __forceinline__ void dense_store_pair(void* base, long long at, uint3
 }
 __device__ __forceinline__ uint32_t dense_load_pair(const void* base, long long at, bool two) {
   const uint16_t* p = static_cast<const uint16_t*>(base) + at;
-  if (two && (reinterpret_cast<uintptr_t>(p) & 3u) == 0) return __ldg(reinterpret_cast<const uint32_t*>(p));
-  const uint32_t lo = __ldg(p);
-  return two ? lo | (static_cast<uint32_t>(__ldg(p + 1)) << 16) : lo;
+  if (two && (reinterpret_cast<uintptr_t>(p) & 3u) == 0) return *reinterpret_cast<const uint32_t*>(p);
+  const uint32_t lo = *p;
+  return two ? lo | (static_cast<uint32_t>(p[1]) << 16) : lo;
 }
 // A warp's copy of a 32 x 32 staging box (64-byte rows and swizzle) to rows that TMA does not store: two rows at a
 // time, 16 lanes with neighbouring pairs each.
@@ -118,6 +119,70 @@ __device__ __forceinline__ void dense_copy_box(uint32_t box, void* base, long lo
   for (int i = 0; i < 16; ++i) {
     const int row = m0 + 2 * i + (lane >> 4);
     if (row < M && col < N) dense_store_pair(base, static_cast<long long>(row) * ld + col, w[i], col + 1 < N);
+  }
+}
+
+// Eight values of a row from p on, of which n exist (n <= 0: none), the others zero. ALIGNED: p is a multiple of 16
+// bytes and n >= 8 or n <= 0. Otherwise the two aligned 16-byte pieces that hold them are read and shifted together: a
+// piece is read only if it holds a value that exists, and memory is given out in larger units than 16 bytes.
+template <bool ALIGNED>
+__device__ __forceinline__ uint4 load8(const void* p, int n) {
+  uint4 u = make_uint4(0u, 0u, 0u, 0u);
+  if (n <= 0) return u;
+  if constexpr (ALIGNED) return __ldg(static_cast<const uint4*>(p));
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+  const int off = static_cast<int>(a & 15u) >> 1;
+  const uint4* q = reinterpret_cast<const uint4*>(a & ~static_cast<uintptr_t>(15));
+  const uint4 lo = __ldg(q);
+  uint4 hi = u;
+  if (off + (n < 8 ? n : 8) > 8) hi = __ldg(q + 1);
+  uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+  if (off & 4) {
+#pragma unroll
+    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+  }
+  if (off & 2) {
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+  }
+  const uint32_t bits = (off & 1) * 16;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], bits);
+  if (n < 8) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = 2 * i + 1 < n ? w[i] : (2 * i < n ? w[i] & 0xFFFFu : 0u);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// The way back, for rows that TMA does not load: 16-byte pieces, four lanes a row. alone: not a byte besides the box's
+// own, in pairs (what is read is written by other warps meanwhile).
+__device__ __forceinline__ void dense_load_box(uint32_t box, const void* base, long long ld, int m0, int n0, int M,
+                                               int N, bool alone) {
+  const int lane = threadIdx.x & 31;
+  if (!alone) {
+    uint4 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = m0 + 8 * i + (lane >> 2), col = n0 + 8 * (lane & 3);
+      v[i] = load8<false>(static_cast<const uint16_t*>(base) + static_cast<long long>(row < M ? row : m0) * ld + col,
+                          N - col);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t r = 8 * i + (lane >> 2), piece = static_cast<uint32_t>(lane & 3) ^ ((r >> 1) & 3u);
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(box + r * 64u + (piece << 4)), "r"(v[i].x),
+                   "r"(v[i].y), "r"(v[i].z), "r"(v[i].w) : "memory");
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int j = lane & 15, row = m0 + 2 * i + (lane >> 4), col = n0 + 2 * j;
+    const uint32_t r = 2 * i + (lane >> 4), piece = static_cast<uint32_t>(j >> 2) ^ ((r >> 1) & 3u);
+    const uint32_t w =
+        row < M && col < N ? dense_load_pair(base, static_cast<long long>(row) * ld + col, col + 1 < N) : 0u;
+    asm volatile("st.shared.b32 [%0], %1;" ::"r"(box + r * 64u + (piece << 4) + (j & 3) * 4), "r"(w) : "memory");
   }
 }
 
@@ -330,7 +395,7 @@ dense_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
       const uint32_t r = ((lane >> 3) & 1) * 8 + (lane & 7), piece = 4 * c + 2 * q + (lane >> 4);
       return b + (16 * hf + r) * (BC * 2u) + ((BC == 64 ? piece ^ (r & 7) : piece ^ ((r >> 1) & 3)) << 4);
     };
-    const bool fetch = !PART && has_aux;
+    const bool load = !PART && ANY && has_aux && p.direct_aux, fetch = !PART && has_aux && !load;
     [[maybe_unused]] uint32_t aux_phase = 0;
     // first row and column of this warp's part of a tile; whether there is anything of it
     auto part_of = [&](int tile, int& m, int& n) -> bool {
@@ -384,6 +449,14 @@ dense_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
       for (int c0 = 0; c0 < WARP_COLS; c0 += BC) {              // a box
         const bool box_live = live && n_warp0 + c0 < p.N;
         if (!AHEAD && fetch && box_live) fetch_aux(m_warp, n_warp0 + c0);
+        if constexpr (ANY && !PART && BC == 32) {
+          if (load && box_live) {
+            if (elect_one()) tma_store_wait_read0();
+            __syncwarp();
+            dense_load_box(box, p.aux, p.ldaux, m_warp, n_warp0 + c0, p.M, p.N, p.aux == p.out);
+            __syncwarp();
+          }
+        }
         if (!acc_ready) {
           if (!gemm_wait(accf_bar(buf), (it >> 1) & 1u, abort_flag, ST_TIMEOUT_EPILOGUE)) {
             ok = false;
@@ -503,9 +576,9 @@ dense_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
 }
 
 // ---------------------------------------------------------------- the second half of a split product
-// Adds up a tile's slabs in a fixed order and applies the epilogue. A thread has four columns of a row; where a tile has
-// many slabs, eight threads share them (64 x 64 of 64678 rows, 148 slabs: dW 30.7 us -> 15.8).
-// Without slabs: the column sums alone (db where no product is asked for).
+// Adds up a tile's slabs in a fixed order and applies the epilogue. A thread has four columns of a row; where a tile
+// has many slabs, eight threads share them (64 x 64 of 64678 rows, 148 slabs: dW 30.7 us -> 15.8). Without slabs: the
+// column sums alone (db where no product adds them up).
 struct DenseFinish {
   DenseParams p;
   int tile_m, bn, tiles_n, blocks_per_tile, ways;

@@ -253,9 +253,9 @@ struct QkRing {
   static constexpr int BYTES = 8 * STAGES * STAGE;
 };
 
-// GRAD false: y; true: dx and the sums of dw. SPLIT: a token's heads go to the blocks of a grid column (a kernel of its
-// own: with its limits in registers the loop over many tokens is 5 to 11 % slower). Blocks of 256 threads, a stride loop
-// over the tokens; a step is QK_ROUNDS rounds of a token's q heads or k heads, asked for STAGES - 1 steps ahead.
+// GRAD false: y; true: dx and the sums of dw. SPLIT: a token's heads go to the blocks of a grid column (a kernel of
+// its own: with its limits in registers the loop over many tokens is 5 to 11 % slower). Blocks of 256 threads, a stride
+// loop over the tokens; a step is QK_ROUNDS rounds of a token's q heads or k heads, asked for STAGES - 1 steps ahead.
 template <typename T, int G, int TAB, bool ADJ, bool GRAD, bool SPLIT>
 __global__ void __launch_bounds__(256, GRAD ? 2 : 4) qk_norm_rope_kernel(const QkParams p) {
   using Ring = QkRing<TAB, ADJ, GRAD>;

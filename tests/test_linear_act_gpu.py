@@ -253,6 +253,25 @@ def test_out_may_be_the_residual_and_leaves_the_rest_alone(ops, M, N):
     assert bool((wide == 7.0).all())
 
 
+# every tile, one and several turns, with and without other operands that have to be copied, split sums
+@pytest.mark.parametrize("M,N,K", [(40, 17, 64), (300, 65, 64), (24000, 105, 40), (2500, 650, 207),
+                                   (40000, 97, 128), (9000, 1001, 64), (9000, 1002, 77), (64, 130, 4096)])
+@pytest.mark.parametrize("t", [BF, HF])
+def test_residual_rows_off_the_grid(ops, M, N, K, t):
+    """Contiguous, one element off, and in place between NaN; out leaves what lies around it alone. (Every result against
+    64 bits: kernels for different rows may contract the activation's products differently.)"""
+    d = data(M, N, K, t)
+    check_forward(ops.linear_act(d["x"], d["w"], d["b"], "silu", d["r"]), None, d, "silu")
+    for lead in (1, 2, 8):
+        wide = torch.full((M + 2, N + lead + 5), float("nan"), device="cuda", dtype=t)
+        r = wide[1:M + 1, lead:lead + N]
+        r.copy_(d["r"])
+        check_forward(ops.linear_act(d["x"], d["w"], d["b"], "silu", r), None, d, "silu")
+        assert ops.linear_act(d["x"], d["w"], d["b"], "silu", r, out=r) is r
+        check_forward(r, None, d, "silu")
+        assert int(wide.isnan().sum()) == wide.numel() - M * N
+
+
 def test_no_rows(ops):
     d = data(0, 24, 16, HF)
     assert ops.linear_act(d["x"], d["w"], d["b"], "gelu", d["r"]).shape == (0, 24)

@@ -11,8 +11,8 @@
 // (several tokens where both q and k have fewer heads than that), in steps of two rounds of q heads or of k heads. So
 // the token's table row is read and unpacked once for all its heads. A head whose width is no power of two leaves the
 // group's last lanes idle. What a step reads is asked for two steps ahead with cp.async into slots of shared memory
-// that only the asking lane reads: bytes in flight that cost no registers, and no barrier. Divisions by launch
-// constants are multiplications; arithmetic runs on fp32 pairs.
+// that only the asking lane reads (but for shared table rows): bytes in flight that cost no registers, and no barrier.
+// Divisions by launch constants are multiplications; arithmetic runs on fp32 pairs.
 // Measured (8 + 8 heads of 64, 262144 tokens, bf16, half table; the bytes alone take 166 us forward, 250 backward):
 // forward 198 us, backward 292 (178 and 263 without rotation). With the loads straight into registers, two rounds of q
 // and two of k at a time: 190 and 355 (16 + 4 heads of 128: 303 against 248, 370 against 323); more blocks per SM at
@@ -60,6 +60,9 @@ struct QkParams {
 };
 
 enum QkTable : int { QK_NO_TABLE = 0, QK_HALF_TABLE = 1, QK_F32_TABLE = 2 };
+// How a token's heads come: QK_ROUNDS rounds of q heads or of k heads a step; the same for a part of them, the other
+// parts in other blocks; a round of q heads and one of k heads a step, which are all.
+enum QkHeads : int { QK_ALL = 0, QK_PARTS = 1, QK_FEW = 2 };
 
 // Table row of token m; -1: a padding token, -2: no such row.
 __device__ __forceinline__ int qk_row(const QkParams& p, long long m) {
@@ -245,20 +248,31 @@ __device__ __forceinline__ uint4 qk_got(uint32_t slot) {
   return u;
 }
 
-template <int TAB, bool ADJ, bool GRAD>
+// A stage of a warp: the lanes' vectors, the table's, and the lanes' table rows. The table's vectors are each lane's
+// own like the others, or (SHARE) those of the tokens' rows side by side, each loaded once by whichever lane and read
+// by all that need it: where a lane needs four, 64 bytes from the next lane's, and two beside a single step's vectors.
+// Own / shared, microseconds forward, 142667 tokens of 4 + 4 heads of 64: four 188 / 93, two 87 / 79, one 60 / 64;
+// 65536 of 16 + 4 heads of 128: four 169 / 164, two 145 / 152; 262144 of 8 + 8 heads of 64, one: 200 / 219.
+template <int TAB, bool ADJ, bool GRAD, int HEADS>
 struct QkRing {
   static constexpr int STAGES = 3;
-  static constexpr int VECTORS = (GRAD ? 2 : 1) * QK_ROUNDS + QkTab<TAB, ADJ>::TV;      // of a lane and stage
-  static constexpr int STAGE = VECTORS * 512 + (TAB == QK_NO_TABLE ? 0 : 128);         // of a warp; + the lanes' rows
+  static constexpr int TV = QkTab<TAB, ADJ>::TV;
+  static constexpr bool SHARE = TV == 4 || (TV == 2 && HEADS == QK_FEW);
+  static constexpr int VECTORS = (GRAD ? 2 : 1) * QK_ROUNDS;                      // of a lane
+  static constexpr int TABLE = SHARE ? (TAB == QK_F32_TABLE ? 2 : 1) : TV;
+  static constexpr int ROWS = (VECTORS + TABLE) * 512;
+  static constexpr int STAGE = ROWS + (TAB == QK_NO_TABLE ? 0 : 128);
   static constexpr int BYTES = 8 * STAGES * STAGE;
 };
 
-// GRAD false: y; true: dx and the sums of dw. SPLIT: a token's heads go to the blocks of a grid column (a kernel of
-// its own: with its limits in registers the loop over many tokens is 5 to 11 % slower). Blocks of 256 threads, a stride
-// loop over the tokens; a step is QK_ROUNDS rounds of a token's q heads or k heads, asked for STAGES - 1 steps ahead.
-template <typename T, int G, int TAB, bool ADJ, bool GRAD, bool SPLIT>
+// GRAD false: y; true: dx and the sums of dw. Blocks of 256 threads, a stride loop over the tokens, steps asked for
+// STAGES - 1 ahead. Kernels of their own for the ways of the heads: with the limits of QK_PARTS in registers the loop
+// over many tokens is 5 to 11 % slower; QK_FEW has twice the bytes in flight of two half-empty steps (64458 tokens of
+// 4 + 4 heads of 64: 46 us -> 35, backward 64 -> 48).
+template <typename T, int G, int TAB, bool ADJ, bool GRAD, int HEADS>
 __global__ void __launch_bounds__(256, GRAD ? 2 : 4) qk_norm_rope_kernel(const QkParams p) {
-  using Ring = QkRing<TAB, ADJ, GRAD>;
+  using Ring = QkRing<TAB, ADJ, GRAD, HEADS>;
+  constexpr bool SPLIT = HEADS == QK_PARTS, FEW = HEADS == QK_FEW;
   constexpr int S = 32 / G, R = QK_ROUNDS, N = QkTab<TAB, ADJ>::N, TV = QkTab<TAB, ADJ>::TV, D = Ring::STAGES;
   extern __shared__ uint4 ring[];
   chain_begin();
@@ -269,7 +283,7 @@ __global__ void __launch_bounds__(256, GRAD ? 2 : 4) qk_norm_rope_kernel(const Q
   const int partner = ADJ ? lane : v_raw < hv ? lane + hv : v_raw < 2 * hv ? lane - hv : lane;
   const float inv = 1.0f / static_cast<float>(p.head_dim);
   const uint32_t slots = smem_u32(ring) + (threadIdx.x >> 5) * (D * Ring::STAGE) + lane * 16;
-  const uint32_t rows = smem_u32(ring) + (threadIdx.x >> 5) * (D * Ring::STAGE) + Ring::VECTORS * 512 + lane * 4;
+  const uint32_t rows = slots + Ring::ROWS - lane * 12;
   // heads side by side in the warp, and the tokens that leaves room for
   int width = 1;
   while (width < S && (width < p.part[0] || width < p.part[1])) width *= 2;
@@ -286,6 +300,21 @@ __global__ void __launch_bounds__(256, GRAD ? 2 : 4) qk_norm_rope_kernel(const Q
     return const_cast<uint16_t*>(static_cast<const uint16_t*>(t.p)) + static_cast<long long>(m) * t.token +
            static_cast<long long>(h) * t.head + 8 * v;
   };
+  // SHARE: lane j asks for vector j (fp32: and j + 32) of the tokens' table rows; swizzled, so that eight lanes'
+  // vectors are in different banks
+  constexpr int PER = TAB == QK_F32_TABLE ? 2 : 4;          // entries of a vector
+  const uint32_t tab0 = slots - lane * 16 + Ring::VECTORS * 512;
+  auto tab_at = [](int x) { return static_cast<uint32_t>(x ^ ((x >> 3) & 3)) * 16u; };
+  [[maybe_unused]] int row_vectors = 1, tab_token[2] = {0, 0}, tab_vector[2] = {0, 0}, tab_first = 0;
+  if constexpr (Ring::SHARE) {
+    row_vectors = (p.rot >> 1) / PER;
+#pragma unroll
+    for (int q = 0; q < Ring::TABLE; ++q) {
+      tab_token[q] = (lane + 32 * q) / row_vectors;
+      tab_vector[q] = lane + 32 * q - tab_token[q] * row_vectors;
+    }
+    tab_first = tok * row_vectors + (turns ? qk_entry<ADJ>(p, v_raw) / PER : 0);
+  }
   // the step that is asked for next: token m_a (of the warp's first lanes), tensor k_a, heads from h_a; its stage
   uint32_t m_a = first;
   int k_a = 0, h_a = 0, stage_a = 0, row_a = 0;
@@ -295,23 +324,36 @@ __global__ void __launch_bounds__(256, GRAD ? 2 : 4) qk_norm_rope_kernel(const Q
       const uint32_t slot = slots + stage_a * Ring::STAGE, m = m_a + tok;
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const int h = h_a + r * width + head;
-        const bool on = lane_on && m < M && h < lim(k_a);
-        qk_ask(slot + r * 512, at(p.x[k_a], on ? m : 0, on ? base(k_a) + h : 0), on);
-        if constexpr (GRAD) qk_ask(slot + (R + r) * 512, at(p.dy[k_a], on ? m : 0, on ? base(k_a) + h : 0), on);
+        const int k = FEW ? r : k_a, h = FEW ? head : h_a + r * width + head;
+        const bool on = lane_on && m < M && h < lim(k);
+        qk_ask(slot + r * 512, at(p.x[k], on ? m : 0, on ? base(k) + h : 0), on);
+        if constexpr (GRAD) qk_ask(slot + (R + r) * 512, at(p.dy[k], on ? m : 0, on ? base(k) + h : 0), on);
       }
-      if (TAB != QK_NO_TABLE && k_a == 0 && h_a == 0) {
+      if (TAB != QK_NO_TABLE && (FEW || (k_a == 0 && h_a == 0))) {
         if (m >= M) row_a = -1;
-        const bool on = turns && row_a >= 0;
-        const long long e =
-            (on ? static_cast<long long>(row_a) * (p.rot >> 1) : 0) + (turns ? qk_entry<ADJ>(p, v_raw) : 0);
-        const char* src = static_cast<const char*>(p.table) + e * (TAB == QK_F32_TABLE ? 8 : 4);
+        const char* table = static_cast<const char*>(p.table);
+        if constexpr (Ring::SHARE) {
 #pragma unroll
-        for (int i = 0; i < TV; ++i) qk_ask(slot + ((GRAD ? 2 : 1) * R + i) * 512, src + i * 16, on);
+          for (int q = 0; q < Ring::TABLE; ++q) {
+            const int row = __shfl_sync(0xffffffffu, row_a, tab_token[q] * (width * G) & 31);
+            const bool there = tab_token[q] < tokens, on = there && row >= 0;
+            const long long at16 = on ? static_cast<long long>(row) * row_vectors + tab_vector[q] : 0;
+            if (there) qk_ask(tab0 + stage_a * Ring::STAGE + tab_at(lane + 32 * q), table + at16 * 16, on);
+          }
+        } else {
+          const bool on = turns && row_a >= 0;
+          const long long e =
+              (on ? static_cast<long long>(row_a) * (p.rot >> 1) : 0) + (turns ? qk_entry<ADJ>(p, v_raw) : 0);
+#pragma unroll
+          for (int i = 0; i < TV; ++i)
+            qk_ask(slot + (Ring::VECTORS + i) * 512, table + e * (16 / PER) + i * 16, on);
+        }
         asm volatile("st.shared.b32 [%0], %1;" ::"r"(rows + stage_a * Ring::STAGE), "r"(row_a) : "memory");
         if (m + stride < M) row_a = qk_row(p, m + stride);       // (the next token's, a token ahead)
       }
-      if ((h_a += R * width) >= lim(k_a)) {
+      if constexpr (FEW) {
+        m_a += stride;
+      } else if ((h_a += R * width) >= lim(k_a)) {
         h_a = 0;
         if (++k_a == 2) {
           k_a = 0;
@@ -334,38 +376,57 @@ __global__ void __launch_bounds__(256, GRAD ? 2 : 4) qk_norm_rope_kernel(const Q
   for (uint32_t m0 = first; m0 < M; m0 += stride) {
     const uint32_t m = m0 + tok;
     int row = 0;
-    float c[N], s[N];
+    float c[N], s[N], w[8];
+    auto arrive = [&](bool with_table) {      // the next step's slot
+      if constexpr (Ring::SHARE) __syncwarp();        // (all have read the last step's table rows)
+      ask();
+      asm volatile("cp.async.wait_group %0;" ::"n"(D - 1) : "memory");
+      const uint32_t slot = slots + stage * Ring::STAGE;
+      if (TAB != QK_NO_TABLE && with_table) {
+        if constexpr (Ring::SHARE) __syncwarp();
+        uint4 raw[TV > 0 ? TV : 1];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {      // (a part without k heads: an empty step)
-      for (int h0 = 0; (SPLIT && h0 == 0) || h0 < lim(k); h0 += R * width) {
-        ask();
-        asm volatile("cp.async.wait_group %0;" ::"n"(D - 1) : "memory");
-        const uint32_t slot = slots + stage * Ring::STAGE;
-        if (TAB != QK_NO_TABLE && k == 0 && h0 == 0) {
-          uint4 raw[TV > 0 ? TV : 1];
+        for (int i = 0; i < TV; ++i)
+          raw[i] = qk_got(Ring::SHARE ? tab0 + stage * Ring::STAGE + tab_at(tab_first + i)
+                                      : slot + (Ring::VECTORS + i) * 512);
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(row) : "r"(rows + stage * Ring::STAGE) : "memory");
+        if (row == -2) atomicCAS(&g_status, 0, ST_BAD_POSITION);
+        if constexpr (TAB != QK_NO_TABLE)
+          qk_table<TAB, ADJ>(p, raw, turns && row >= 0, v_raw, GRAD ? 1.f : -1.f, c, s);
+      }
+      stage = stage + 1 == D ? 0 : stage + 1;
+      return slot;
+    };
+    auto round = [&](uint32_t slot, int r, int k, int h) {
+      const uint4 xr = qk_got(slot + r * 512), gr = GRAD ? qk_got(slot + (R + r) * 512) : xr;
+      uint4 o = qk_vector<T, G, TAB, ADJ, GRAD>(xr, gr, w, c, s, partner, TAB == QK_NO_TABLE || row >= 0, inv, p.eps,
+                                               sums[k]);
+      if (TAB != QK_NO_TABLE && p.positions != nullptr && row < 0) {     // padding: zero; behind the table: NaN
+        const uint32_t u = row == -1 ? 0u : 0x7FFF7FFFu;
+        o = make_uint4(u, u, u, u);
+      }
+      if (lane_on && m < M && h < lim(k)) *reinterpret_cast<uint4*>(at(p.y[k], m, base(k) + h)) = o;
+    };
+    if constexpr (FEW) {
+      static_assert(R == 2, "q and k");
+      const uint32_t slot = arrive(true);
 #pragma unroll
-          for (int i = 0; i < TV; ++i) raw[i] = qk_got(slot + ((GRAD ? 2 : 1) * R + i) * 512);
-          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(row) : "r"(rows + stage * Ring::STAGE) : "memory");
-          if (row == -2) atomicCAS(&g_status, 0, ST_BAD_POSITION);
-          if constexpr (TAB != QK_NO_TABLE)
-            qk_table<TAB, ADJ>(p, raw, turns && row >= 0, v_raw, GRAD ? 1.f : -1.f, c, s);
-        }
-        float w[8];
+      for (int k = 0; k < 2; ++k) {
         qk_weights(p.w[k], v, w);
+        round(slot, k, k, head);
+      }
+    } else {
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-          if (r > 0 && h0 + r * width >= lim(k)) continue;       // (the same for the block)
-          const int h = h0 + r * width + head;
-          const uint4 xr = qk_got(slot + r * 512), gr = GRAD ? qk_got(slot + (R + r) * 512) : xr;
-          uint4 o = qk_vector<T, G, TAB, ADJ, GRAD>(xr, gr, w, c, s, partner, TAB == QK_NO_TABLE || row >= 0, inv,
-                                                   p.eps, sums[k]);
-          if (TAB != QK_NO_TABLE && p.positions != nullptr && row < 0) {     // padding: zero; behind the table: NaN
-            const uint32_t u = row == -1 ? 0u : 0x7FFF7FFFu;
-            o = make_uint4(u, u, u, u);
+      for (int k = 0; k < 2; ++k) {      // (a part without k heads: an empty step)
+        for (int h0 = 0; (SPLIT && h0 == 0) || h0 < lim(k); h0 += R * width) {
+          const uint32_t slot = arrive(k == 0 && h0 == 0);
+          qk_weights(p.w[k], v, w);
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            if (r > 0 && h0 + r * width >= lim(k)) continue;       // (the same for the block)
+            round(slot, r, k, h0 + r * width + head);
           }
-          if (lane_on && m < M && h < lim(k)) *reinterpret_cast<uint4*>(at(p.y[k], m, base(k) + h)) = o;
         }
-        stage = stage + 1 == D ? 0 : stage + 1;
       }
     }
   }
@@ -447,10 +508,10 @@ inline dim3 qk_grid(QkParams& p, bool grad, int sms) {
   return dim3(static_cast<unsigned>(blocks < cap ? blocks : cap), static_cast<unsigned>(parts));
 }
 
-template <typename T, int G, int TAB, bool ADJ, bool GRAD, bool SPLIT>
+template <typename T, int G, int TAB, bool ADJ, bool GRAD, int HEADS>
 inline int launch_qk_s(const QkParams& p, dim3 grid, cudaStream_t st) {
-  auto kern = qk_norm_rope_kernel<T, G, TAB, ADJ, GRAD, SPLIT>;
-  constexpr int bytes = QkRing<TAB, ADJ, GRAD>::BYTES;
+  auto kern = qk_norm_rope_kernel<T, G, TAB, ADJ, GRAD, HEADS>;
+  constexpr int bytes = QkRing<TAB, ADJ, GRAD, HEADS>::BYTES;
   static_assert(bytes >= 8 * 2 * G * 8 * 4, "the sums of a block");
   static std::atomic<uint64_t> smem_set;
   if (const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), bytes, smem_set); e != cudaSuccess)
@@ -459,8 +520,9 @@ inline int launch_qk_s(const QkParams& p, dim3 grid, cudaStream_t st) {
 }
 template <typename T, int G, int TAB, bool ADJ, bool GRAD>
 inline int launch_qk_k(const QkParams& p, dim3 grid, cudaStream_t st) {
-  return grid.y > 1 ? launch_qk_s<T, G, TAB, ADJ, GRAD, true>(p, grid, st)
-                    : launch_qk_s<T, G, TAB, ADJ, GRAD, false>(p, grid, st);
+  if (grid.y > 1) return launch_qk_s<T, G, TAB, ADJ, GRAD, QK_PARTS>(p, grid, st);
+  return p.heads[0] <= 32 / G && p.heads[1] <= 32 / G ? launch_qk_s<T, G, TAB, ADJ, GRAD, QK_FEW>(p, grid, st)
+                                                      : launch_qk_s<T, G, TAB, ADJ, GRAD, QK_ALL>(p, grid, st);
 }
 template <typename T, int G, bool GRAD>
 inline int launch_qk_t(const QkParams& p, bool adjacent, dim3 grid, cudaStream_t st) {

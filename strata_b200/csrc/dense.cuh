@@ -285,19 +285,18 @@ struct DenseArena {
 };
 
 // Adds a copy of o to a and makes o the copy.
-inline void align_add(AlignRows& a, DenseOperand& o, void* to, long long rows, int cols) {
+inline void align_add(AlignRows& a, DenseOperand& o, void* to, long long rows, int cols, int sms) {
   const int ld = dense_pitch(cols);
   const int n = a.n++;
   a.src[n] = static_cast<const uint16_t*>(o.p); a.lds[n] = o.ld;
   a.dst[n] = static_cast<uint16_t*>(to); a.ldd[n] = ld;
-  a.rows[n] = rows; a.cols[n] = cols;
+  a.rows[n] = rows; a.cols[n] = cols; a.per[n] = align_block_rows(rows, cols, sms);
   o = {to, ld, ld};
 }
 inline int align_blocks(const AlignRows& a, int sms) {       // of one matrix
   long long most = 0;
   for (int j = 0; j < a.n; ++j) {
-    const int per = align_block_rows(a.cols[j]);
-    const long long blocks = (a.rows[j] + per - 1) / per;
+    const long long blocks = (a.rows[j] + a.per[j] - 1) / a.per[j];
     most = blocks > most ? blocks : most;
   }
   return static_cast<int>(most < 8LL * sms ? most : 8LL * sms);
@@ -305,10 +304,10 @@ inline int align_blocks(const AlignRows& a, int sms) {       // of one matrix
 
 // ---------------------------------------------------------------- forward
 // A residual that TMA cannot read is read by the epilogue's warps, or copied where a kernel for copies runs anyway and
-// units have several tiles (which hide a TMA load better). Read / copied, microseconds (x aligned but for the first
-// two): 10473 x 650, K = 207 27 / 24; 2500 x 650, K = 207 11.4 / 14.1; 10473 x 650, K = 208 18 / 22; 24000 x 105, K =
-// 40 15 / 30; 61552 x 97, K = 552 29 / 41; 16899 x 913, K = 3448 105 / 116; 20000 x 2047, K = 512 92 / 91; 120828 x
-// 1428, K = 40 308 / 294.
+// units have several tiles (which hide a TMA load better). Read / copied, microseconds: 10473 x 650, K = 207 24.0 /
+// 22.7 (half); 30000 x 1001, K = 207 78 / 73; 40000 x 250, K = 77 25 / 28; 2500 x 650, K = 207 11.4 / 14.1; x aligned:
+// 10473 x 650, K = 208 18 / 22; 24000 x 105, K = 40 15 / 30; 61552 x 97, K = 552 29 / 41; 16899 x 913, K = 3448 105 /
+// 116; 20000 x 2047, K = 512 92 / 91; 120828 x 1428, K = 40 308 / 294.
 inline bool dense_copies_residual(const DenseChoice& c, bool x_ok, bool w_ok, bool r_ok) {
   return !r_ok && !(x_ok && w_ok) && c.plan.tiles > c.plan.units;
 }
@@ -330,13 +329,13 @@ inline int launch_dense_forward(DenseOperand x, DenseOperand w, DenseParams p, v
   if (dense_few(p.M, p.N, p.K)) return launch_few_rows(x, w, p, x_ok && w_ok && p.K % 8 == 0, sms, st);
   DenseArena ws{static_cast<uint8_t*>(workspace), 0};
   AlignRows a{};
-  if (!x_ok) align_add(a, x, ws.take(2LL * dense_pitch(p.K) * p.M), p.M, p.K);
-  if (!w_ok) align_add(a, w, ws.take(2LL * dense_pitch(p.K) * p.N), p.N, p.K);
+  if (!x_ok) align_add(a, x, ws.take(2LL * dense_pitch(p.K) * p.M), p.M, p.K, sms);
+  if (!w_ok) align_add(a, w, ws.take(2LL * dense_pitch(p.K) * p.N), p.N, p.K, sms);
   const DenseChoice c = dense_choice(p.M, p.N, p.K, sms);
   p.direct_aux = p.aux && !dense_aligned(p.aux, p.ldaux);
   if (dense_copies_residual(c, x_ok, w_ok, !p.direct_aux)) {
     DenseOperand r{p.aux, p.ldaux};
-    align_add(a, r, ws.take(2LL * dense_pitch(p.N) * p.M), p.M, p.N);
+    align_add(a, r, ws.take(2LL * dense_pitch(p.N) * p.M), p.M, p.N, sms);
     p.aux = r.p;
     p.ldaux = r.ld;
     p.direct_aux = false;
@@ -412,8 +411,8 @@ inline int launch_dense_backward(const DenseGradParams& q, const DenseGradPlan& 
   DenseOperand x = q.x, w = q.w, dz = q.dy;
   int r;
   AlignRows a{};
-  if (g.copy_x) align_add(a, x, g.xs, q.M, q.K);
-  if (g.copy_w) align_add(a, w, g.ws, q.N, q.K);
+  if (g.copy_x) align_add(a, x, g.xs, q.M, q.K, sms);
+  if (g.copy_w) align_add(a, w, g.ws, q.N, q.K, sms);
   if (g.make_dz || q.db || a.n > 0) {
     SlopeParams s{};
     s.dy = q.dy.p; s.ldy = q.dy.ld;

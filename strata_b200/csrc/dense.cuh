@@ -148,7 +148,7 @@ inline int launch_dense_t(const DenseOperand& A, const DenseOperand& B, const De
 
 // Forward pass on pairs of CTAs: a kernel for each activation, with and without a residual. One kernel that reads both
 // from its parameters keeps the registers and the code of all of them in its loop; 262144 x 2048, K = 512, microseconds
-// that way / this: no activation 431 / 415, silu 539 / 435, gelu 673 / 481 (473 with the shorter fit), with a residual
+// that way / this: no activation 431 / 415, silu 539 / 435, gelu (a longer formula then) 673 / 481, with a residual
 // 658 / 590. The residual a tile ahead, in boxes of 64 columns: 590 -> 537; such boxes without a residual: silu 435 ->
 // 497.
 template <int EPI, typename T, bool AUX>

@@ -1,0 +1,69 @@
+"""The dense layer's activations where their values are small: errors relative to the value itself, in every form of the
+product (dot products, mma.sync, tiles, split sums, pairs of CTAs).
+
+Tolerance beside the result's own rounding u |y| (u = finfo.eps / 2):
+  gelu   Phi(-a) = 2^q(a) with a fitted q. The formula in 64 bits on 800001 points: bf16 off by 8.1e-5 of |y| for z > -4,
+         2.2e-4 for z > -6, 3.8e-3 for z > -8, 5.2 % for z > -9, 25 % for z > -10 and 4.5e-23 below; fp16 by 6.2e-6 of
+         |y| for z > -4 and 4e-10 below. Evaluated in fp32 (seven steps, |q| up to 17 at -4, 29 at -6 and 50 at -8, each
+         2^-24 |q| ln 2 at most, and exp2 to 2^-22): 6e-6 more at -4, 1e-5 at -6, 2e-5 at -8
+and what the type cannot hold: half of fp16's smallest step, 2^-25; in bf16, whose smallest normal number is fp32's, what
+lies below 13 2^-126 (a value times a power of two that is flushed to zero)."""
+import pytest
+import torch
+
+from tests.test_linear_act_gpu import BF, HF
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from strata_b200 import ops
+    return ops
+
+
+def act64(z, act):
+    if act == "gelu":        # (torch.special.ndtr takes 1 + erf, whose 2^-53 is 5 % of Phi(-8))
+        return z * torch.special.erfc(z * -(0.5 ** 0.5)) / 2
+
+
+def forms(ops, z, act):
+    """act(z) by every form of the product: z [P] of a 16-bit type stands on the diagonal of a weight of ones and zeros."""
+    one = torch.ones(1, 1, device="cuda", dtype=z.dtype)
+    eye = lambda n, k: torch.eye(n, k, device="cuda", dtype=z.dtype)
+    P = z.numel()
+    assert P % 2000 == 0
+    yield ops.linear_act(z[:, None], one, None, act)[:, 0]                                        # tiles
+    yield torch.cat([ops.linear_act(part.view(4, -1), eye(P // 8, P // 8), None, act).flatten()
+                     for part in z.view(2, -1)])                                                  # four rows
+    yield torch.cat([ops.linear_act(part.view(20, -1), eye(P // 40, P // 40), None, act).flatten()
+                     for part in z.view(2, -1)])                                                  # mma.sync
+    wide = torch.cat([z.view(40, -1), torch.zeros(40, 8192 - P // 40, device="cuda", dtype=z.dtype)], 1)
+    yield ops.linear_act(wide, eye(P // 40, 8192), None, act).flatten()                           # split sums
+    big = z.view(-1, 100)
+    big = big.repeat(40000 // len(big), 1)
+    y = ops.linear_act(big, eye(600, 100), None, act)[:, :100]                                    # pairs of CTAs
+    yield y[:P // 100].flatten()
+
+
+def near(got, z, act, rel, rest=0.0):
+    t, z = got.dtype, z.double()
+    want = act64(z, act)
+    u = torch.finfo(t).eps / 2
+    least = 2.0 ** -25 if t == HF else 13 * 2.0 ** -126
+    over = (got.double() - want).abs() - ((rel + u * (1 + rel)) * want.abs() + least + rest)
+    i = int(over.argmax())
+    assert float(over.max()) <= 0, f"{act}({float(z[i]):.5g}) = {float(got[i]):.5g}, not {float(want[i]):.5g}"
+
+
+@pytest.mark.parametrize("t", [BF, HF])
+def test_gelu_in_its_tail(ops, t):
+    z = torch.cat([torch.linspace(-14, 0, 12001)[:-1], torch.linspace(0, 8, 2000), -torch.logspace(-5, 1.14, 2000)])
+    z = z.to(t).cuda()
+    steps = [(-4, 1e-4), (-6, 2.5e-4), (-8, 4e-3), (-9, 6e-2), (-10, 0.3)] if t == BF else [(-4, 1.3e-5)]
+    rel = torch.zeros(z.shape, dtype=torch.float64, device="cuda")
+    for above, r in reversed(steps):
+        rel[z > above] = r
+    rest = 5e-23 if t == BF else 5e-10
+    for y in forms(ops, z, "gelu"):
+        near(y, z, "gelu", rel, rest)

@@ -63,25 +63,24 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return y;
 }
 // x / (1 + 2^v) of a pair with one reciprocal for both: 1 / a = b / (a b). 2^v must stay below 2^63, and v may not be
-// NaN: it would reach the other value.
+// NaN: it would reach the other value. b times the reciprocal comes first: x b may leave fp32 where x / a does not.
 __device__ __forceinline__ uint64_t dense_sigmoid_pair(uint64_t x, uint64_t v) {
   float v0, v1, d0, d1;
   unpack2(v, v0, v1);
   unpack2(fadd2(pack2(fast_exp2(v0), fast_exp2(v1)), pack2(1.f, 1.f)), d0, d1);
   const float r = fast_rcp(d0 * d1);
-  return fmul2(fmul2(x, pack2(d1, d0)), pack2(r, r));
+  return fmul2(x, fmul2(pack2(d1, d0), pack2(r, r)));
 }
 
 // The forward pass's gelu: max(x, 0) - a Phi(-a), a = |x|, with Phi(-a) = 2^q(a): the logarithm of the tail is smooth,
-// so a polynomial in a has it over all magnitudes at once, nothing cancels, and one special-function instruction a value
-// is enough (x / (1 + e^-L(x)) with a fitted logit takes three a pair, and an erf of absolute accuracy has nothing
-// right in the tail). Fitted for the least largest error, relative to |gelu| where a type can see that (half steps: bf16
-// 3.9e-3, fp16 4.9e-4):
+// so a polynomial in a has it over all magnitudes at once, nothing cancels, and one special-function instruction a
+// value is enough (x / (1 + e^-L(x)) with a fitted logit takes three a pair, and an erf of absolute accuracy has
+// nothing right in the tail). Fitted for the least largest error, relative to |gelu| where a type can see that (half
+// steps: bf16 3.9e-3, fp16 4.9e-4):
 //   bf16   8.1e-5 for x > -4, 2.2e-4 to -6, 3.8e-3 to -8, 5 % to -9; below -10, where |gelu| < 1e-22, the right order
 //   fp16   6.3e-6 for x > -4, off by 4e-10 at most below (half of the smallest step: 3e-8)
-// 262144 x 2048, K = 512, bf16: 465 us with seven coefficients, 493 with nine (one fit for both types), 495 with the
-// fitted logit of five.
-// (coefficients: in -a, which stops at FAR)
+// 262144 x 2048, K = 512, bf16: 465 us with seven coefficients, 493 with nine (one fit for both types), 495 with a
+// fitted logit of five. (coefficients: in -a, which stops at FAR)
 template <typename T> struct GeluFit;
 template <> struct GeluFit<__nv_bfloat16> {
   static constexpr int N = 7;

@@ -2,12 +2,12 @@
 product (dot products, mma.sync, tiles, split sums, pairs of CTAs).
 
 Tolerance beside the result's own rounding u |y| (u = finfo.eps / 2):
-  gelu   Phi(-a) = 2^q(a) with a fitted q. The formula in 64 bits on 800001 points: bf16 off by 8.1e-5 of |y| for z > -4,
-         2.2e-4 for z > -6, 3.8e-3 for z > -8, 5.2 % for z > -9, 25 % for z > -10 and 4.5e-23 below; fp16 by 6.2e-6 of
-         |y| for z > -4 and 4e-10 below. Evaluated in fp32 (seven steps, |q| up to 17 at -4, 29 at -6 and 50 at -8, each
-         2^-24 |q| ln 2 at most, and exp2 to 2^-22): 6e-6 more at -4, 1e-5 at -6, 2e-5 at -8
-and what the type cannot hold: half of fp16's smallest step, 2^-25; in bf16, whose smallest normal number is fp32's, what
-lies below 13 2^-126 (a value times a power of two that is flushed to zero)."""
+  gelu   Phi(-a) = 2^q(a) with a fitted q. The formula in 64 bits on 800001 points: bf16 off by 8.1e-5 of |y| for
+         z > -4, 2.2e-4 for z > -6, 3.8e-3 for z > -8, 5.2 % for z > -9, 25 % for z > -10 and 4.5e-23 below; fp16 by
+         6.2e-6 of |y| for z > -4 and 4e-10 below. Evaluated in fp32 (seven steps, |q| up to 17 at -4, 29 at -6 and 50 at
+         -8, each 2^-24 |q| ln 2 at most, and exp2 to 2^-22): 6e-6 more at -4, 1e-5 at -6, 2e-5 at -8
+and what the type cannot hold: half of fp16's smallest step, 2^-25; in bf16, whose smallest normal number is fp32's,
+what lies below 13 2^-126 (a value times a power of two that is flushed to zero)."""
 import pytest
 import torch
 
@@ -23,12 +23,14 @@ def ops():
 
 
 def act64(z, act):
+    if act == "silu":
+        return z / (1 + torch.exp(-z))
     if act == "gelu":        # (torch.special.ndtr takes 1 + erf, whose 2^-53 is 5 % of Phi(-8))
         return z * torch.special.erfc(z * -(0.5 ** 0.5)) / 2
 
 
 def forms(ops, z, act):
-    """act(z) by every form of the product: z [P] of a 16-bit type stands on the diagonal of a weight of ones and zeros."""
+    """act(z) by every form of the product: z [P] of a 16-bit type against a weight of ones on the diagonal."""
     one = torch.ones(1, 1, device="cuda", dtype=z.dtype)
     eye = lambda n, k: torch.eye(n, k, device="cuda", dtype=z.dtype)
     P = z.numel()
@@ -67,3 +69,20 @@ def test_gelu_in_its_tail(ops, t):
     rest = 5e-23 if t == BF else 5e-10
     for y in forms(ops, z, "gelu"):
         near(y, z, "gelu", rel, rest)
+
+
+@pytest.mark.parametrize("act,low", [("silu", -50.0), ("gelu", -6.0)])
+@pytest.mark.parametrize("M,N,K", [(3, 40, 64), (20, 40, 512), (64, 72, 4096), (200, 72, 64), (40000, 512, 64)])
+def test_a_large_value_beside_a_small_one(ops, act, low, M, N, K):
+    """Two columns share a reciprocal: the finite result of the one does not depend on the other's denominator. (silu
+    keeps the value of -40 below that: 2e-16.)"""
+    x, w = (torch.zeros(s, K, device="cuda", dtype=BF) for s in (M, N))
+    for big in (1e25, 1e37):
+        for first in (0, 1):
+            b = torch.full((N,), low, device="cuda")
+            b[first::2] = big
+            want = act64(b.double(), act).to(BF)
+            y = ops.linear_act(x, w, b, act)
+            assert torch.equal(y[:, first::2], want[first::2].expand(M, -1))
+            small = (y[:, 1 - first::2].double() - want[1 - first::2].double()).abs()
+            assert bool((small <= 2 * torch.finfo(BF).eps * want[1 - first::2].double().abs() + 2e-16).all())

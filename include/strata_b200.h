@@ -69,7 +69,7 @@ int strata_linear_bf16(const void* x, int64_t ldx, const void* w, int64_t ldw, c
 /* Activations of strata_linear_act. */
 #define STRATA_ACT_NONE 0
 #define STRATA_ACT_GELU 1      /* z Phi(z) */
-#define STRATA_ACT_GELU_TANH 2 /* its tanh form, with the hardware's tanh as STRATA_EPI_GELU */
+#define STRATA_ACT_GELU_TANH 2 /* its tanh form */
 #define STRATA_ACT_SILU 3
 #define STRATA_ACT_RELU 4
 

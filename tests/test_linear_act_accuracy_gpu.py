@@ -6,8 +6,13 @@ Tolerance beside the result's own rounding u |y| (u = finfo.eps / 2):
          z > -4, 2.2e-4 for z > -6, 3.8e-3 for z > -8, 5.2 % for z > -9, 25 % for z > -10 and 4.5e-23 below; fp16 by
          6.2e-6 of |y| for z > -4 and 4e-10 below. Evaluated in fp32 (seven steps, |q| up to 17 at -4, 29 at -6 and 50 at
          -8, each 2^-24 |q| ln 2 at most, and exp2 to 2^-22): 6e-6 more at -4, 1e-5 at -6, 2e-5 at -8
+  gelu_tanh, silu   z / (1 + 2^-w): four roundings or rounded constants in w, 2^-24 |w| ln 2 each, below 2^-22 |w| in
+         all; exp2 to 2^-22, the reciprocal to 2^-23, four more roundings: below 2^-20 together. They stand still below
+         -7.5 (at 4.017e-18; with its rounding to bf16, 2^-8 of it, 4.033e-18) and -40 (1.7e-16)
 and what the type cannot hold: half of fp16's smallest step, 2^-25; in bf16, whose smallest normal number is fp32's,
 what lies below 13 2^-126 (a value times a power of two that is flushed to zero)."""
+import math
+
 import pytest
 import torch
 
@@ -27,6 +32,7 @@ def act64(z, act):
         return z / (1 + torch.exp(-z))
     if act == "gelu":        # (torch.special.ndtr takes 1 + erf, whose 2^-53 is 5 % of Phi(-8))
         return z * torch.special.erfc(z * -(0.5 ** 0.5)) / 2
+    return z / (1 + torch.exp(-2 * (2 / math.pi) ** 0.5 * (z + 0.044715 * z ** 3)))
 
 
 def forms(ops, z, act):
@@ -71,7 +77,18 @@ def test_gelu_in_its_tail(ops, t):
         near(y, z, "gelu", rel, rest)
 
 
-@pytest.mark.parametrize("act,low", [("silu", -50.0), ("gelu", -6.0)])
+@pytest.mark.parametrize("act,far,least", [("gelu_tanh", -9, 4.05e-18), ("silu", -50, 1.72e-16)])
+@pytest.mark.parametrize("t", [BF, HF])
+def test_logistic_forms_in_their_tail(ops, act, far, least, t):
+    z = torch.cat([torch.linspace(far, 0, 12001)[:-1], torch.linspace(0, 8, 2000), -torch.logspace(-5, 4, 2000)])
+    z = z.to(t).cuda()
+    d = z.double()
+    w = (d if act == "silu" else 2 * (2 / math.pi) ** 0.5 * (d + 0.044715 * d ** 3)) / math.log(2)
+    for y in forms(ops, z, act):
+        near(y, z, act, 2.0 ** -20 + w.abs().clamp(max=100) * 2.0 ** -22, least)
+
+
+@pytest.mark.parametrize("act,low", [("silu", -50.0), ("gelu", -6.0), ("gelu_tanh", -5.0)])
 @pytest.mark.parametrize("M,N,K", [(3, 40, 64), (20, 40, 512), (64, 72, 4096), (200, 72, 64), (40000, 512, 64)])
 def test_a_large_value_beside_a_small_one(ops, act, low, M, N, K):
     """Two columns share a reciprocal: the finite result of the one does not depend on the other's denominator. (silu

@@ -177,7 +177,8 @@ __device__ __forceinline__ float qk_group_sum(float v) {
   return v;
 }
 
-// One head's vector of this lane: y of x, or dx of x and dy = gr and its part of dw (if it counts: not padding).
+// One head's vector of this lane: y of x, or dx of x and dy = gr and its part of dw (if it counts: a head that exists,
+// of a token that is not padding).
 template <typename T, int G, int TAB, bool ADJ, bool GRAD, int N>
 __device__ __forceinline__ uint4 qk_vector(const uint4& xr, const uint4& gr, const float (&w)[8], const float (&c)[N],
                                            const float (&s)[N], int partner, bool counts, float inv, float eps,
@@ -399,8 +400,9 @@ __global__ void __launch_bounds__(256, GRAD ? 2 : 4) qk_norm_rope_kernel(const Q
     };
     auto round = [&](uint32_t slot, int r, int k, int h) {
       const uint4 xr = qk_got(slot + r * 512), gr = GRAD ? qk_got(slot + (R + r) * 512) : xr;
-      uint4 o = qk_vector<T, G, TAB, ADJ, GRAD>(xr, gr, w, c, s, partner, TAB == QK_NO_TABLE || row >= 0, inv, p.eps,
-                                               sums[k]);
+      // (a slot without a head holds zeros, whose 1 / r has no bound but eps: 0 times infinity where that is 0)
+      const bool counts = GRAD && lane_on && m < M && h < lim(k) && (TAB == QK_NO_TABLE || row >= 0);
+      uint4 o = qk_vector<T, G, TAB, ADJ, GRAD>(xr, gr, w, c, s, partner, counts, inv, p.eps, sums[k]);
       if (TAB != QK_NO_TABLE && p.positions != nullptr && row < 0) {     // padding: zero; behind the table: NaN
         const uint32_t u = row == -1 ? 0u : 0x7FFF7FFFu;
         o = make_uint4(u, u, u, u);

@@ -211,15 +211,15 @@ __device__ __forceinline__ uint4 qk_vector(const uint4& xr, const uint4& gr, con
       sq += __shfl_xor_sync(0xffffffffu, sq, ofs);
       dot += __shfl_xor_sync(0xffffffffu, dot, ofs);
     }
-    // dx = r h - x r^3 mean(h x), h = g w;  dw += g x r
-    const float rs = rsqrtf(fmaf(sq, inv, eps)), b = -rs * rs * rs * (dot * inv);
+    // dx = r (h - x r^2 mean(h x)), h = g w;  dw += g (x r). (r^3 by itself leaves fp32 at an rms of 1e13 or 1e-13)
+    const float rs = rsqrtf(fmaf(sq, inv, eps)), b = -(rs * (dot * inv)) * rs;
     const uint64_t r2 = pack2(rs, rs), b2 = pack2(b, b);
     if (counts) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sums[i] = ffma2(fmul2(g[i], x[i]), r2, sums[i]);
+      for (int i = 0; i < 4; ++i) sums[i] = ffma2(g[i], fmul2(x[i], r2), sums[i]);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = ffma2(h[i], r2, fmul2(x[i], b2));
+    for (int i = 0; i < 4; ++i) h[i] = fmul2(ffma2(x[i], b2, h[i]), r2);
     return qk_pack<T, ADJ>(h);
   }
 }

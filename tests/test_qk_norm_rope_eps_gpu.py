@@ -1,4 +1,5 @@
-"""The gradients of qk_norm_rope where eps does not hold 1 / rms down: eps = 0, heads that leave slots of a warp empty."""
+"""The gradients of qk_norm_rope where eps does not hold 1 / rms down: eps = 0, heads that leave slots of a warp empty,
+values from one end of bf16 to the other."""
 import pytest
 import torch
 
@@ -26,3 +27,26 @@ def test_eps_of_zero(ops, M, hq, hk, hd, table, t):
     for adjacent in (True, False):
         at = None if rot is None else torch.arange(M, device="cuda").flip(0)
         check(ops, d, adjacent, at, eps=0.0, **({} if rot is None else dict(positions=at)))
+
+
+# (the squares of a head and their sum stay inside fp32)
+@pytest.mark.parametrize("power", [-54, -44, 42, 54])
+@pytest.mark.parametrize("hq,hk,hd,rot", [(3, 1, 64, 64), (12, 12, 64, None), (16, 4, 128, 64)])
+def test_large_and_small_heads(ops, power, hq, hk, hd, rot):
+    """dx has both of its terms, dw its sum, at any size of q and k."""
+    M = 50
+    d = data(M, hq, hk, hd, BF, rot=rot, rows=M, f32=True, seed=hq)
+    d["q"], d["k"] = d["q"] * 2.0 ** power, d["k"] * 2.0 ** power
+    for adjacent in (True, False):
+        check(ops, d, adjacent, torch.arange(M, device="cuda"), eps=0.0)
+    if power > 0:
+        check(ops, d, True, torch.arange(M, device="cuda"))
+
+
+def test_heads_of_zeros(ops):
+    """r = eps^-1/2 and nothing else is left."""
+    d = data(9, 4, 2, 64, BF)
+    d["q"], d["k"] = d["q"].clone(), d["k"].clone()
+    d["q"][3:5], d["k"][4] = 0, 0
+    for eps in (1e-6, 1e-26, 1e-30):
+        check(ops, d, True, eps=eps)

@@ -301,9 +301,9 @@ int strata_adaln_rows_bf16(const void* x, int64_t ldx, const void* y, int64_t ld
  * (qk_norm_pixel of screamcast/strata_wrappers.py:437, non-affine). */
 int strata_qk_norm_rows_bf16(void* qkv, int64_t ld, int64_t M, int C, float eps, void* stream);
 
-/* Per-head RMS norm and rotation of q and k in one pass: y = R (x (mean x^2 + eps)^-1/2 w), for M tokens of heads_q and
- * heads_k heads of head_dim channels (a multiple of 8, at most 256) in one 16-bit type. Element (m, head, c) of an
- * operand lies at base + m*st + head*sh + c; strides in elements, multiples of 8, bases 16-byte aligned. w_q, w_k:
+/* Per-head RMS norm and rotation of q and k in one pass: y = R (x (mean x^2 + eps)^-1/2 w), eps >= 0, for M tokens of
+ * heads_q and heads_k heads of head_dim channels (a multiple of 8, at most 256) in one 16-bit type. Element (m, head,
+ * c) of an operand lies at base + m*st + head*sh + c; strides in elements, multiples of 8, bases 16-byte aligned. w_q, w_k:
  * [head_dim] fp32, 16-byte aligned, or NULL. R turns the first `rot` channels of a head by the (cos, sin) pairs of the
  * token's row of table [table_rows, rot/2] (IEEE half, or float with table_f32; 16-byte aligned; NULL: no rotation):
  * pairs (2i, 2i+1) with `adjacent`, rot a multiple of 8, else (i, i + rot/2), rot a multiple of 16. The row is

@@ -995,7 +995,7 @@ static int qk_params(QkParams& p, int heads_q, int heads_k, int head_dim, int ro
                      int table_f32, int table_rows, const void* positions, int positions_64, int tokens_per_tile, int hw,
                      int64_t M, float eps, int dtype) {
   if (M < 0 || M > 0x7FFF0000 || heads_q <= 0 || heads_k <= 0 || heads_q > 65536 || heads_k > 65536 || head_dim <= 0 ||
-      (dtype != STRATA_BF16 && dtype != STRATA_F16))
+      !(eps >= 0.f && eps < INFINITY) || (dtype != STRATA_BF16 && dtype != STRATA_F16))
     return STRATA_ERR_ARG;
   if (head_dim % 8 != 0 || head_dim > 256) return STRATA_ERR_UNSUPPORTED;
   if (table) {

@@ -6,6 +6,8 @@ nothing falls back to PyTorch kernels.
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import _lib
@@ -726,8 +728,10 @@ def _heads_out(t: torch.Tensor, name: str, like: torch.Tensor):
     return t3, token, head
 
 
-def _qk_arguments(q, k, q_weight, k_weight, rope_cs, positions, tokens_per_tile, hw, interleaved):
+def _qk_arguments(q, k, q_weight, k_weight, rope_cs, positions, tokens_per_tile, hw, interleaved, eps):
     """What both directions check: (heads_q, heads_k, head_dim, tokens, tensors, the C arguments from rot to hw)."""
+    if not 0.0 <= eps < math.inf:
+        raise ValueError(f"eps must be finite and not negative, got {eps}")
     _like(k, "k", q)
     qs, ks = q.shape, k.shape
     if len(qs) < 3 or len(ks) != len(qs):
@@ -792,7 +796,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
                  positions: torch.Tensor | None = None, tokens_per_tile: int | None = None, hw: int | None = None,
                  eps: float = 1e-6, interleaved: bool = True, out=None):
     """RMS norm of every q and k head and the rotary turn behind it, in one pass over both: returns (q', k') with
-    x' = R (x * rsqrt(mean(x^2) + eps) * weight).
+    x' = R (x * rsqrt(mean(x^2) + eps) * weight), eps >= 0.
 
     q [..., heads_q, head_dim], k [..., heads_k, head_dim]: bfloat16 or float16, the same tokens, views of a packed qkv
     matrix included; head_dim a multiple of 8 up to 256. q_weight, k_weight: [head_dim] fp32, or None for a plain norm.
@@ -804,7 +808,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
     allowed. The gradients are qk_norm_rope_backward's; torch.ops.strata_b200.qk_norm_rope is the differentiable form."""
     dtype = _require_16bit(q, "q")
     hq, hk, hd, M, keep, args = _qk_arguments(q, k, q_weight, k_weight, rope_cs, positions, tokens_per_tile, hw,
-                                              interleaved)
+                                              interleaved, eps)
     yq, yk = (q.new_empty(q.shape), k.new_empty(k.shape)) if out is None else out
     if not M:
         return yq, yk
@@ -835,7 +839,7 @@ def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k
     weights). A padding token has no gradient and no part in the weights'."""
     dtype = _require_16bit(q, "q")
     hq, hk, hd, M, keep, args = _qk_arguments(q, k, q_weight, k_weight, rope_cs, positions, tokens_per_tile, hw,
-                                              interleaved)
+                                              interleaved, eps)
     xq, xk = q.new_empty(q.shape), k.new_empty(k.shape)
     wq, wk = keep[:2]
     dwq = None if wq is None else wq.new_empty(hd)

@@ -171,6 +171,37 @@ def _packed_rows(t: torch.Tensor, cols: int, name: str):
     return t, rows, row if rows > 1 else cols
 
 
+def _span(start: int, run: int, *dims):
+    """Memory of a strided operand: runs of `run` bytes at start + i * stride + ..., dims (stride, count), long strides
+    first."""
+    dims = tuple(sorted(((stride, n) for stride, n in dims if n > 1 and stride), reverse=True))
+    return start, start + run + sum(stride * (n - 1) for stride, n in dims), dims
+
+
+def _inner(a, at: int = 0):
+    """Slice number `at` of a span along its longest stride."""
+    stride, n = a[2][0]
+    return a[0] + at * stride, a[1] - (n - 1 - at) * stride, a[2][1:]
+
+
+def _meet(a, b) -> bool:
+    """Whether two spans share a byte. Column blocks of one matrix, or heads of one packed row, lie between one another
+    and do not. (Spans that would take thousands of slices to tell apart count as sharing.)"""
+    if a[1] <= b[0] or b[1] <= a[0]:
+        return False
+    if not a[2] and not b[2]:
+        return True
+    if not a[2] or (b[2] and b[2][0][0] > a[2][0][0]):
+        a, b = b, a
+    stride, n = a[2][0]
+    one = _inner(a)
+    least = 0
+    if b[2] and b[2][0][0] == stride:       # slices i of a and j of b: as slice i - j of a and the first of b
+        least, b = 1 - b[2][0][1], _inner(b)
+    first, last = max(least, (b[0] - one[1]) // stride + 1), min(n - 1, (b[1] - one[0] - 1) // stride)
+    return last - first > 4096 or any(_meet(_inner(a, i), b) for i in range(first, last + 1))
+
+
 _MOST = 0x7FFF0000      # rows, columns and tokens that the kernels count with 32 bits
 
 
@@ -203,8 +234,8 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     multiple of eight the results are views of rows that are (not contiguous): the next call reads them without a copy.
 
     save_preact: returns (y, z); linear_act_backward needs z for any activation but "none". out: where y goes, [M, N]
-    with unit inner stride; it may be the residual, no other operand. The gradients are linear_act_backward's;
-    torch.ops.strata_b200.linear_act is the differentiable form."""
+    with unit inner stride; it may be the residual, and shares no memory with an operand otherwise. The gradients are
+    linear_act_backward's; torch.ops.strata_b200.linear_act is the differentiable form."""
     dtype = _require_16bit(x, "x")
     act = _activation(activation)
     _like(weight, "weight", x)
@@ -228,9 +259,15 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
         _like(out, "out", x)
         if out.shape != (M, N) or (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
             raise ValueError(f"out must be [{M}, {N}] with unit inner stride")
-        if out.data_ptr() in (x2.data_ptr(), w2.data_ptr()) and M:
-            raise ValueError("out may be the residual, but not x or weight")
         y, ldy = out, out.stride(0) if M > 1 else N
+        rows = lambda t, m, ld, cols: _span(t.data_ptr(), 2 * cols, (2 * ld, m))
+        to = rows(y, M, ldy, N)
+        if M and (_meet(to, rows(x2, M, ldx, K)) or _meet(to, rows(w2, N, ldw, K))):
+            raise ValueError("out may be the residual, but not x or weight, nor share memory with them")
+        if M and r2 is not None and (r2.data_ptr(), ldr) != (to[0], ldy) and _meet(to, rows(r2, M, ldr, N)):
+            raise ValueError("out may be the residual itself, but not share a part of its memory")
+        if M and bias is not None and _meet(to, _span(bias.data_ptr(), 4 * N)):
+            raise ValueError("out may not share memory with bias")
     z, ldz = _padded_rows(x, shape) if save_preact else (None, 0)
     if M:
         lib = _lib.load()

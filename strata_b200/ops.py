@@ -842,7 +842,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
     of rot (a multiple of 16). A token's row: positions [tokens] (int32 / int64; negative: a padding token, its outputs
     are zero; one behind the table gives NaN and device status 107), else as in qkv_rope
     m // tokens_per_tile * hw + m % hw (default: token m has row m). out: (q', k') to write to, q and k themselves
-    allowed. The gradients are qk_norm_rope_backward's; torch.ops.strata_b200.qk_norm_rope is the differentiable form."""
+    allowed (in this order), other memory of an operand not. The gradients are qk_norm_rope_backward's; torch.ops.strata_b200.qk_norm_rope is the differentiable form."""
     dtype = _require_16bit(q, "q")
     hq, hk, hd, M, keep, args = _qk_arguments(q, k, q_weight, k_weight, rope_cs, positions, tokens_per_tile, hw,
                                               interleaved, eps)
@@ -855,6 +855,15 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
         yq_token, yq_head, yk_token, yk_head = hq * hd, hd, hk * hd, hd
     else:
         (_, yq_token, yq_head), (_, yk_token, yk_head) = _heads_out(yq, "out[0]", q), _heads_out(yk, "out[1]", k)
+        heads = lambda t, token, head, n: _span(t.data_ptr(), 2 * hd, (2 * token, M), (2 * head, n))
+        xs = heads(q3, q_token, q_head, hq), heads(k3, k_token, k_head, hk)
+        ys = heads(yq, yq_token, yq_head, hq), heads(yk, yk_token, yk_head, hk)
+        own = ((yq.data_ptr(), yq_token, yq_head) == (q3.data_ptr(), q_token, q_head),
+               (yk.data_ptr(), yk_token, yk_head) == (k3.data_ptr(), k_token, k_head))
+        if _meet(*ys) or any(not own[j] and _meet(ys[i], xs[j]) for i in (0, 1) for j in (0, 1)):
+            raise ValueError("out may be q and k themselves, each its own, and shares no other memory with them or in itself")
+        if any(t is not None and _meet(y, _span(t.data_ptr(), t.numel() * t.element_size())) for y in ys for t in keep):
+            raise ValueError("out may not share memory with the weights, rope_cs or positions")
     wq, wk = keep[:2]
     with _lib.on_device(q):
         code = _lib.load().strata_qk_norm_rope(

@@ -20,9 +20,10 @@ def host(monkeypatch):
     """Lets host tensors through to where the library would be called."""
     monkeypatch.setattr(ops, "_require_16bit", lambda t, name: ops._DTYPES[t.dtype])
 
-    def load():
+    def launch(*_):
         raise Launched
-    monkeypatch.setattr(_lib, "load", load)
+    monkeypatch.setattr(_lib, "load", launch)
+    monkeypatch.setattr(_lib, "on_device", launch)
 
 
 @pytest.fixture
@@ -87,3 +88,33 @@ def test_out_that_shares_memory_with_an_operand(host):
     b = torch.zeros(24)
     with pytest.raises(ValueError, match="bias"):
         run(b.view(BF).view(2, 24), None, x[:2], b)
+
+
+def test_outputs_that_share_memory_with_q_or_k(host):
+    """In place in this order, and into other heads and tokens of the same rows; nothing that is yet to be read."""
+    M, h, hd = 12, 4, 16
+    packed = torch.zeros(M, 5 * h * hd, dtype=BF)
+    q, k, v, a, b = (packed[:, i * h * hd:(i + 1) * h * hd].view(M, h, hd) for i in range(5))
+    other, more = torch.zeros(M, h, hd, dtype=BF), torch.zeros(M, h, hd, dtype=BF)
+    woven = torch.zeros(M, h, 3, hd, dtype=BF)          # the heads of q, k and v in turn
+    run = lambda out, q=q, k=k, **more: ops.qk_norm_rope(q, k, out=out, **more)
+    for out in ((q, k), (a, b), (b, other), (q, b), (a, k), (other, more)):
+        with pytest.raises(Launched):
+            run(out)
+    for out in ((woven[:, :, 0], woven[:, :, 1]), (woven[:, :, 2], woven[:, :, 1]), (other, more)):
+        with pytest.raises(Launched):
+            run(out, woven[:, :, 0], woven[:, :, 1])
+    with pytest.raises(Launched):
+        run((q[:, :1], k[:, 3:]), q[:, :1], k[:, 3:])
+    step = packed[1:, :h * hd].view(M - 1, h, hd)
+    square = torch.zeros(h, h, hd, dtype=BF)
+    for out, x in (((k, q), (q, k)), ((k, a), (q, k)), ((a, q), (q, k)), ((a, a), (q, k)), ((q, q), (q, k)),
+                   ((other, packed[:, 8:72].view(M, h, hd)), (q, k)), ((step, a[1:]), (q[:-1], k[:-1])),
+                   ((a[1:], step), (q[:-1], k[:-1])), ((a, other), (q, a[:, :, :])), ((q, other), (q, q)),
+                   ((square.transpose(0, 1), other[:h]), (square, k[:h])),
+                   ((woven[:, :, 1], woven[:, :, 0]), (woven[:, :, 0], woven[:, :, 1]))):
+        with pytest.raises(ValueError, match="themselves"):
+            run(out, *x)
+    w = torch.zeros(hd)
+    with pytest.raises(ValueError, match="weights"):
+        ops.qk_norm_rope(q[:1, :2], k[:1, :2], w, out=(w.view(BF).view(1, 2, hd), other[:1, :2]))

@@ -238,7 +238,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
                  positions: Optional[torch.Tensor] = None, tokens_per_tile: Optional[int] = None,
                  hw: Optional[int] = None, eps: float = 1e-6,
                  interleaved: bool = True) -> tuple[torch.Tensor, torch.Tensor]:
-    """ops.qk_norm_rope, differentiable in q, k and the two weights."""
+    """ops.qk_norm_rope, differentiable in q, k and the two weights; a rope_cs that asks for a gradient is refused."""
     from . import ops
     return ops.qk_norm_rope(q, k, q_weight, k_weight, rope_cs=rope_cs, positions=positions,
                             tokens_per_tile=tokens_per_tile, hw=hw, eps=eps, interleaved=interleaved)
@@ -272,6 +272,8 @@ def _qk_norm_rope_backward_fake(dq, dk, q, k, q_weight, k_weight, rope_cs, posit
 
 def _qk_norm_rope_context(ctx, inputs, output):
     q, k, q_weight, k_weight, rope_cs, positions, *ctx.rest = inputs
+    if rope_cs is not None and rope_cs.requires_grad:
+        raise NotImplementedError("rope_cs has no gradient: detach it")
     _claim(ctx, q)
     ctx.save_for_backward(q, k, q_weight, k_weight, rope_cs, positions)
 

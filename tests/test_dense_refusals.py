@@ -118,3 +118,17 @@ def test_outputs_that_share_memory_with_q_or_k(host):
     w = torch.zeros(hd)
     with pytest.raises(ValueError, match="weights"):
         ops.qk_norm_rope(q[:1, :2], k[:1, :2], w, out=(w.view(BF).view(1, 2, hd), other[:1, :2]))
+
+
+def test_a_table_that_asks_for_a_gradient(cuda):
+    from strata_b200 import torch_ops  # noqa: F401  (registers the operators)
+    op = torch.ops.strata_b200.qk_norm_rope
+    q, k, cs = cuda(5, 4, 64), cuda(5, 2, 64), cuda(5, 32, 2, dtype=torch.float32)
+    op(q.requires_grad_(), k, None, None, cs)
+    cs.requires_grad_()
+    for one in (q, q.detach()):
+        with pytest.raises(NotImplementedError, match="rope_cs"):
+            op(one, k, None, None, cs)
+    with torch.no_grad():
+        op(q, k, None, None, cs)
+    op(q, k, None, None, cs.detach())

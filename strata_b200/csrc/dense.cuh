@@ -371,7 +371,7 @@ inline DenseGradSums dense_grad_sums(int M, int N, int sms) {
   const long long most = (M + 4LL * step - 1) / (4LL * step);
   if (blocks > most) blocks = most;
   g.rows_per_block = static_cast<int>((M + blocks - 1) / blocks);
-  g.blocks = (M + g.rows_per_block - 1) / g.rows_per_block;
+  g.blocks = static_cast<int>((M - 1LL + g.rows_per_block) / g.rows_per_block);     // (the sum may leave 32 bits)
   return g;
 }
 

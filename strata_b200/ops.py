@@ -210,6 +210,12 @@ def _countable(*sizes) -> None:
         raise ValueError(f"sizes up to {_MOST} are supported, got {sizes}")
 
 
+def _widths(weight) -> tuple[int, int]:
+    if weight.dim() != 2 or 0 in weight.shape:
+        raise ValueError(f"weight must be [N, K] with at least one row and column, got {tuple(weight.shape)}")
+    return weight.shape
+
+
 def _scratch(need: int, x):
     if need < 0:
         _lib.check(need, "workspace size")
@@ -230,8 +236,9 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
                residual: torch.Tensor | None = None, *, save_preact: bool = False, out: torch.Tensor | None = None):
     """y = residual + act(z), z = x @ weight.T + bias, in one pass: x [..., K], weight [N, K], residual and y [..., N] of
     one type (bfloat16 or float16), bias [N] fp32; activation one of "none", "gelu" (erf), "gelu_tanh", "silu", "relu".
-    Any number of rows, any widths and row strides. Sums and the epilogue are fp32, y is rounded once. Where N is no
-    multiple of eight the results are views of rows that are (not contiguous): the next call reads them without a copy.
+    Any number of rows, any widths from one on, any row strides. Sums and the epilogue are fp32, y is rounded once. Where
+    N is no multiple of eight the results are views of rows that are (not contiguous): the next call reads them without
+    a copy.
 
     save_preact: returns (y, z); linear_act_backward needs z for any activation but "none". out: where y goes, [M, N]
     with unit inner stride; it may be the residual, and shares no memory with an operand otherwise. The gradients are
@@ -239,9 +246,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     dtype = _require_16bit(x, "x")
     act = _activation(activation)
     _like(weight, "weight", x)
-    if weight.dim() != 2:
-        raise ValueError(f"weight must be [N, K], got {tuple(weight.shape)}")
-    N, K = weight.shape
+    N, K = _widths(weight)
     x2, M, ldx = _packed_rows(x, K, "x")
     w2, _, ldw = _packed_rows(weight, K, "weight")
     _countable(M, N, K)
@@ -299,9 +304,7 @@ def linear_act_backward(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tenso
     act = _activation(activation)
     _like(x, "x", grad)
     _like(weight, "weight", grad)
-    if weight.dim() != 2:
-        raise ValueError(f"weight must be [N, K], got {tuple(weight.shape)}")
-    N, K = weight.shape
+    N, K = _widths(weight)
     x2, M, ldx = _packed_rows(x, K, "x")
     w2, _, ldw = _packed_rows(weight, K, "weight")
     _countable(M, N, K)

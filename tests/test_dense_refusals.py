@@ -132,3 +132,13 @@ def test_a_table_that_asks_for_a_gradient(cuda):
     with torch.no_grad():
         op(q, k, None, None, cs)
     op(q, k, None, None, cs.detach())
+
+
+@pytest.mark.parametrize("N,K", [(0, 16), (8, 0), (0, 0)])
+def test_widths_of_zero(cuda, N, K):
+    for lead in ((4,), (0,), (2, 3)):
+        x, w, dy = cuda(*lead, K), cuda(N, K), cuda(*lead, N)
+        with pytest.raises(ValueError, match="at least one"):
+            ops.linear_act(x, w)
+        with pytest.raises(ValueError, match="at least one"):
+            ops.linear_act_backward(dy, x, w)

@@ -780,8 +780,9 @@ def _qk_arguments(q, k, q_weight, k_weight, rope_cs, positions, tokens_per_tile,
     hk = ks[-2]
     if ks[:-2] != qs[:-2] or ks[-1] != hd:
         raise ValueError(f"q {tuple(qs)} and k {tuple(ks)} must have the same tokens and head_dim")
-    if hd % 8 or not 8 <= hd <= 256 or not hq or not hk:
-        raise ValueError(f"head_dim must be a multiple of 8 up to 256 and both have heads, got {hq} + {hk} heads of {hd}")
+    if hd % 8 or not 8 <= hd <= 256 or not 0 < hq <= 65536 or not 0 < hk <= 65536:
+        raise ValueError("head_dim must be a multiple of 8 up to 256, and q and k have 1 to 65536 heads, got "
+                         f"{hq} + {hk} heads of {hd}")
     M = qs[0] if len(qs) == 3 else qs[:-2].numel()
     _countable(M)
     wq, wk = _f32_like(q_weight, "q_weight", hd, q), _f32_like(k_weight, "k_weight", hd, q)

@@ -142,3 +142,9 @@ def test_widths_of_zero(cuda, N, K):
             ops.linear_act(x, w)
         with pytest.raises(ValueError, match="at least one"):
             ops.linear_act_backward(dy, x, w)
+
+
+def test_more_heads_than_are_counted(cuda):
+    for hq, hk in ((65537, 1), (1, 65537)):
+        with pytest.raises(ValueError, match="65536 heads"):
+            ops.qk_norm_rope(cuda(0, hq, 8), cuda(0, hk, 8))

@@ -276,3 +276,12 @@ def device_status(reset: bool = True) -> int:
     st = c_int(0)
     check(load().strata_device_status(ctypes.byref(st), 1 if reset else 0), "strata_device_status")
     return st.value
+
+
+def raise_for_status(st: int, what: str) -> None:
+    """Raises for a device status that is not 0; `what` names the work that waits of kernels belong to."""
+    if st == 107:      # none of them, but the first thing that went wrong
+        raise RuntimeError("a position given to ops.qk_norm_rope lies behind its table (device status 107)")
+    if st != 0:
+        raise RuntimeError(f"{what} failed on the device (status {st}: "
+                           f"{'peer flag wait timed out' if st == 105 else 'kernel wait timed out'})")

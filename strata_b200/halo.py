@@ -187,12 +187,7 @@ class DistributedTileCopyHaloPadding(torch.nn.Module):
         """Synchronise and raise if a peer never reached a barrier (or any kernel timed out).
         Until this is called (it clears the condition) every padded tile produced after the
         failed barrier is NaN, so a missed poll cannot let a rollout continue on stale halos."""
-        st = _lib.device_status()
-        if st != 0:
-            if st == 107:      # not of an exchange, but the first thing that went wrong
-                raise RuntimeError("a position given to ops.qk_norm_rope lies behind its table (device status 107)")
-            raise RuntimeError(f"halo exchange failed on the device (status {st}: "
-                               f"{'peer flag wait timed out' if st == 105 else 'kernel wait timed out'})")
+        _lib.raise_for_status(_lib.device_status(), "halo exchange")
 
     # ---------------------------------------------------------------- field space (reference API)
     def forward(self, x: torch.Tensor) -> torch.Tensor:

@@ -198,9 +198,7 @@ class TiledBlockRunner:
         return y.view(tpr, tokens, C)
 
     def check_status(self) -> None:
-        st = _lib.device_status()
-        if st != 0:
-            raise RuntimeError(f"tiled block run failed on the device (status {st})")
+        _lib.raise_for_status(_lib.device_status(), "tiled block run")
 
     def close(self):
         if self._shared is not None:

@@ -21,8 +21,10 @@ them have gradients, for fine-tuning: `::linear_act` (a dense layer with its act
 
 Capturing a training step in a CUDA graph: torch ties a leaf's gradient accumulation to the stream on which its first
 living graph was built, and a captured backward pass that meets an accumulation of another stream ends the
-process. The two operators refuse the case they can see: a forward pass under capture whose leaves still have an eager
-graph of these operators on another stream (delete the losses and outputs of warm-up steps first).
+process. The two operators refuse the case they can see: a forward pass under capture whose leaves still have an
+accumulation that a pass of these operators met on another stream. Delete the losses and outputs of warm-up steps
+first; where something keeps the accumulations themselves (data-parallel wrappers do, as long as the module lives),
+warm up and capture on one stream: `torch.cuda.graph(g, stream=s)`.
 """
 from __future__ import annotations
 
@@ -149,7 +151,8 @@ def claim_leaves(next_functions, stream: int, capturing: bool) -> None:
         if node.metadata.setdefault(_STREAM_TAG, stream) != stream and capturing:
             raise RuntimeError(
                 "this forward pass is being captured, but an eager graph of the same leaves is alive on another stream: "
-                "its backward pass could not be captured. Delete what the eager passes returned (outputs, losses) first")
+                "its backward pass could not be captured. Delete what the eager passes returned (outputs, losses), "
+                "or capture on their stream where something else keeps the leaves' gradient accumulation")
 
 
 def _claim(ctx, x) -> None:

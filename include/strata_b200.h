@@ -80,8 +80,9 @@ int strata_linear_bf16(const void* x, int64_t ldx, const void* w, int64_t ldw, c
  * caller's to write in every row of y and preact (zeros may land there), which lets rows of such strides use TMA.
  * workspace: 256-byte aligned, of strata_linear_act_workspace_bytes bytes (negative: an error code), where an operand
  * counts as aligned when its address and its row stride are multiples of 16 bytes, or it is not there (others may be
- * copied there first). Up to 8 rows are one launch without workspace; M = 0 does nothing. Replaces the nn.Linear
- * calls of a block together with the operators around them (attn.proj, mlp.layers.*) in fine-tuning. */
+ * copied there first). Up to 8 rows are one launch without workspace; M = 0 does nothing, N and K are one at least.
+ * Replaces the nn.Linear calls of a block together with the operators around them (attn.proj, mlp.layers.*) in
+ * fine-tuning. */
 int64_t strata_linear_act_workspace_bytes(int M, int N, int K, int x_aligned, int w_aligned, int residual_aligned);
 int strata_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const float* bias, const void* residual,
                       int64_t ldr, void* y, int64_t ldy, void* preact, int64_t ldz, int M, int N, int K, int activation,
@@ -303,14 +304,14 @@ int strata_qk_norm_rows_bf16(void* qkv, int64_t ld, int64_t M, int C, float eps,
 
 /* Per-head RMS norm and rotation of q and k in one pass: y = R (x (mean x^2 + eps)^-1/2 w), eps >= 0, for M tokens of
  * heads_q and heads_k heads of head_dim channels (a multiple of 8, at most 256) in one 16-bit type. Element (m, head,
- * c) of an operand lies at base + m*st + head*sh + c; strides in elements, multiples of 8, bases 16-byte aligned. w_q, w_k:
- * [head_dim] fp32, 16-byte aligned, or NULL. R turns the first `rot` channels of a head by the (cos, sin) pairs of the
- * token's row of table [table_rows, rot/2] (IEEE half, or float with table_f32; 16-byte aligned; NULL: no rotation):
- * pairs (2i, 2i+1) with `adjacent`, rot a multiple of 8, else (i, i + rot/2), rot a multiple of 16. The row is
+ * c) of an operand lies at base + m*st + head*sh + c; strides in elements, multiples of 8, bases 16-byte aligned. w_q,
+ * w_k: [head_dim] fp32, 16-byte aligned, or NULL. R turns the first `rot` channels of a head by the (cos, sin) pairs of
+ * the token's row of table [table_rows, rot/2] (IEEE half, or float with table_f32; 16-byte aligned; NULL: no
+ * rotation): pairs (2i, 2i+1) with `adjacent`, rot a multiple of 8, else (i, i + rot/2), rot a multiple of 16. The row is
  * positions[m] (int32, or int64 with positions_64); without positions m / tokens_per_tile * hw + m % hw, which has to
  * stay below table_rows. A negative position is padding: its outputs are zero. One behind the table gives NaN and
- * device status 107. y may be x. The q/k norm and rotation of strata_qkv_rope_bf16 and strata_qk_norm_rows_bf16 for
- * projections made elsewhere, with affine weights, shared key heads and other widths. */
+ * device status 107. y may be x; nothing else may overlap. The q/k norm and rotation of strata_qkv_rope_bf16 and
+ * strata_qk_norm_rows_bf16 for projections made elsewhere, with affine weights, shared key heads and other widths. */
 int strata_qk_norm_rope(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh, void* yq,
                         int64_t yq_st, int64_t yq_sh, void* yk, int64_t yk_st, int64_t yk_sh, const float* w_q,
                         const float* w_k, int heads_q, int heads_k, int head_dim, int rot, int adjacent,

@@ -15,7 +15,7 @@ A case is a dict of plain values with a "kind":
   halo       the field-space halo exchange: pad the tiles of a sphere (copied or interpolated
              halo), and un-pad by windowed overlap-add
 
-Everything is inference (the library has no backward pass); tokens are bf16, fields fp32.
+Everything here is inference; tokens are bf16, fields fp32.
 Weights and inputs are drawn from the seed on the GPU; what depends on the geometry alone (halo
 plans, RoPE delta tables, peer buffers) is built once per geometry and kept, as a program
 that steps one grid keeps it.

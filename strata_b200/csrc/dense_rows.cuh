@@ -254,8 +254,10 @@ __global__ void __launch_bounds__(256) dense_align_rows_kernel(const AlignRows a
 
 // ---------------------------------------------------------------- dz = dy act'(z), and its column sums
 // HBM-bound: reads dy and z, writes dz (act = none: reads dy, and writes it only where the products need aligned
-// rows). A thread keeps its eight columns over all rows of the block, so the sums cost no extra read; the blocks' sums
-// (fp32, of dz before it is rounded) are added up in a fixed order by dense_finish_kernel.
+// rows). dz is rounded to the 16-bit type, which the tensor cores read: a second half of its digits would be a second
+// product each for dx and dW (1024 x 512, K = 128: 0.24 % off 64 bits, 0.17 % with dz in 32). A thread keeps its eight
+// columns over all rows of the block, so the sums cost no extra read; the blocks' sums (fp32, of dz before it is
+// rounded) are added up in a fixed order by dense_finish_kernel.
 struct SlopeParams {
   const void* dy;  long long ldy;
   const void* z;   long long ldz;       // nullptr: act is none

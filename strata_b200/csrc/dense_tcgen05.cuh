@@ -13,8 +13,7 @@
 //             DENSE_PART: fp32 partial sums of a split contraction (DensePlan), which dense_finish_kernel adds up
 //             with the same epilogue.
 //   widths    Rows of y and z that TMA cannot store (it writes whole 16-byte pieces) are copied from the staging boxes
-// by
-//             the warps.
+//             by the warps.
 #pragma once
 #include "dense_common.cuh"
 #include "gemm_tcgen05.cuh"

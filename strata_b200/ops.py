@@ -236,9 +236,9 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
                residual: torch.Tensor | None = None, *, save_preact: bool = False, out: torch.Tensor | None = None):
     """y = residual + act(z), z = x @ weight.T + bias, in one pass: x [..., K], weight [N, K], residual and y [..., N] of
     one type (bfloat16 or float16), bias [N] fp32; activation one of "none", "gelu" (erf), "gelu_tanh", "silu", "relu".
-    Any number of rows, any widths from one on, any row strides. Sums and the epilogue are fp32, y is rounded once. Where
-    N is no multiple of eight the results are views of rows that are (not contiguous): the next call reads them without
-    a copy.
+    Any number of rows, any widths from one on, any row strides. Sums and the epilogue are fp32, y is rounded once.
+    Where N is no multiple of eight the results are views of rows that are (not contiguous): the next call reads them
+    without a copy.
 
     save_preact: returns (y, z); linear_act_backward needs z for any activation but "none". out: where y goes, [M, N]
     with unit inner stride; it may be the residual, and shares no memory with an operand otherwise. The gradients are
@@ -846,7 +846,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
     of rot (a multiple of 16). A token's row: positions [tokens] (int32 / int64; negative: a padding token, its outputs
     are zero; one behind the table gives NaN and device status 107), else as in qkv_rope
     m // tokens_per_tile * hw + m % hw (default: token m has row m). out: (q', k') to write to, q and k themselves
-    allowed (in this order), other memory of an operand not. The gradients are qk_norm_rope_backward's; torch.ops.strata_b200.qk_norm_rope is the differentiable form."""
+    allowed (in this order), other memory of an operand not. The gradients are qk_norm_rope_backward's;
+    torch.ops.strata_b200.qk_norm_rope is the differentiable form."""
     dtype = _require_16bit(q, "q")
     hq, hk, hd, M, keep, args = _qk_arguments(q, k, q_weight, k_weight, rope_cs, positions, tokens_per_tile, hw,
                                               interleaved, eps)
@@ -865,7 +866,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
         own = ((yq.data_ptr(), yq_token, yq_head) == (q3.data_ptr(), q_token, q_head),
                (yk.data_ptr(), yk_token, yk_head) == (k3.data_ptr(), k_token, k_head))
         if _meet(*ys) or any(not own[j] and _meet(ys[i], xs[j]) for i in (0, 1) for j in (0, 1)):
-            raise ValueError("out may be q and k themselves, each its own, and shares no other memory with them or in itself")
+            raise ValueError("out may be q and k themselves, in this order, but not share other memory with them")
         if any(t is not None and _meet(y, _span(t.data_ptr(), t.numel() * t.element_size())) for y in ys for t in keep):
             raise ValueError("out may not share memory with the weights, rope_cs or positions")
     wq, wk = keep[:2]
